@@ -50,6 +50,8 @@ typedef enum {
 } ternocl_status;
 
 typedef enum { TERNOCL_FP16 = 0, TERNOCL_BF16 = 1 } ternocl_dtype;
+/* fp32, taken where an entry says so (logits, routing weights) beside the two above. */
+#define TERNOCL_FP32 2
 
 /* Workspaces.  Every entry that takes a device scratch (ws, ws_bytes) keeps
  * the same first TERNOCL_WS_HEADER_BYTES of it for its cross-workgroup
@@ -474,6 +476,83 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
                                                int T, int E, int topk, int H, int I, const uint32_t *Bg,
                                                const void *Sg, const uint32_t *Bu, const void *Su,
                                                const uint32_t *Bd, const void *Sd, void *O, void *stream);
+
+/* ---- int4 GEMV / GEMM ---------------------------------------------------------
+ * Products with 4-bit weights and group scales, for the projections that a model
+ * of ternary layers keeps at 4 bits, its head first (no reference counterpart; the
+ * tensors, epilogues and workspace are those of ternocl_int2_fp16_upcvt_gemm):
+ *   C[m,n] = ct(epi(sum_g S[g,n] * sum_{k in g} A[m,k] * (q(B[k,n]) - Z[g,n])))
+ *   B    : uint32 [K/32][N][4], 16 bytes for 32 rows of a column.  Word w of (kb, n)
+ *          holds rows 32 kb + 8 w .. + 7 as signed 4-bit values -8..7, row 2i in
+ *          nibble i (bits 4i..4i+3), row 2i + 1 in nibble i + 4 (i = 0..3)
+ *   group: rows per scale, 32, 64 or 128
+ *   S    : DT [K/group, N] scales;  Z: DT [K/group, N] zero points, any finite
+ *          value (NULL: 0)
+ * Codes, activations and zero points are multiplied as they are and summed in fp32
+ * (or exact integers) per group; nothing is rounded to DT before the epilogue.  A
+ * row of A that holds an infinity or a NaN gives infinities or NaN.
+ * N % 16 == 0, K % 128 == 0, any M >= 1.  B starts on 16 bytes.  M <= 8 runs the
+ * decode GEMV and larger M the matrix-core GEMM where the other operands are
+ * 16-byte aligned too, a plain kernel otherwise.
+ * ws / ws_bytes: optional device scratch of ternocl_int4_gemm_ws_bytes(M, N, K,
+ * group) bytes (0: none used), 16-byte aligned, laid out and used as
+ * ternocl_int2_fp16_upcvt_gemm's: a deterministic K split of few tiles over a long
+ * K, fp32 slice sums added in slice order; its counters take any contents.  NULL
+ * or short: unsplit. */
+size_t ternocl_int4_gemm_ws_bytes(int M, int N, int K, int group);
+ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z,
+                                 void *C, const void *Other, const void *Bias, int M, int N, int K, int group,
+                                 int postop, int out_f32, void *ws, size_t ws_bytes, void *stream);
+/* Host packers of that format (CPU; no GPU call): W int8 [K, N] row-major, values
+ * -8..7 (any other: TERNOCL_ERR_INVALID_ARG); K % 32 == 0. */
+ternocl_status ternocl_int4_pack(const int8_t *W, uint32_t *B, int K, int N);
+ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
+
+/* ---- MoE routing -----------------------------------------------------------------
+ * The experts and weights of each token from its router logits, as the MoE entries
+ * take them (ids int32 [T, topk], RW [T, topk]; no reference counterpart):
+ *   s[e]  = softmax(logits)[e] (score 0) or 1 / (1 + exp(-logits[e])) (score 1)
+ *   v[e]  = s[e] + bias[e] (bias fp32 [E], NULL: none): what experts are chosen by
+ *   groups of E / n_group experts in a row: a group's value is the sum of its
+ *     group_best (1 or 2) largest v; the topk_group groups of the largest values
+ *     stay (n_group == topk_group: all)
+ *   ids   = the topk largest v among them, in falling order (equal values: the
+ *           lowest index first, groups too)
+ *   RW    = scale * s[ids], with renorm divided by the sum of the chosen s first
+ * Choices are made on v as in 64-bit arithmetic; sums and weights are fp64,
+ * rounded to fp32, then to wtype.  An expert whose logit or v is -inf is never chosen and
+ * adds nothing to its group's value; slots left without an expert get id -1 and
+ * weight 0 (which the MoE entries skip).  A group without experts to choose counts
+ * as -inf.  A NaN ranks first, and a softmax row with a NaN or +inf logit has NaN
+ * weights.  Weights whose sum is 0 renormalise to 0.
+ * logits: ltype [T, E] (TERNOCL_FP16, _BF16 or _FP32) with ld elements from row to
+ * row (ld >= E); wtype: the same three.
+ * T >= 1, 1 <= E <= 512, 1 <= n_group <= 64 dividing E, 1 <= topk_group <= n_group,
+ * group_best <= E / n_group, 1 <= topk <= min(64, topk_group * E / n_group). */
+ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const float *bias, int *ids, int wtype,
+                                void *RW, int T, int E, int topk, int score, int n_group, int topk_group,
+                                int group_best, int renorm, float scale, void *stream);
+
+/* ---- log probabilities --------------------------------------------------------------
+ * Of the rows of logits that a head writes (fp32 with out_f32, or DT), under the
+ * distribution p = softmax(scale * logits) over V entries:
+ *   logp[m]    = ln p[m, tokens[m]]: 0 where tokens[m] is outside [0, V) (padding)
+ *   entropy[m] = -sum_v p ln p
+ *   top_ids / top_logp [m, topn]: the topn largest entries in falling order (equal
+ *                logits: the lowest index first) and their ln p
+ * all fp32 (ids int32).  tokens / logp, entropy and top_ids / top_logp may each be
+ * NULL (top: with topn 0).  An entry of -inf has p = 0 and is not listed; slots left
+ * over get id -1 and -inf.  A row of -inf alone gives logp -inf, entropy 0, ids -1; a
+ * row with a NaN or +inf gives NaN, ids -1.
+ * logits: ltype [M, V] with ld elements from row to row (ld >= V), its rows at any
+ * element alignment.  M >= 1, V >= 1, 0 <= topn <= 64, scale > 0 and finite.
+ * ws: optional scratch of ternocl_logprobs_ws_bytes(M, V, topn) bytes (0: none used),
+ * 16-byte aligned: rows are spread over workgroups where there are few.  NULL or
+ * short: one workgroup a row.  The same results, to rounding, either way. */
+size_t ternocl_logprobs_ws_bytes(int M, int V, int topn);
+ternocl_status ternocl_logprobs(int ltype, const void *logits, int64_t ld, const int *tokens, float *logp,
+                                float *entropy, int *top_ids, float *top_logp, int M, int V, int topn, float scale,
+                                void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -29,9 +29,10 @@ __all__ = [
     "hadamard_fwht",
     "moe_tile_rows", "int2_moe_route", "int2_moe_gather", "int2_moe_gemm", "int2_moe_combine",
     "int2_moe_prefill_ws_bytes", "int2_moe_prefill", "int2_moe_prefill_int8_ws_bytes", "int2_moe_prefill_int8",
+    "int4_gemm", "int4_gemm_ws_bytes", "int4_pack", "int4_unpack", "moe_topk", "logprobs", "logprobs_ws_bytes",
 ]
 
-FP16, BF16 = 0, 1
+FP16, BF16, FP32 = 0, 1, 2  # (FP32: logits and routing weights)
 # TERNOCL_WS_HEADER_BYTES: the front of every workspace, where the K splits keep
 # their counters (zero between calls); all other workspace data lies after it.
 WS_HEADER_BYTES = 64 << 10
@@ -105,6 +106,12 @@ def _dtype_of(t) -> int:
     if t.dtype == torch.bfloat16:
         return BF16
     raise TernoclError(1, f"activations must be float16 or bfloat16, got {t.dtype}")
+
+
+def _float_type(t) -> int:
+    """The type of a tensor that may be fp32 too (logits, routing weights)."""
+    import torch
+    return FP32 if t.dtype == torch.float32 else _dtype_of(t)
 
 
 def _nbytes(t) -> int:
@@ -430,3 +437,73 @@ def int2_moe_decode(X, ids, RW, T: int, E: int, topk: int, H: int, I: int, Bg, S
     _check(lib().ternocl_int2_moe_decode(_dtype_of(X), _ptr(X), _ptr(ids), _ptr(RW), T, E, topk, H, I,
                                          _ptr(Bg), _ptr(Sg), _ptr(Bu), _ptr(Su), _ptr(Bd), _ptr(Sd), _ptr(O),
                                          _ptr(ws), _nbytes(ws), _stream(stream)))
+
+
+# ---- int4: 4-bit weights with group scales (no reference counterpart) --------------------
+
+def int4_gemm_ws_bytes(M: int, N: int, K: int, group: int = 128) -> int:
+    """Workspace bytes of ``int4_gemm`` (0 when none is used)."""
+    return lib().ternocl_int4_gemm_ws_bytes(M, N, K, group)
+
+
+def int4_gemm(A, B, S, Z, C, Other, Bias, M: int, N: int, K: int, group: int = 128, postop: int = 0,
+              out_f32: bool = False, ws=None, stream=None) -> None:
+    """C = ct(epi(A x ((q - Z) S))): B int32 [K/32, N, 4] of ``int4_pack``, scales S and zero points Z
+    (None: 0) [K/group, N] in A's dtype, the epilogues of ``int2_fp16_upcvt_gemm``.  ``ws``
+    (int4_gemm_ws_bytes, 16-byte aligned): the K split of few tiles over a long K."""
+    _check(lib().ternocl_int4_gemm(_dtype_of(A), _ptr(A), _ptr(B), _ptr(S), _ptr(Z), _ptr(C), _ptr(Other), _ptr(Bias),
+                                   M, N, K, group, postop, int(bool(out_f32)), _ptr(ws), _nbytes(ws), _stream(stream)))
+
+
+def int4_pack(W):
+    """int8 [K, N], values -8..7 -> B uint32 [K/32, N, 4] (ternocl_int4_pack, on the host)."""
+    import numpy as np
+    W = _host_i8(W)
+    K, N = W.shape
+    B = np.empty((K // 32, N, 4), np.uint32)
+    _check(lib().ternocl_int4_pack(_cptr(W), _cptr(B), K, N))
+    return B
+
+
+def int4_unpack(B, K: int):
+    """B uint32 [K/32, N, 4] -> int8 [K, N] (ternocl_int4_unpack, on the host)."""
+    import numpy as np
+    B = np.ascontiguousarray(B, dtype=np.uint32)
+    W = np.empty((K, B.shape[1]), np.int8)
+    _check(lib().ternocl_int4_unpack(_cptr(B), _cptr(W), K, B.shape[1]))
+    return W
+
+
+# ---- routing and log probabilities (no reference counterpart) ------------------------------
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_topk(logits, bias, ids, RW, T: int, E: int, topk: int, score: str = "softmax", n_group: int = 1,
+             topk_group: int = 1, group_best: int = 1, renorm: bool = True, scale: float = 1.0, ld=None,
+             stream=None) -> None:
+    """ids int32 [T, topk] and weights RW [T, topk] of the experts that router logits [T, E] choose, as the
+    MoE calls take them: scores softmax or sigmoid, chosen by score + bias (fp32 [E] or None) within the
+    topk_group best of n_group groups (valued by their group_best largest), the weights renormalised or as
+    they are, times scale.  logits and RW: fp16, bf16 or fp32; ld: elements from row to row (E)."""
+    if score not in _SCORES:
+        raise TernoclError(1, f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    _check(lib().ternocl_moe_topk(_float_type(logits), _ptr(logits), E if ld is None else ld, _ptr(bias), _ptr(ids),
+                                  _float_type(RW), _ptr(RW), T, E, topk, _SCORES[score], n_group, topk_group, group_best,
+                                  int(bool(renorm)), scale, _stream(stream)))
+
+
+def logprobs_ws_bytes(M: int, V: int, topn: int = 0) -> int:
+    """Workspace bytes of ``logprobs`` (0 when none is used)."""
+    return lib().ternocl_logprobs_ws_bytes(M, V, topn)
+
+
+def logprobs(logits, tokens, logp, entropy, top_ids, top_logp, M: int, V: int, ld=None, topn: int = 0,
+             scale: float = 1.0, ws=None, stream=None) -> None:
+    """Of softmax(scale * logits) over rows of V entries (ld elements from row to row): logp fp32 [M] of
+    tokens int32 [M] (0 outside [0, V)), entropy fp32 [M], and the topn largest entries, top_ids int32 and
+    top_logp fp32 [M, topn].  tokens and logp, entropy, or the alternatives may be None.  ``ws``
+    (logprobs_ws_bytes): spreads few rows over workgroups."""
+    _check(lib().ternocl_logprobs(_float_type(logits), _ptr(logits), V if ld is None else ld, _ptr(tokens), _ptr(logp),
+                                  _ptr(entropy), _ptr(top_ids), _ptr(top_logp), M, V, topn, scale, _ptr(ws), _nbytes(ws),
+                                  _stream(stream)))

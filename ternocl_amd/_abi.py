@@ -72,6 +72,13 @@ SYMBOLS: dict[str, tuple] = {
     "ternocl_int2_moe_prefill_int8": (I, [I, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, Z, P]),
     "ternocl_int2_moe_decode_ws_bytes": (Z, [I, I, I, I]),
     "ternocl_int2_moe_decode": (I, [I, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, Z, P]),
+    "ternocl_int4_gemm_ws_bytes": (Z, [I, I, I, I]),
+    "ternocl_int4_gemm": (I, [I, P, P, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
+    "ternocl_int4_pack": (I, [P, P, I, I]),
+    "ternocl_int4_unpack": (I, [P, P, I, I]),
+    "ternocl_moe_topk": (I, [I, P, C.c_int64, P, P, I, P, I, I, I, I, I, I, I, I, C.c_float, P]),
+    "ternocl_logprobs_ws_bytes": (Z, [I, I, I]),
+    "ternocl_logprobs": (I, [I, P, C.c_int64, P, P, P, P, P, I, I, I, C.c_float, P, Z, P]),
     "ternocl_int2_moe_decode_noalloc": (I, [I, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P]),
 }
 

@@ -148,6 +148,19 @@ ternocl_status moe_decode_noalloc_run(int dtype, const void *X, const int *ids, 
                                       int topk, int H, int I, const uint32_t *Bg, const void *Sg,
                                       const uint32_t *Bu, const void *Su, const uint32_t *Bd, const void *Sd,
                                       void *O, hipStream_t st);
+// kernels (int4_plain.hip)
+ternocl_status int4_plain_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                              const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
+                              int out_f32, hipStream_t st);
+// kernels (moe_topk.hip)
+ternocl_status moe_topk_run(int ltype, const void *logits, long ld, const float *bias, int *ids, int wtype, void *RW,
+                            int T, int E, int topk, int score, int n_group, int topk_group, int group_best, int renorm,
+                            float scale, hipStream_t st);
+// kernels (logprobs.hip)
+size_t logprobs_ws_need(int M, int V, int topn);
+ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *tokens, float *logp, float *entropy,
+                            int *top_ids, float *top_logp, int M, int V, int topn, float scale, void *ws,
+                            size_t ws_bytes, hipStream_t st);
 // kernels (misc.hip)
 ternocl_status fill_zero_run(void *p, size_t bytes, hipStream_t st);
 
@@ -664,6 +677,73 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
                                     "call ternocl_int2_moe_decode with a workspace");
     return moe_decode_noalloc_run(dtype, X, ids, RW, T, E, topk, H, I, Bg, Sg, Bu, Su, Bd, Sd, O,
                                   (hipStream_t)stream);
+}
+
+// ---- int4 ------------------------------------------------------------------
+
+static bool int4_group(int group) { return group == 32 || group == 64 || group == 128; }
+
+size_t ternocl_int4_gemm_ws_bytes(int M, int N, int K, int group) {
+    if (M < 1 || N < 16 || N % 16 || K < kGS || K % kGS || !int4_group(group)) return 0;
+    return 0;
+}
+
+ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                                 const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
+                                 int out_f32, void *ws, size_t ws_bytes, void *stream) {
+    ternocl_status s = check_gemm_common(dtype, A, B, S, C, Other, Bias, M, N, K, postop, out_f32);
+    if (s != TERNOCL_OK) return s;
+    if (!int4_group(group)) FAIL(TERNOCL_ERR_INVALID_ARG, "group must be 32, 64 or 128");
+    if ((uintptr_t)B & 15) FAIL(TERNOCL_ERR_INVALID_ARG, "B must be 16-byte aligned");
+    return int4_plain_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
+}
+
+// ---- routing, log probabilities ------------------------------------------------
+
+static bool float_type(int t) { return t == TERNOCL_FP16 || t == TERNOCL_BF16 || t == TERNOCL_FP32; }
+
+ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const float *bias, int *ids, int wtype,
+                                void *RW, int T, int E, int topk, int score, int n_group, int topk_group,
+                                int group_best, int renorm, float scale, void *stream) {
+    if (!float_type(ltype) || !float_type(wtype))
+        FAIL(TERNOCL_ERR_INVALID_ARG, "ltype and wtype must be TERNOCL_FP16, TERNOCL_BF16 or TERNOCL_FP32");
+    if (!logits || !ids || !RW) FAIL(TERNOCL_ERR_INVALID_ARG, "logits, ids and RW must be non-null");
+    if (score != 0 && score != 1) FAIL(TERNOCL_ERR_INVALID_ARG, "score must be 0 (softmax) or 1 (sigmoid)");
+    if (renorm != 0 && renorm != 1) FAIL(TERNOCL_ERR_INVALID_ARG, "renorm must be 0 or 1");
+    if (!std::isfinite(scale)) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be finite");
+    if (T < 1 || E < 1 || E > 512) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need T >= 1 and 1 <= E <= 512");
+    if (ld < E) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ld must be at least E");
+    if (n_group < 1 || n_group > 64 || E % n_group) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "n_group must be 1..64 and divide E");
+    if (topk_group < 1 || topk_group > n_group) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "topk_group must be 1..n_group");
+    if (group_best < 1 || group_best > 2 || group_best > E / n_group)
+        FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "group_best must be 1 or 2 and at most E / n_group");
+    if (topk < 1 || topk > 64 || topk > topk_group * (E / n_group))
+        FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "topk must be 1..64 and at most topk_group * E / n_group");
+    return moe_topk_run(ltype, logits, (long)ld, bias, ids, wtype, RW, T, E, topk, score, n_group, topk_group, group_best,
+                        renorm, scale, (hipStream_t)stream);
+}
+
+size_t ternocl_logprobs_ws_bytes(int M, int V, int topn) {
+    if (M < 1 || V < 1 || topn < 0 || topn > 64) return 0;
+    return logprobs_ws_need(M, V, topn);
+}
+
+ternocl_status ternocl_logprobs(int ltype, const void *logits, int64_t ld, const int *tokens, float *logp,
+                                float *entropy, int *top_ids, float *top_logp, int M, int V, int topn, float scale,
+                                void *ws, size_t ws_bytes, void *stream) {
+    if (!float_type(ltype)) FAIL(TERNOCL_ERR_INVALID_ARG, "ltype must be TERNOCL_FP16, TERNOCL_BF16 or TERNOCL_FP32");
+    if (!logits) FAIL(TERNOCL_ERR_INVALID_ARG, "logits must be non-null");
+    if ((tokens == nullptr) != (logp == nullptr)) FAIL(TERNOCL_ERR_INVALID_ARG, "tokens and logp go together");
+    if (topn < 0 || topn > 64) FAIL(TERNOCL_ERR_INVALID_ARG, "topn must be 0..64");
+    if (topn && (!top_ids || !top_logp)) FAIL(TERNOCL_ERR_INVALID_ARG, "topn > 0 writes top_ids and top_logp: both must be non-null");
+    if (!logp && !entropy && !topn) FAIL(TERNOCL_ERR_INVALID_ARG, "nothing to compute: logp, entropy and topn are all absent");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be positive and finite");
+    if (M < 1 || V < 1) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "M and V must be positive");
+    if (ld < V) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ld must be at least V");
+    const uintptr_t es = ltype == TERNOCL_FP32 ? 4 : 2;
+    if ((uintptr_t)logits % es) FAIL(TERNOCL_ERR_INVALID_ARG, "logits must be aligned to its element");
+    return logprobs_run(ltype, logits, (long)ld, tokens, logp, entropy, top_ids, top_logp, M, V, topn, scale, ws, ws_bytes,
+                        (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -9,7 +9,8 @@
 //     streams, the sign streams (one bit per non-zero in k order, 1 = -1,
 //     column after column, each padded to whole words with zeros) and 4 zero
 //     pad words; slice ranks [ls-1][N] = non-zeros of column n in the bitmap
-//     words below s * ceil(K / ls) / 32 (common/bitcos.hpp:81-94).
+//     words below s * ceil(K / ls) / 32 (common/bitcos.hpp:81-94);
+//   * int4 (values -8..7): the layout of ternocl_int4_gemm.
 // Nothing here touches the GPU.
 #include <cstdint>
 #include <cstring>
@@ -57,6 +58,35 @@ void bitcos_presence(const int8_t *W, int K, int N, uint32_t *bitmap, std::vecto
 }  // namespace
 
 extern "C" {
+
+ternocl_status ternocl_int4_pack(const int8_t *W, uint32_t *B, int K, int N) {
+    if (!W || !B) FAIL(TERNOCL_ERR_INVALID_ARG, "W and B must be non-null");
+    if (N < 1 || K < 32 || K % 32) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need N >= 1 and K % 32 == 0");
+    for (size_t i = 0; i < (size_t)K * N; ++i)
+        if (W[i] < -8 || W[i] > 7) FAIL(TERNOCL_ERR_INVALID_ARG, "W must hold -8..7");
+    for (int kw = 0; kw < K / 8; ++kw)
+        for (int n = 0; n < N; ++n) {
+            uint32_t x = 0;
+            for (int r = 0; r < 8; ++r)  // row r of the word in nibble r / 2 (+ 4 where odd)
+                x |= (uint32_t)(W[(size_t)(8 * kw + r) * N + n] & 15) << (4 * (r / 2 + 4 * (r % 2)));
+            B[((size_t)(kw / 4) * N + n) * 4 + kw % 4] = x;
+        }
+    return TERNOCL_OK;
+}
+
+ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N) {
+    if (!W || !B) FAIL(TERNOCL_ERR_INVALID_ARG, "W and B must be non-null");
+    if (N < 1 || K < 32 || K % 32) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need N >= 1 and K % 32 == 0");
+    for (int kw = 0; kw < K / 8; ++kw)
+        for (int n = 0; n < N; ++n) {
+            const uint32_t x = B[((size_t)(kw / 4) * N + n) * 4 + kw % 4];
+            for (int r = 0; r < 8; ++r) {
+                const int q = (int)(x >> (4 * (r / 2 + 4 * (r % 2)))) & 15;
+                W[(size_t)(8 * kw + r) * N + n] = (int8_t)(q > 7 ? q - 16 : q);
+            }
+        }
+    return TERNOCL_OK;
+}
 
 ternocl_status ternocl_int2_pack(const int8_t *W, uint32_t *B, int K, int N) {
     if (!W || !B) FAIL(TERNOCL_ERR_INVALID_ARG, "W and B must be non-null");

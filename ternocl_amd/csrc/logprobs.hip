@@ -1,0 +1,497 @@
+// logprobs.hip -- log probabilities of given tokens, entropy and top alternatives of
+// rows of logits (ternocl_logprobs), in one pass over them.
+//
+//   d = scale * (l - max), r = sum e^d over all entries but one of the largest
+//   ln p = d - log1p(r),   H = log1p(r) - (sum d e^d) / (1 + r)
+//
+// (the largest entry's own term, 1, is left out of r: a peaked row's r may be far
+// below 2^-24, and 1 + r would lose it).
+//
+// The stream: a workgroup's 256 threads take 16-byte vectors in turn, kU of them in
+// flight per thread; a wave keeps one running maximum for its lanes, raised at most
+// once per batch of kU vectors (r and t = sum d e^d, in base 2, are scaled then).  What
+// bounds it is HBM; a few rows are spread over workgroups, whose sums meet in a second
+// launch.
+//
+// The alternatives: every thread also keeps the largest of each run of its vectors (a
+// "piece").  The topn-th largest of any 256 maxima of disjoint pieces is a bound that
+// at least topn entries reach, and only pieces whose maximum reaches it hold any:
+// those are read again, their entries at or above the bound (about topn of them where
+// values are spread) collected in LDS and ranked by (logit, lowest index).  Where more
+// than kCap reach it (many equal logits), a radix selection over the whole row first
+// finds the exact topn-th (value, index) key.
+#include "common.hpp"
+
+namespace tcl {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kU = 4;      // vectors in flight per thread
+constexpr int kPieces = 32;  // runs of batches per thread at most (LDS)
+constexpr int kCap = 1024; // candidates ranked in LDS
+
+template <int LT> struct LpVec {
+    static constexpr int NV = LT == TERNOCL_FP32 ? 4 : 8;  // entries of 16 bytes
+    static constexpr int ES = LT == TERNOCL_FP32 ? 4 : 2;
+};
+
+template <int LT> __device__ __forceinline__ void lp_unpack(const uint4 &v, float x[LpVec<LT>::NV]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (LT == TERNOCL_FP32) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[2 * i] = dt2f<LT == TERNOCL_BF16>(w[i] & 0xffffu);
+            x[2 * i + 1] = dt2f<LT == TERNOCL_BF16>(w[i] >> 16);
+        }
+    }
+}
+template <int LT> __device__ __forceinline__ float lp_load1(const void *row, int i) {
+    if constexpr (LT == TERNOCL_FP32) return ((const float *)row)[i];
+    else return dt2f<LT == TERNOCL_BF16>(((const uint16_t *)row)[i]);
+}
+
+// A row: `head` entries before its first 16-byte boundary, then nvec vectors, then the
+// rest.  Head and rest (at most 14 entries) are the "edge", entry e of it thread e's.
+template <int LT> struct LpRow {
+    const uint8_t *p;
+    int V, head, nvec, edge;
+    __device__ __forceinline__ LpRow(const void *logits, long ld, int m, int V_) : V(V_) {
+        constexpr int NV = LpVec<LT>::NV, ES = LpVec<LT>::ES;
+        p = (const uint8_t *)logits + (size_t)m * ld * ES;
+        head = min(V, (int)((16 - ((uintptr_t)p & 15)) & 15) / ES);
+        nvec = (V - head) / NV;
+        edge = V - NV * nvec;
+    }
+    __device__ __forceinline__ int edge_index(int e) const { return e < head ? e : e + LpVec<LT>::NV * nvec; }
+    __device__ __forceinline__ uint4 vec(int i) const {
+        return *(const uint4 *)(p + (size_t)head * LpVec<LT>::ES + 16 * (size_t)i);
+    }
+};
+
+__device__ __forceinline__ float lp_wave_max(float v, int lane) {
+    v = fmaxf(v, lane_xor<1>(v, lane));
+    v = fmaxf(v, lane_xor<2>(v, lane));
+    v = fmaxf(v, lane_xor<4>(v, lane));
+    v = fmaxf(v, lane_xor<8>(v, lane));
+    v = fmaxf(v, lane_xor<16>(v, lane));
+    return fmaxf(v, lane_xor<32>(v, lane));
+}
+__device__ __forceinline__ float lp_wave_sum(float v, int lane) {
+    v += lane_xor<1>(v, lane);
+    v += lane_xor<2>(v, lane);
+    v += lane_xor<4>(v, lane);
+    v += lane_xor<8>(v, lane);
+    v += lane_xor<16>(v, lane);
+    return v + lane_xor<32>(v, lane);
+}
+
+// Sums of a set of entries: largest m (-inf: none above -inf), r and t as above, t in
+// base 2 (sum of e2 2^e2, e2 = d log2 e).  A NaN anywhere makes r NaN.
+struct LpSum {
+    float m, r, t;
+};
+// a and b together; c = scale * log2 e.
+__device__ __forceinline__ LpSum lp_join(LpSum a, LpSum b, float c) {
+    if (b.m > a.m) {
+        const LpSum x = a;
+        a = b;
+        b = x;
+    }
+    LpSum o = a;
+    if (b.m == -__builtin_inff()) {  // nothing in b (or a NaN in its r)
+        o.r += b.r;
+        return o;
+    }
+    const float d = (b.m - a.m) * c, f = __builtin_amdgcn_exp2f(d);
+    o.r += f * (1.0f + b.r);
+    if (f > 0.0f) o.t += f * (b.t + d * (1.0f + b.r));
+    return o;
+}
+
+// One entry's terms: (2^e2, e2 2^e2).
+__device__ __forceinline__ void lp_term(float x, float m, float c, float &r, float &t) {
+    const float d = (x - m) * c, e = __builtin_amdgcn_exp2f(d);
+    r += e;
+    t += e > 0.0f ? d * e : 0.0f;
+}
+
+// A wave's running sums: m uniform, r and t a lane's part of the sums relative to m.
+struct LpState {
+    float m, r, t;
+    __device__ __forceinline__ void init() {
+        m = -__builtin_inff();
+        r = t = 0.0f;
+    }
+    // n entries of each lane (padding: -inf) whose lane maximum is tm
+    template <int n> __device__ __forceinline__ void add(const float (&x)[n], float tm, float c, int lane) {
+        const float wm = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(lp_wave_max(tm, lane))));
+        if (wm > m) {  // (uniform) a new maximum: one of its entries is left out below
+            if (m != -__builtin_inff()) {
+                // the lanes' sums so far, and the old maximum's own term in lane 0
+                const float d = (m - wm) * c, f = __builtin_amdgcn_exp2f(d);
+                const float old = r + (lane == 0 ? 1.0f : 0.0f);
+                t = f > 0.0f ? f * (t + d * old) : 0.0f;
+                r = f * old;
+            }
+            m = wm;
+            const bool skip = lane == __builtin_ctzll(__ballot(tm == wm));
+            bool done = !skip;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                if (!done && x[i] == wm) done = true;
+                else lp_term(x[i], m, c, r, t);
+            }
+            return;
+        }
+        if (m == -__builtin_inff()) {  // only -inf so far (or NaN: its r must show it)
+#pragma unroll
+            for (int i = 0; i < n; ++i) r += x[i] != x[i] ? x[i] : 0.0f;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < n; ++i) lp_term(x[i], m, c, r, t);
+    }
+};
+
+// Streams vectors [v0, v1) of a row (and, with edge, its edge entries) through this
+// workgroup; pm[p * 256 + tid] = the largest entry of thread tid's piece p (batches of
+// 256 kU vectors, bpp in a piece; the edge belongs to piece 0).  Returns each wave's
+// sums in LDS ws[wave] after a barrier.
+template <int LT, bool TOP>
+__device__ __forceinline__ void lp_stream(const LpRow<LT> &row, int v0, int v1, bool edge, int bpp, float c, float *pm,
+                                          LpSum *wsum) {
+    constexpr int NV = LpVec<LT>::NV;
+    const int tid = threadIdx.x, lane = tid & 63;
+    LpState st;
+    st.init();
+    float piece = -__builtin_inff();
+    if (edge && __builtin_amdgcn_readfirstlane(tid) < 64) {
+        float x[1] = {-__builtin_inff()};
+        if (tid < row.edge) x[0] = lp_load1<LT>(row.p, row.edge_index(tid));
+        piece = fmaxf(x[0], -__builtin_inff());
+        st.add(x, piece, c, lane);
+    }
+    int b = 0, p = 0;
+    for (int v = v0; v < v1; v += kThreads * kU) {
+        uint4 raw[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int i = v + u * kThreads + tid;
+            raw[u] = row.vec(min(i, v1 - 1));
+        }
+        float x[kU * NV];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float y[NV];
+            lp_unpack<LT>(raw[u], y);
+            const bool in = v + u * kThreads + tid < v1;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) x[u * NV + i] = in ? y[i] : -__builtin_inff();
+        }
+        float tm = x[0];
+#pragma unroll
+        for (int i = 1; i < kU * NV; ++i) tm = fmaxf(tm, x[i]);
+        tm = fmaxf(tm, -__builtin_inff());
+        st.add(x, tm, c, lane);
+        if constexpr (TOP) {
+            piece = fmaxf(piece, tm);
+            if (++b == bpp) {
+                pm[p * kThreads + tid] = piece;
+                piece = -__builtin_inff();
+                b = 0;
+                ++p;
+            }
+        }
+    }
+    if constexpr (TOP) {
+        if (b || p == 0) pm[p * kThreads + tid] = piece;
+    }
+    const float r = lp_wave_sum(st.r, lane), t = lp_wave_sum(st.t, lane);
+    if (lane == 0) wsum[tid >> 6] = LpSum{st.m, r, t};
+    __syncthreads();
+}
+
+struct LpArgs {
+    const void *logits;
+    long ld;
+    const int *tokens;
+    float *logp, *entropy;
+    int *top_ids;
+    float *top_logp;
+    int M, V, topn;
+    float scale;
+    int chunks, chunk_vecs;  // of the split launch
+    LpSum *sums;             // [M][chunks] (workspace)
+    float *maxima;           // [M][chunks][256] (workspace)
+};
+
+__device__ __forceinline__ u64 lp_key(float v, int i) {  // larger: before (v not NaN)
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return ((u64)(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u)) << 32) | (uint32_t)~i;
+}
+__device__ __forceinline__ float lp_key_value(u64 k) {
+    const uint32_t h = (uint32_t)(k >> 32);
+    return __uint_as_float(h & 0x80000000u ? h ^ 0x80000000u : ~h);
+}
+
+struct LpLds {
+    float sorted[kThreads];
+    u64 cand[kCap];
+    uint32_t hist[256];
+    int count;
+    float bound;
+    u64 key;
+    int need;
+};
+
+// Calls f(value, index) on every entry of the row, thread by thread.
+template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<LT> &row, F &&f) {
+    constexpr int NV = LpVec<LT>::NV;
+    const int tid = threadIdx.x;
+    if (tid < row.edge) {
+        const int i = row.edge_index(tid);
+        f(lp_load1<LT>(row.p, i), i);
+    }
+    for (int v = tid; v < row.nvec; v += kThreads) {
+        float y[NV];
+        lp_unpack<LT>(row.vec(v), y);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) f(y[i], row.head + v * NV + i);
+    }
+}
+
+// The row's outputs from its sums and its pieces' maxima: pm [chunks][pieces][256],
+// chunk k's thread t piece p = batches p bpp .. of vectors [k chunk_vecs, ...).
+template <int LT, bool TOP>
+__device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row, int m, const LpSum &s, const float *pm,
+                                          int chunks, int chunk_vecs, int pieces, int bpp, LpLds &L) {
+    constexpr int NV = LpVec<LT>::NV;
+    const int tid = threadIdx.x;
+    const bool empty = s.m == -__builtin_inff() && s.r == 0.0f;
+    const bool bad = !(s.r < __builtin_inff()) || s.m == __builtin_inff();
+    const float l1 = log1pf(s.r), nan = __builtin_nanf("");
+    if (tid == 0) {
+        if (a.logp) {
+            const int tok = a.tokens[m];
+            float o = 0.0f;
+            if (tok >= 0 && tok < a.V) {
+                const float x = lp_load1<LT>(row.p, tok);
+                o = bad ? nan : empty ? -__builtin_inff() : (x - s.m) * a.scale - l1;
+            }
+            a.logp[m] = o;
+        }
+        if (a.entropy)
+            a.entropy[m] = bad ? nan : empty ? 0.0f : l1 - s.t * 0.693147180559945309f / (1.0f + s.r);
+    }
+    if constexpr (!TOP) return;
+    int *ids = a.top_ids + (size_t)m * a.topn;
+    float *out = a.top_logp + (size_t)m * a.topn;
+    if (bad || empty) {  // (uniform)
+        if (tid < a.topn) {
+            ids[tid] = -1;
+            out[tid] = bad ? nan : -__builtin_inff();
+        }
+        return;
+    }
+    // the bound: the topn-th largest of the 256 threads' maxima
+    float v = -__builtin_inff();
+    for (int i = 0; i < chunks * pieces; ++i) v = fmaxf(v, pm[i * kThreads + tid]);
+    L.sorted[tid] = v;
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < kThreads; ++i) {
+        const float o = L.sorted[i];
+        rank += o > v || (o == v && i < tid);
+    }
+    if (rank == a.topn - 1) L.bound = v;
+    __syncthreads();
+    const float bound = L.bound;
+    auto take = [&](float x, int i) __attribute__((always_inline)) {
+        if (x >= bound && x > -__builtin_inff()) {
+            const int n = atomicAdd(&L.count, 1);
+            if (n < kCap) L.cand[n] = lp_key(x, i);
+        }
+    };
+    for (int k = 0; k < chunks; ++k) {
+        const int v1 = min(row.nvec, (k + 1) * chunk_vecs);
+        for (int p = 0; p < pieces; ++p) {
+            if (pm[(k * pieces + p) * kThreads + tid] < bound) continue;
+            if (k == 0 && p == 0 && tid < row.edge) {
+                const int i = row.edge_index(tid);
+                take(lp_load1<LT>(row.p, i), i);
+            }
+            const int b0 = k * chunk_vecs + p * bpp * kThreads * kU;
+            const int b1 = min(v1, b0 + bpp * kThreads * kU);
+            for (int w = b0 + tid; w < b1; w += kThreads) {
+                float y[NV];
+                lp_unpack<LT>(row.vec(w), y);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) take(y[i], row.head + w * NV + i);
+            }
+        }
+    }
+    __syncthreads();
+    int count = L.count;
+    if (count > kCap) {  // (uniform)
+        // the topn-th largest key, 8 bits at a time over the whole row
+        u64 prefix = 0;
+        int need = a.topn;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            L.hist[tid] = 0;
+            __syncthreads();
+            lp_scan<LT>(row, [&](float x, int i) __attribute__((always_inline)) {
+                const u64 k = lp_key(x, i);
+                if (x > -__builtin_inff() && (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))))
+                    atomicAdd(&L.hist[(k >> shift) & 255], 1u);
+            });
+            __syncthreads();
+            if (tid == 0) {
+                int b = 255, n = need;
+                while (b > 0 && (int)L.hist[b] < n) n -= (int)L.hist[b--];
+                L.key = prefix | ((u64)b << shift);
+                L.need = n;
+            }
+            __syncthreads();
+            prefix = L.key;
+            need = L.need;
+            __syncthreads();
+        }
+        if (tid == 0) L.count = 0;
+        __syncthreads();
+        lp_scan<LT>(row, [&](float x, int i) __attribute__((always_inline)) {
+            const u64 k = lp_key(x, i);
+            if (k >= prefix && x > -__builtin_inff()) {
+                const int n = atomicAdd(&L.count, 1);
+                if (n < kCap) L.cand[n] = k;
+            }
+        });
+        __syncthreads();
+        count = min(L.count, kCap);
+    }
+    for (int c = tid; c < count; c += kThreads) {
+        const u64 k = L.cand[c];
+        int before = 0;
+        for (int i = 0; i < count; ++i) before += L.cand[i] > k;
+        if (before < a.topn) {
+            ids[before] = (int)~(uint32_t)k;
+            out[before] = (lp_key_value(k) - s.m) * a.scale - l1;
+        }
+    }
+    for (int i = count + tid; i < a.topn; i += kThreads) {
+        ids[i] = -1;
+        out[i] = -__builtin_inff();
+    }
+}
+
+template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_row(const LpArgs a, int pieces, int bpp) {
+    __shared__ LpSum wsum[kWaves];
+    __shared__ float pm[TOP ? kPieces * kThreads : 1];
+    __shared__ std::conditional_t<TOP, LpLds, int> L;
+    const int m = blockIdx.x;
+    const LpRow<LT> row(a.logits, a.ld, m, a.V);
+    const float c = a.scale * 1.44269504088896341f;
+    if constexpr (TOP)
+        for (int p = 1; p < pieces; ++p) pm[p * kThreads + threadIdx.x] = -__builtin_inff();
+    lp_stream<LT, TOP>(row, 0, row.nvec, true, bpp, c, pm, wsum);
+    LpSum s = wsum[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
+    lp_finish<LT, TOP>(a, row, m, s, pm, 1, pieces * bpp * kThreads * kU, pieces, bpp, reinterpret_cast<LpLds &>(L));
+}
+
+template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_part(const LpArgs a) {
+    __shared__ LpSum wsum[kWaves];
+    const int m = blockIdx.y, k = blockIdx.x;
+    const LpRow<LT> row(a.logits, a.ld, m, a.V);
+    const float c = a.scale * 1.44269504088896341f;
+    const int v0 = min(k * a.chunk_vecs, row.nvec), v1 = min(row.nvec, v0 + a.chunk_vecs);
+    const size_t o = (size_t)m * a.chunks + k;
+    lp_stream<LT, TOP>(row, v0, v1, k == 0, a.chunk_vecs, c, a.maxima + o * kThreads, wsum);
+    if (threadIdx.x == 0) {
+        LpSum s = wsum[0];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
+        a.sums[o] = s;
+    }
+}
+
+template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_join(const LpArgs a) {
+    __shared__ std::conditional_t<TOP, LpLds, int> L;
+    __shared__ LpSum total;
+    const int m = blockIdx.x;
+    const LpRow<LT> row(a.logits, a.ld, m, a.V);
+    const float c = a.scale * 1.44269504088896341f;
+    if (threadIdx.x == 0) {
+        LpSum s = a.sums[(size_t)m * a.chunks];
+        for (int k = 1; k < a.chunks; ++k) s = lp_join(s, a.sums[(size_t)m * a.chunks + k], c);
+        total = s;
+    }
+    __syncthreads();
+    const LpSum s = total;
+    lp_finish<LT, TOP>(a, row, m, s, a.maxima + (size_t)m * a.chunks * kThreads, a.chunks, a.chunk_vecs, 1,
+                       a.chunk_vecs / (kThreads * kU), reinterpret_cast<LpLds &>(L));
+}
+
+// Workgroups a row is spread over: as many as whole batches give, while all rows stay
+// within about two workgroups a CU.
+// (nv: entries of a vector)
+int lp_chunks(int M, int V, int nv, int &chunk_vecs) {
+    const long batch = (long)kThreads * kU;
+    const long nb = V < nv ? 1 : ((long)V / nv + batch - 1) / batch;
+    long c = M >= 512 ? 1 : 512 / M;
+    if (c > nb) c = nb;
+    if (c < 1) c = 1;
+    const long per = (nb + c - 1) / c;
+    chunk_vecs = (int)(per * batch);
+    return (int)((nb + per - 1) / per);
+}
+
+}  // namespace
+
+size_t logprobs_ws_need(int M, int V, int topn) {
+    int cv;
+    const int c = lp_chunks(M, V, 4, cv);  // (16-bit rows have fewer)
+    return c == 1 ? 0 : kWsHeader + (size_t)M * c * (sizeof(LpSum) + (topn ? 4 * kThreads : 0));
+}
+
+ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *tokens, float *logp, float *entropy,
+                            int *top_ids, float *top_logp, int M, int V, int topn, float scale, void *ws,
+                            size_t ws_bytes, hipStream_t st) {
+    LpArgs a = {logits, ld, tokens, logp, entropy, top_ids, top_logp, M, V, topn, scale, 1, 0, nullptr, nullptr};
+    const int nv = ltype == TERNOCL_FP32 ? 4 : 8;
+    const size_t need = logprobs_ws_need(M, V, topn);
+    const bool split = need && ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0;
+    if (split) {
+        a.chunks = lp_chunks(M, V, nv, a.chunk_vecs);
+        a.sums = (LpSum *)((uint8_t *)ws + kWsHeader);
+        a.maxima = (float *)(a.sums + (size_t)M * a.chunks);
+    }
+    // pieces of the unsplit launch: at most kPieces runs of batches
+    const int nb = (V / nv + kThreads * kU - 1) / (kThreads * kU);
+    const int bpp = nb > kPieces ? (nb + kPieces - 1) / kPieces : 1, pieces = nb > 0 ? (nb + bpp - 1) / bpp : 1;
+    auto go = [&](auto lt, auto top) {
+        constexpr int LT = decltype(lt)::value;
+        constexpr bool TOP = decltype(top)::value;
+        if (split) {
+            hipLaunchKernelGGL((k_logprobs_part<LT, TOP>), dim3(a.chunks, M), dim3(kThreads), 0, st, a);
+            hipLaunchKernelGGL((k_logprobs_join<LT, TOP>), dim3(M), dim3(kThreads), 0, st, a);
+        } else {
+            hipLaunchKernelGGL((k_logprobs_row<LT, TOP>), dim3(M), dim3(kThreads), 0, st, a, pieces, bpp);
+        }
+    };
+    auto lt = [&](auto top) {
+        if (ltype == TERNOCL_FP32) go(std::integral_constant<int, TERNOCL_FP32>{}, top);
+        else if (ltype == TERNOCL_BF16) go(std::integral_constant<int, TERNOCL_BF16>{}, top);
+        else go(std::integral_constant<int, TERNOCL_FP16>{}, top);
+    };
+    if (topn) lt(std::true_type{});
+    else lt(std::false_type{});
+    return check_launch();
+}
+
+}  // namespace tcl

@@ -21,6 +21,10 @@ Operators (the reference kernels they stand for, as in the C ABI):
   moe_prefill       the int2 MoE prefill layer            (int2_moe/prefill.cpp:268-279)
   moe_decode        the int2 MoE decode layer             (int2_moe/int2_moe.cl:61-174)
   moe_prefill_int8  the int8 MoE prefill layer            (int2_moe/int2_moe_prefill_int8.cl)
+and, without a reference counterpart, what stands around those layers in a model:
+  int4_gemm         products with 4-bit weights and group scales (a head)
+  moe_topk          routing: router logits -> the MoE layers' ids and weights
+  logprobs          log probabilities, entropy and top alternatives of logits
 """
 from __future__ import annotations
 
@@ -30,7 +34,8 @@ import torch
 
 import ternocl_amd as T
 
-__all__ = ["int2_gemm", "quant_a", "int2_int8_gemm", "bitcos_gemm", "fwht", "moe_prefill", "moe_decode", "moe_prefill_int8"]
+__all__ = ["int2_gemm", "quant_a", "int2_int8_gemm", "bitcos_gemm", "fwht", "moe_prefill", "moe_decode", "moe_prefill_int8",
+           "int4_gemm", "moe_topk", "logprobs"]
 
 
 def _out_dtype(A: torch.Tensor, out_f32: bool) -> torch.dtype:
@@ -302,3 +307,126 @@ def moe_prefill_int8(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, E: in
 def _(X, ids, RW, E, Bg, Sg, Bu, Su, Bd, Sd):
     _chk_moe(X, ids, RW, E, Bg, Sg, Bu, Su, Bd, Sd)
     return torch.empty_like(X)
+
+
+# ---- the calls around those layers -----------------------------------------------------
+# They launch on the current stream of their tensors' device, whichever device is
+# current.  Their workspaces need no zeroing: one is allocated per call, so that a
+# captured graph keeps its own and two graphs, or two streams, never share one.
+
+def _scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+_LT = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _chk_int4(A, B, S, Z, group, other, bias, out_f32) -> None:
+    _chk_act(A)
+    M, K = A.shape
+    torch._check(B.dim() == 3, lambda: "B must be int32 [K/32, N, 4]")
+    torch._check(group in (32, 64, 128), lambda: "group must be 32, 64 or 128")
+    torch._check(K >= 128 and K % 128 == 0, lambda: "K must be a multiple of 128")
+    N = B.shape[1]
+    torch._check(N >= 16 and N % 16 == 0, lambda: "N must be a multiple of 16")
+    _chk(B, "B", torch.int32, (K // 32, N, 4), A.device)
+    _chk(S, "S", A.dtype, (K // group, N), A.device)
+    _chk(Z, "Z", A.dtype, (K // group, N), A.device)
+    _chk(other, "other", A.dtype, (M, N), A.device)
+    _chk(bias, "bias", _out_dtype(A, out_f32), (N,), A.device)
+
+
+@torch.library.custom_op("ternocl::int4_gemm", mutates_args=())
+def int4_gemm(A: torch.Tensor, B: torch.Tensor, S: torch.Tensor, Z: Optional[torch.Tensor], group: int,
+              other: Optional[torch.Tensor], bias: Optional[torch.Tensor], postop: int, out_f32: bool) -> torch.Tensor:
+    """C [M, N] = ct(epi(A x ((q - Z) S))); B int32 [K/32, N, 4] (int4_pack), S and Z [K/group, N] in A's dtype."""
+    _chk_int4(A, B, S, Z, group, other, bias, out_f32)
+    M, K = A.shape
+    N = B.shape[1]
+    C = torch.empty((M, N), dtype=_out_dtype(A, out_f32), device=A.device)
+    if M == 0:
+        return C
+    with torch.cuda.device(A.device):
+        ws = _scratch(A.device, T.int4_gemm_ws_bytes(M, N, K, group))
+        T.int4_gemm(A, B, S, Z, C, other, bias, M, N, K, group, postop, out_f32, ws=ws)
+    return C
+
+
+@int4_gemm.register_fake
+def _(A, B, S, Z, group, other, bias, postop, out_f32):
+    _chk_int4(A, B, S, Z, group, other, bias, out_f32)
+    return A.new_empty((A.shape[0], B.shape[1]), dtype=_out_dtype(A, out_f32))
+
+
+def _chk_rows(x: torch.Tensor, name: str) -> None:
+    """fp16, bf16 or fp32 [rows, n], each row's elements adjacent and rows in order, without overlap."""
+    torch._check(x.dim() == 2, lambda: f"{name} must be 2-D")
+    torch._check(x.dtype in _LT, lambda: f"{name}: dtype {x.dtype}, expected float16, bfloat16 or float32")
+    torch._check(x.shape[1] <= 1 or x.stride(1) == 1, lambda: f"{name}: a row's elements must be adjacent")
+    torch._check(x.shape[0] <= 1 or x.stride(0) >= x.shape[1], lambda: f"{name}: rows must not overlap")
+
+
+def _pitch(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _chk_topk(logits, bias, topk, dtype) -> None:
+    _chk_rows(logits, "logits")
+    torch._check(dtype in _LT, lambda: "dtype must be float16, bfloat16 or float32")
+    torch._check(1 <= topk <= 64, lambda: "topk must be 1..64")
+    _chk(bias, "bias", torch.float32, (logits.shape[1],), logits.device)
+
+
+@torch.library.custom_op("ternocl::moe_topk", mutates_args=())
+def moe_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], topk: int, dtype: torch.dtype, score: str, n_group: int,
+             topk_group: int, group_best: int, renorm: bool, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """(ids int32 [T, topk], RW [T, topk] in dtype) of router logits [T, E], as moe_prefill and moe_decode take them."""
+    _chk_topk(logits, bias, topk, dtype)
+    Tk, E = logits.shape
+    ids = torch.empty((Tk, topk), dtype=torch.int32, device=logits.device)
+    RW = torch.empty((Tk, topk), dtype=dtype, device=logits.device)
+    if Tk:
+        with torch.cuda.device(logits.device):
+            T.moe_topk(logits, bias, ids, RW, Tk, E, topk, score, n_group, topk_group, group_best, renorm, scale,
+                       ld=_pitch(logits))
+    return ids, RW
+
+
+@moe_topk.register_fake
+def _(logits, bias, topk, dtype, score, n_group, topk_group, group_best, renorm, scale):
+    _chk_topk(logits, bias, topk, dtype)
+    Tk = logits.shape[0]
+    return logits.new_empty((Tk, topk), dtype=torch.int32), logits.new_empty((Tk, topk), dtype=dtype)
+
+
+def _chk_logprobs(logits, tokens, topn) -> None:
+    _chk_rows(logits, "logits")
+    torch._check(0 <= topn <= 64, lambda: "topn must be 0..64")
+    _chk(tokens, "tokens", torch.int32, (logits.shape[0],), logits.device)
+
+
+@torch.library.custom_op("ternocl::logprobs", mutates_args=())
+def logprobs(logits: torch.Tensor, tokens: torch.Tensor, topn: int,
+             scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logp [M] of tokens int32 [M], entropy [M], top_ids int32 [M, topn], top_logp [M, topn]) of
+    softmax(scale * logits), logits [M, V] fp16, bf16 or fp32."""
+    _chk_logprobs(logits, tokens, topn)
+    M, V = logits.shape
+    d = logits.device
+    f = dict(dtype=torch.float32, device=d)
+    logp, entropy, top_logp = torch.empty(M, **f), torch.empty(M, **f), torch.empty((M, topn), **f)
+    top_ids = torch.empty((M, topn), dtype=torch.int32, device=d)
+    if M:
+        with torch.cuda.device(d):
+            T.logprobs(logits, tokens, logp, entropy, top_ids if topn else None, top_logp if topn else None, M, V,
+                       _pitch(logits), topn, scale, ws=_scratch(d, T.logprobs_ws_bytes(M, V, topn)))
+    return logp, entropy, top_ids, top_logp
+
+
+@logprobs.register_fake
+def _(logits, tokens, topn, scale):
+    _chk_logprobs(logits, tokens, topn)
+    M = logits.shape[0]
+    f = torch.float32
+    return (logits.new_empty(M, dtype=f), logits.new_empty(M, dtype=f), logits.new_empty((M, topn), dtype=torch.int32),
+            logits.new_empty((M, topn), dtype=f))

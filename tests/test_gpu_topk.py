@@ -1,0 +1,197 @@
+"""moe_topk on the GPU against the definition in 64 bits: ids equal, weights within the two roundings of the
+output (fp32, then its type: eps / 2 and 2^-24, relative) and 2^-40 for the fp64 exponentials."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+NAMES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def gold(logits, bias, topk, score, n_group, topk_group, group_best, renorm, scale):
+    """Row by row, in Python's own order of comparison: (-value, index)."""
+    ids, ws = [], []
+    per = logits.shape[1] // n_group
+    b = [0.0] * logits.shape[1] if bias is None else bias.double().tolist()
+    for row in logits.double().tolist():
+        if score == "softmax":
+            mx = max(row)
+            ex = [0.0 if x == -math.inf else math.exp(x - mx) for x in row]
+            tot = math.fsum(ex)
+            s = [e / tot if tot else 0.0 for e in ex]
+        else:
+            s = [1 / (1 + math.exp(-x)) if x > -700 else 0.0 for x in row]
+        v = [-math.inf if x == -math.inf else si + bi for x, si, bi in zip(row, s, b)]
+        order = [-math.inf if x == -math.inf else x for x in row] if bias is None else v
+        pool = range(len(row))
+        if topk_group < n_group:
+            src = v if group_best == 2 or bias is not None else order
+            gv = []
+            for g in range(n_group):
+                top = [x for x in sorted(src[g * per:(g + 1) * per], reverse=True)[:group_best] if x != -math.inf]
+                gv.append(sum(top) if top else -math.inf)
+            kept = sorted(range(n_group), key=lambda g: (-gv[g], g))[:topk_group]
+            pool = [e for e in pool if e // per in kept]
+        pick = sorted((e for e in pool if order[e] != -math.inf and v[e] != -math.inf), key=lambda e: (-order[e], e))[:topk]
+        w = [s[e] for e in pick]
+        if renorm:
+            t = math.fsum(w)
+            w = [x / t if t else 0.0 for x in w]
+        ids.append(pick + [-1] * (topk - len(pick)))
+        ws.append([x * scale for x in w] + [0.0] * (topk - len(pick)))
+    return torch.tensor(ids, dtype=torch.int32), torch.tensor(ws, dtype=torch.float64)
+
+
+def check(T, logits, bias, topk, wt, score="softmax", n_group=1, topk_group=1, group_best=1, renorm=True, scale=1.0, ld=None):
+    Tk, E = logits.shape
+    L = logits.cuda()
+    if ld:
+        buf = torch.full((Tk, ld), 99.0, dtype=logits.dtype, device="cuda")
+        buf[:, :E] = L
+        L = buf
+    ids = torch.full((Tk + 1, topk), 77, dtype=torch.int32, device="cuda")
+    RW = torch.full((Tk + 1, topk), 7.0, dtype=NAMES[wt], device="cuda")
+    T.moe_topk(L, None if bias is None else bias.cuda(), ids, RW, Tk, E, topk, score, n_group, topk_group, group_best, renorm,
+               scale, ld=ld)
+    torch.cuda.synchronize()
+    assert (ids[Tk] == 77).all() and (RW[Tk] == 7).all()
+    want, w = gold(logits, bias, topk, score, n_group, topk_group, group_best, renorm, scale)
+    assert torch.equal(ids[:Tk].cpu(), want)
+    got = RW[:Tk].cpu().double()
+    u = torch.finfo(NAMES[wt]).eps / 2
+    tiny = {"f16": 2.0**-25, "bf16": 2.0**-126, "f32": 2.0**-126}[wt]  # (subnormal weights)
+    assert ((got - w).abs() <= (u + 2.0**-24 + 2.0**-40) * w.abs() + tiny).all()
+
+
+def logits_of(seed, Tk, E, lt, sigma=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((Tk, E), generator=g) * sigma).to(NAMES[lt]), torch.randn(E, generator=g) * 0.1
+
+
+@pytest.mark.parametrize("E,topk", [(1, 1), (2, 2), (3, 1), (8, 2), (17, 5), (60, 4), (64, 8), (65, 8), (100, 10), (128, 8),
+                                    (200, 1), (256, 8), (257, 64), (384, 6), (512, 10), (512, 64)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_experts(dev, E, topk, score, biased):
+    import ternocl_amd as T
+    for i, lt in enumerate(NAMES):
+        x, b = logits_of(E + topk, 37, E, lt)
+        check(T, x, b if biased else None, topk, ("bf16", "f16", "f32")[i], score, renorm=i != 1, scale=(1.0, 2.5, 1.0)[i])
+
+
+@pytest.mark.parametrize("Tk", [1, 2, 3, 4, 5, 63, 1001])
+def test_tokens(dev, Tk):
+    import ternocl_amd as T
+    x, b = logits_of(Tk, Tk, 128, "bf16")  # (many equal logits)
+    check(T, x, None, 8, "bf16")
+    check(T, x, b, 8, "f32", "sigmoid", 8, 3, 2)
+
+
+@pytest.mark.parametrize("E,n_group,topk_group", [(64, 8, 4), (64, 8, 8), (256, 8, 4), (160, 8, 3), (512, 64, 7), (48, 3, 1),
+                                                  (64, 64, 32), (126, 9, 2)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("group_best", [1, 2])
+def test_groups(dev, E, n_group, topk_group, score, biased, group_best):
+    import ternocl_amd as T
+    if group_best > E // n_group:
+        pytest.skip("a group of one expert")
+    x, b = logits_of(E + n_group, 41, E, "f32")
+    check(T, x, b if biased else None, min(6, topk_group * (E // n_group)), "f32", score, n_group, topk_group, group_best, True, 2.5)
+
+
+def test_close_scores(dev):
+    """Scores closer than fp32 tells apart are ordered as in 64 bits; equal ones by index."""
+    import ternocl_amd as T
+    g = torch.Generator().manual_seed(1)
+    x = torch.full((64, 96), 3.0) + torch.randint(0, 4, (64, 96), generator=g) * 2.0**-22
+    check(T, x, None, 12, "f32")
+    check(T, x, None, 12, "f32", "sigmoid")
+    check(T, x, torch.randint(0, 3, (96,), generator=g) * 2.0**-25, 12, "f32", "sigmoid", 6, 3, 1)
+    check(T, torch.zeros(3, 40), None, 5, "f32")
+    check(T, torch.zeros(3, 40), torch.zeros(40), 5, "f32", "sigmoid", 4, 2, 2)
+    z = torch.zeros(2, 40)
+    z[:, ::2] = -0.0
+    check(T, z, None, 5, "f32")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_masks(dev, score, biased):
+    """Experts at -inf are never chosen; rows with few or none left end in -1 and 0; the type's lowest value
+    is a value like any other."""
+    import ternocl_amd as T
+    x, b = logits_of(3, 6, 64, "f32")
+    x[0] = -math.inf
+    x[1, 5:] = -math.inf
+    x[2, :60] = -math.inf
+    x[3] = torch.finfo(torch.float32).min
+    x[4, 1:] = torch.finfo(torch.float32).min
+    b = b if biased else None
+    check(T, x, b, 8, "f32", score)
+    check(T, x, b, 8, "bf16", score, renorm=False)
+    check(T, x[[0, 1, 2, 5]], b, 8, "f32", score, 8, 2, 2)
+    if biased:
+        b2 = b.clone()
+        b2[7:] = -math.inf
+        check(T, x[5:], b2, 8, "f32", score)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_not_finite(dev, bad):
+    """A NaN (softmax: an infinity too) makes its row's weights NaN and no other row's."""
+    import ternocl_amd as T
+    x, _ = logits_of(3, 3, 64, "f32")
+    x[1, 9] = bad
+    ids = torch.empty((3, 4), dtype=torch.int32, device="cuda")
+    w = torch.empty((3, 4), device="cuda")
+    for renorm in (False, True):
+        T.moe_topk(x.cuda(), None, ids, w, 3, 64, 4, "softmax", renorm=renorm)
+        assert torch.isnan(w[1]).all() and ids[1, 0] == 9 and torch.isfinite(w[[0, 2]]).all()
+        assert len(set(ids[1].tolist())) == 4
+        T.moe_topk(x.cuda(), None, ids, w, 3, 64, 4, "sigmoid", renorm=renorm)
+        assert ids[1, 0] == 9 and torch.isfinite(w[[0, 2]]).all()
+        if bad != bad:
+            assert torch.isnan(w[1, 0]) and (torch.isnan(w[1]).all() if renorm else torch.isfinite(w[1, 1:]).all())
+
+
+def test_pitch(dev):
+    import ternocl_amd as T
+    x, b = logits_of(3, 9, 60, "bf16")
+    check(T, x, b, 6, "f16", ld=61)
+    x, b = logits_of(3, 9, 128, "f32")
+    check(T, x, None, 6, "f16", ld=131)
+
+
+def test_op_graph_and_stream(dev):
+    import ternocl_amd as T
+    import ternocl_amd.torch_ops  # noqa: F401
+    op = torch.ops.ternocl.moe_topk
+    x = torch.randn(33, 256, device="cuda")
+    b = torch.randn(256, device="cuda") * 0.1
+    args = (8, torch.bfloat16, "sigmoid", 8, 4, 2, True, 2.5)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        op(x, b, *args)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            ids, w = op(x, b, *args)
+    for _ in range(3):
+        x.normal_()
+        i2, w2 = op(x, b, *args)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ids, i2) and torch.equal(w, w2)
+    v = x[:, :128]  # rows with a pitch
+    i1, w1 = op(v, None, 4, torch.float32, "softmax", 1, 1, 1, True, 1.0)
+    i2, w2 = op(v.contiguous(), None, 4, torch.float32, "softmax", 1, 1, 1, True, 1.0)
+    assert torch.equal(i1, i2) and torch.equal(w1, w2)
+    assert op(x[:0], None, 4, torch.float32, "softmax", 1, 1, 1, True, 1.0)[0].shape == (0, 4)
+    with pytest.raises(RuntimeError):
+        op(x, None, 4, torch.float32, "softmax", 7, 1, 1, True, 1.0)
+    torch.library.opcheck(op.default, (x, b, *args), test_utils=("test_schema", "test_faketensor"))
