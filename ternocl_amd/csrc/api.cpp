@@ -148,6 +148,11 @@ ternocl_status moe_decode_noalloc_run(int dtype, const void *X, const int *ids, 
                                       int topk, int H, int I, const uint32_t *Bg, const void *Sg,
                                       const uint32_t *Bu, const void *Su, const uint32_t *Bd, const void *Sd,
                                       void *O, hipStream_t st);
+// kernels (int4_gemv.hip)
+bool int4_gemv_supports(int M, int K, int group, bool zero);
+ternocl_status int4_gemv_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                             const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
+                             int out_f32, hipStream_t st);
 // kernels (int4_plain.hip)
 ternocl_status int4_plain_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
                               const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
@@ -695,6 +700,8 @@ ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, co
     if (s != TERNOCL_OK) return s;
     if (!int4_group(group)) FAIL(TERNOCL_ERR_INVALID_ARG, "group must be 32, 64 or 128");
     if ((uintptr_t)B & 15) FAIL(TERNOCL_ERR_INVALID_ARG, "B must be 16-byte aligned");
+    if (((uintptr_t)A & 15) == 0 && int4_gemv_supports(M, K, group, Z != nullptr))
+        return int4_gemv_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
     return int4_plain_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
 }
 
