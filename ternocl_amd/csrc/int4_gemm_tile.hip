@@ -1,0 +1,206 @@
+// int4_gemm_tile.hip -- GEMM of hundreds of rows and more on 4-bit weights with group
+// scales for gfx950 (ternocl_int4_gemm): the same sums as int4_gemm_kw.hip on 128 x 256
+// tiles whose eight waves share the activations in LDS.
+#include "gemm_kw.hpp"
+#include "int4_decode.hpp"
+
+#include <algorithm>
+
+namespace tcl {
+namespace {
+
+constexpr int kMB = 2, kCB = 2;  // a wave: 64 rows x 64 columns
+// WM x WN waves
+template <int WM_, int WN_> struct TileCfg {
+    static constexpr int WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
+    static constexpr int BM = 64 * WM, BN = 64 * WN;
+    static constexpr int A_BYTES = BM * 128;                       // a 64-k unit of the rows
+    static constexpr int LOADS = A_BYTES / (16 * THREADS);         // 16-byte chunks a lane
+    static_assert(LOADS * 16 * THREADS == A_BYTES, "whole loads");
+};
+
+struct I4TileArgs {
+    const uint16_t *A;
+    const uint32_t *B;
+    const uint16_t *S, *Z;
+    void *C;
+    const uint16_t *Other;
+    const void *Bias;
+    int M, N, K, postop, out_f32;
+};
+
+// LDS writes are done and every wave is here; global loads in flight stay so.
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds__(Cfg::THREADS) k_int4_gemm_tile(const I4TileArgs a) {
+    constexpr int MB = kMB, CB = kCB, GU = G < 64 ? 2 : 1;
+    constexpr bool OFF = BF16 || ZP;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][Cfg::A_BYTES];
+    const int mt = (a.M + Cfg::BM - 1) / Cfg::BM, nt = (a.N + Cfg::BN - 1) / Cfg::BN;
+    int tm, tn;
+    {  // XCD x takes a contiguous range of the tiles, column strip by column strip
+        const int per = (mt * nt + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if (t >= mt * nt) return;  // whole workgroup: padding
+        tn = t / mt;
+        tm = t - tn * mt;
+    }
+    const int m0 = tm * Cfg::BM, n0 = tn * Cfg::BN, mrows = min(Cfg::BM, a.M - m0);
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, q = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % Cfg::WM, wn = wave / Cfg::WM;
+    const int units = a.K / 64;
+    // A: chunk tid + THREADS i of the unit: row / 8, position / 8 swizzled by the row
+    const uint16_t *ap[Cfg::LOADS];
+    uint32_t ad[Cfg::LOADS];
+#pragma unroll
+    for (int i = 0; i < Cfg::LOADS; ++i) {
+        const int ch = tid + Cfg::THREADS * i, r = ch >> 3, j = ch & 7;
+        ap[i] = a.A + (size_t)(m0 + min(r, mrows - 1)) * a.K + 8 * j;
+        ad[i] = (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4));
+    }
+    u32x4_t av[Cfg::LOADS];
+    auto a_load = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < Cfg::LOADS; ++i) av[i] = *(const u32x4_t *)(ap[i] + 64 * (size_t)min(u, units - 1));
+    };
+    auto a_store = [&](int p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < Cfg::LOADS; ++i) *(u32x4_t *)(lds[p] + ad[i]) = av[i];
+    };
+    uint32_t ar[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = G < 64 ? 4 * (i >> 1) + 2 * q + (i & 1) : 4 * q + i;
+        ar[i] = (uint32_t)((64 * wm + c) * 128 + ((j ^ (c & 7)) << 4));
+    }
+    I4Src<CB, 2, G, ZP, false> bs;
+    bs.B = a.B;
+    bs.S = a.S;
+    bs.Z = a.Z;
+    bs.N = a.N;
+    bs.units = units;
+    bs.q = q;
+    bs.col = (uint32_t)min(n0 + 64 * wn + CB * c, a.N - CB);
+    const I4Const k4 = i4_const<BF16>();
+    const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
+    const uint32_t ones[4] = {one, one, one, one};
+    f32x16_t acc[MB][CB], part[MB][CB], sums[OFF ? MB : 1];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) acc[mb][cb] = f32x16_t{};
+    auto unit = [&](int u, int s) __attribute__((always_inline)) {
+        // (every wave has read unit u - 1's buffer, which unit u + 1 is stored to)
+        tile_barrier();
+        u32x4_t af[2][MB];
+        auto a_frag = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) af[i & 1][mb] = *(const u32x4_t *)(lds[s] + ar[i] + 4096 * mb);
+        };
+        a_frag(0);
+        a_store(s ^ 1);
+        a_load(u + 2);
+        uint32_t w[CB][4];
+        float sc[GU][CB], of[GU][CB];
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[cb][i] = bs.w[s][cb][i];
+#pragma unroll
+            for (int g = 0; g < GU; ++g) {
+                sc[g][cb] = i4_scale<CB, BF16>(bs.sr[s][g], cb);
+                if constexpr (OFF) {
+                    float z = BF16 ? 24.0f : 0.0f;
+                    if constexpr (ZP) z += i4_scale<CB, BF16>(bs.zr[s][g], cb);
+                    of[g][cb] = -sc[g][cb] * z;
+                }
+            }
+        }
+        bs.load(u + 2, s);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < 3) a_frag(i + 1);
+            const bool first = G == 128 ? i == 0 && s == 0 : G == 64 ? i == 0 : (i & 1) == 0;
+            const bool last = G == 128 ? i == 3 && s == 1 : G == 64 ? i == 3 : (i & 1) == 1;
+            if constexpr (OFF)
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) sums[mb] = kw_mfma<BF16>(af[i & 1][mb], ones, first ? f32x16_t{} : sums[mb]);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                uint32_t b[4];
+                i4_decode<BF16>(w[cb][i], k4, b);
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) part[mb][cb] = kw_mfma<BF16>(af[i & 1][mb], b, first ? f32x16_t{} : part[mb][cb]);
+            }
+            if (last)
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int g = G < 64 ? i >> 1 : 0;
+                            acc[mb][cb][r] = __builtin_fmaf(part[mb][cb][r], sc[g][cb], acc[mb][cb][r]);
+                            if constexpr (OFF) acc[mb][cb][r] = __builtin_fmaf(sums[mb][r], of[g][cb], acc[mb][cb][r]);
+                        }
+        }
+    };
+    a_load(0);
+    bs.load(0, 0);
+    a_store(0);
+    a_load(1);
+    bs.load(1, 1);
+    for (int u = 0; u < units; u += 2) {  // (K is a multiple of 128)
+        unit(u, 0);
+        unit(u + 1, 1);
+    }
+    epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
+        const int n = n0 + 64 * wn + CB * c;
+        if (n >= a.N) return;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = 64 * wm + 32 * mb + 8 * (r >> 2) + 4 * q + (r & 3);
+                if (m >= mrows) continue;
+                const float v[CB] = {acc[mb][0][r], acc[mb][1][r]};
+                kw_store<CB, BF16, decltype(P_)::value, decltype(F_)::value>(a.C, a.Other, a.Bias, a.N, m0 + m, n, v);
+            }
+    });
+}
+
+template <class Cfg, bool BF16, int G, bool ZP> hipError_t tile_launch(const I4TileArgs &a, hipStream_t st) {
+    const int mt = (a.M + Cfg::BM - 1) / Cfg::BM, nt = (a.N + Cfg::BN - 1) / Cfg::BN;
+    hipLaunchKernelGGL((k_int4_gemm_tile<Cfg, BF16, G, ZP>), dim3(8 * ((mt * nt + 7) / 8)), dim3(Cfg::THREADS), 0, st, a);
+    return hipGetLastError();
+}
+template <class Cfg> hipError_t tile_pick(const I4TileArgs &a, bool bf, int group, hipStream_t st) {
+    auto z = [&](auto b, auto g) {
+        return a.Z ? tile_launch<Cfg, decltype(b)::value, decltype(g)::value, true>(a, st)
+                   : tile_launch<Cfg, decltype(b)::value, decltype(g)::value, false>(a, st);
+    };
+    auto g = [&](auto b) {
+        return group == 32   ? z(b, std::integral_constant<int, 32>{})
+               : group == 64 ? z(b, std::integral_constant<int, 64>{})
+                             : z(b, std::integral_constant<int, 128>{});
+    };
+    return bf ? g(std::true_type{}) : g(std::false_type{});
+}
+
+}  // namespace
+
+// Whether the tiles here are ahead of K over the waves (int4_gemm_kw.hip): where they fill most of the chip.
+bool int4_gemm_tile_wins(int M, int N, int K, int group) {
+    return M > 128 && (long)((M + 127) / 128) * ((N + 255) / 256) >= 128;
+}
+
+// (operands 16-byte aligned)
+ternocl_status int4_gemm_tile_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                                  const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
+                                  int out_f32, hipStream_t st) {
+    const I4TileArgs a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other,
+                          Bias, M, N, K, postop, out_f32};
+    return launch_status(tile_pick<TileCfg<2, 4>>(a, dtype == TERNOCL_BF16, group, st));
+}
+
+}  // namespace tcl

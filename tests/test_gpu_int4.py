@@ -116,7 +116,8 @@ def test_shapes(dev, K, N, M):
 
 
 @pytest.mark.parametrize("M,K,N,group", [(1, 4096, 4096, 128), (4, 1024, 16400, 128), (8, 4096, 6144, 32), (2, 2048, 40000, 64),
-                                         (24, 14336, 1024, 128), (300, 1024, 1552, 32), (700, 512, 2064, 64)])
+                                         (24, 14336, 1024, 128), (300, 1024, 1552, 32), (700, 512, 2064, 64),
+                                         (1000, 256, 4112, 128), (333, 512, 11024, 32), (130, 1152, 16400, 64)])
 @pytest.mark.parametrize("bf16", [False, True])
 def test_real_sizes(dev, M, K, N, group, bf16):
     import ternocl_amd as T
