@@ -5,14 +5,18 @@
 //   largest sums of their group_best largest v stay; ids = the topk largest v, RW = s
 //   of those (renormalised), times scale.
 //
-// One wave per token, lane i holding the VPL experts from VPL i on, so that of equal
-// values the lowest lane's lowest expert is the lowest index.  What is compared are
-// unsigned keys in the order of the values (0: never chosen, all ones: NaN):
-//   * without a bias the logits themselves order the experts -- softmax and the sigmoid
-//     rise with them, and in exact arithmetic only equal logits give equal scores --
-//     so a key is the 32 bits of the fp32 logit;
-//   * with a bias v is computed in fp64 (fp32 scores would tie or swap values closer
-//     than 2^-24 that differ), a key is its 64 bits.
+// L lanes take a token (64 / L tokens a wave), lane i of them holding experts i, i + L, ...
+// topk rounds pick the largest value (a maximum over the lanes), the lowest index that has
+// it (a minimum over those), and drop it.
+//   * Without a bias the logits themselves order the experts -- softmax and the sigmoid
+//     rise with them, and in exact arithmetic only equal logits give equal scores -- so the
+//     rounds compare fp32 logits, exactly.
+//   * With a bias (and for the sums of two that value a group) v is computed in fp32,
+//     and one more round is made: where two picks in a row, or the last group kept and the
+//     first one dropped, are closer than its error (tk_margin) tells apart, the token is
+//     done again with 64-bit values (tk_exact, the whole wave).  So is a token
+//     with a NaN or +inf among its values.  Of N(0, 1.5) logits over 256 experts about 1
+//     token in 200 is.
 #include "common.hpp"
 
 namespace tcl {
@@ -20,18 +24,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-template <int LT> __device__ __forceinline__ float tk_load(const void *p, size_t i) {
-    if constexpr (LT == TERNOCL_FP32) return ((const float *)p)[i];
-    else return dt2f<LT == TERNOCL_BF16>(((const uint16_t *)p)[i]);
-}
-
 // Keys: larger value, larger key; -0 as +0, -inf 0, NaN all ones.
-__device__ __forceinline__ uint32_t tk_key(float v) {
-    const uint32_t b = __float_as_uint(v + 0.0f);
-    if (v != v) return ~0u;
-    if (b == 0xff800000u) return 0u;
-    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
-}
 __device__ __forceinline__ u64 tk_key(double v) {
     const u64 b = (u64)__double_as_longlong(v + 0.0);
     if (v != v) return ~0ull;
@@ -56,91 +49,148 @@ template <class K> __device__ __forceinline__ K tk_max(K v, int lane) {
     v = max(v, tk_xor<16>(v, lane));
     return max(v, tk_xor<32>(v, lane));
 }
-__device__ __forceinline__ float tk_fmax(float v, int lane) {
-    v = fmaxf(v, lane_xor<1>(v, lane));
-    v = fmaxf(v, lane_xor<2>(v, lane));
-    v = fmaxf(v, lane_xor<4>(v, lane));
-    v = fmaxf(v, lane_xor<8>(v, lane));
-    v = fmaxf(v, lane_xor<16>(v, lane));
-    return fmaxf(v, lane_xor<32>(v, lane));
-}
-__device__ __forceinline__ double tk_sum(double v) {
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
-
 struct TkArgs {
     const void *logits;
     const float *bias;
     int *ids;
     void *RW;
     long ld;
-    int T, E, topk, wtype, score, n_group, topk_group, group_best, renorm;
+    int ltype, T, E, topk, wtype, score, n_group, topk_group, group_best, renorm;
     float scale;
 };
 
 constexpr int kTkWaves = 4;
 
-// WIDE: 64-bit keys of v (a bias); else the logits' own.  GROUPED: a choice of groups.
-template <int LT, int VPL, bool WIDE, bool GROUPED>
-__global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
-    typedef std::conditional_t<WIDE, u64, uint32_t> Key;
-    __shared__ u64 gkey[GROUPED ? kTkWaves : 1][GROUPED ? 64 * VPL : 1];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x * kTkWaves + w;
-    if (t >= a.T) return;  // (whole wave; no barrier follows)
-    const int e0 = VPL * lane;
-    float l[VPL];
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        const float x = tk_load<LT>(a.logits, (size_t)t * a.ld + min(e0 + j, a.E - 1));
-        l[j] = e0 + j < a.E ? x : -__builtin_inff();
+// Twice the error of an fp32 value v of a choice: two values further apart are in order.
+// A sigmoid: its argument's two roundings (times s (1 - s) |l|, below 0.23), the
+// exponential's and the reciprocal's last places, below 2^-22 together.  A softmax term:
+// 37 additions of its row's sum at most, each term's argument (E |l - max| <= ln 512) and
+// last place, below 56 x 2^-24 < 2^-18.  The bias's addition: 2^-24 |v|.
+__device__ __forceinline__ float tk_margin(float v, int score) { return (score == 0 ? 0x1p-17f : 0x1p-21f) + 0x1p-22f * fabsf(v); }
+
+// A value's bits as an integer in the order of the values (-0 as +0), kNone for -inf; and
+// back.  (Integer comparisons: fmaxf quiets its operands first, twice the instructions.)
+constexpr int kNone = -0x7fffffff - 1;
+__device__ __forceinline__ int tk_int(float v) {
+    const int b = __float_as_int(v + 0.0f);
+    return v == -__builtin_inff() ? kNone : b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float tk_float(int k) {
+    return k == kNone ? -__builtin_inff() : __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
+}
+
+// Sum, maximum, minimum over the L lanes of a token
+template <int L, class V, class Op> __device__ __forceinline__ V tk_lanes(V v, int lane, Op op) {
+    auto x = [&](auto m) __attribute__((always_inline)) {
+        if constexpr (std::is_same_v<V, int>) v = op(v, __float_as_int(lane_xor<decltype(m)::value>(__int_as_float(v), lane)));
+        else v = op(v, lane_xor<decltype(m)::value>(v, lane));
+    };
+    x(std::integral_constant<int, 1>{});
+    x(std::integral_constant<int, 2>{});
+    x(std::integral_constant<int, 4>{});
+    x(std::integral_constant<int, 8>{});
+    if constexpr (L == 64) {
+        x(std::integral_constant<int, 16>{});
+        x(std::integral_constant<int, 32>{});
     }
-    // softmax: the row's largest logit (NaN passed over: it reaches the sum below)
-    float mx = l[0];
+    return v;
+}
+__device__ __forceinline__ float tk_fmax2(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float tk_add2(float a, float b) { return a + b; }
+__device__ __forceinline__ int tk_imax2(int a, int b) { return max(a, b); }
+__device__ __forceinline__ int tk_imin2(int a, int b) { return min(a, b); }
+template <int L> __device__ __forceinline__ double tk_dsum(double v) {
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, l[j]);
-    mx = tk_fmax(mx, lane);
-    double total = 1.0;
-    const bool need_scores = WIDE || (GROUPED && a.group_best == 2);
-    double s[VPL];
-    if (a.score == 0 && (need_scores || !a.renorm)) {
-        double p = 0.0;
+    for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+__device__ __forceinline__ float tk_logit(const TkArgs &a, int t, int e) {
+    const size_t i = (size_t)t * a.ld + e;
+    if (a.ltype == TERNOCL_FP32) return ((const float *)a.logits)[i];
+    const uint32_t h = ((const uint16_t *)a.logits)[i];
+    return a.ltype == TERNOCL_BF16 ? dt2f<true>(h) : dt2f<false>(h);
+}
+// Logits e0, e0 + step, ... of token t (-inf past the last expert), all loads in flight
+template <int n> __device__ __forceinline__ void tk_logits(const TkArgs &a, int t, int e0, int step, float l[n]) {
+    const size_t row = (size_t)t * a.ld;
+    if (a.ltype == TERNOCL_FP32) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            s[j] = l[j] == -__builtin_inff() ? 0.0 : exp((double)l[j] - (double)mx);
-            p += s[j];
-        }
-        total = tk_sum(p);
+        for (int j = 0; j < n; ++j) l[j] = ((const float *)a.logits)[row + min(e0 + j * step, a.E - 1)];
+    } else {
+        uint16_t h[n];
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = s[j] / total;
-    } else if (need_scores) {
+        for (int j = 0; j < n; ++j) h[j] = ((const uint16_t *)a.logits)[row + min(e0 + j * step, a.E - 1)];
+        if (a.ltype == TERNOCL_BF16) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
-    }
-    Key key[VPL];
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        if constexpr (WIDE) {
-            const double v = s[j] + (double)a.bias[min(e0 + j, a.E - 1)];
-            key[j] = l[j] == -__builtin_inff() ? 0 : tk_key(v);
+            for (int j = 0; j < n; ++j) l[j] = dt2f<true>(h[j]);
         } else {
-            key[j] = tk_key(l[j]);
+#pragma unroll
+            for (int j = 0; j < n; ++j) l[j] = dt2f<false>(h[j]);
         }
     }
-    if constexpr (GROUPED) {
+#pragma unroll
+    for (int j = 0; j < n; ++j) l[j] = e0 + j * step < a.E ? l[j] : -__builtin_inff();
+}
+
+// The outputs of slot r of token t: expert id (-1: none) with logit l.  mx, total: the
+// row's largest logit and its softmax sum; L lanes hold the token's slots.
+template <int L>
+__device__ __forceinline__ void tk_write(const TkArgs &a, int t, int r, int id, float l, float mx, double total, bool on) {
+    const bool live = r < a.topk && id >= 0;
+    double wt;
+    if (a.score == 0) wt = exp((double)l - (double)mx) / total;
+    else wt = 1.0 / (1.0 + exp(-(double)l));
+    if (!live) wt = 0.0;
+    if (a.renorm) {
+        const double sum = tk_dsum<L>(wt);
+        wt = sum == 0.0 ? 0.0 : wt / sum;
+    }
+    wt *= (double)a.scale;
+    if (!on || r >= a.topk) return;
+    const size_t o = (size_t)t * a.topk + r;
+    a.ids[o] = id;
+    const float f = live ? (float)wt : 0.0f;
+    if (a.wtype == TERNOCL_FP32) ((float *)a.RW)[o] = f;
+    else ((uint16_t *)a.RW)[o] = (uint16_t)(a.wtype == TERNOCL_BF16 ? f2dt<true>(f) : f2dt<false>(f));
+}
+
+// Token t by a whole wave, compared by 64-bit keys in the order of the values (0: never
+// chosen, all ones: NaN).  gkey: the wave's LDS, 64 VX keys.
+template <int VX> __device__ __forceinline__ void tk_exact(const TkArgs &a, int t, int lane, u64 *gkey) {
+    const bool grouped = a.topk_group < a.n_group;
+    const int e0 = VX * lane;
+    float l[VX];
+    double s[VX], p = 0.0;
+    tk_logits<VX>(a, t, e0, 1, l);
+    float mx = l[0];  // (NaN passed over: it reaches the sum)
+#pragma unroll
+    for (int j = 1; j < VX; ++j) mx = fmaxf(mx, l[j]);
+    mx = tk_lanes<64>(mx, lane, tk_fmax2);
+#pragma unroll
+    for (int j = 0; j < VX; ++j) {
+        if (a.score == 0) s[j] = l[j] == -__builtin_inff() ? 0.0 : exp((double)l[j] - (double)mx);
+        else s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+        p += s[j];
+    }
+    const double total = a.score == 0 ? tk_dsum<64>(p) : 1.0;
+    u64 key[VX];
+#pragma unroll
+    for (int j = 0; j < VX; ++j) {
+        s[j] = s[j] / total;
+        const double v = a.bias ? s[j] + (double)a.bias[min(e0 + j, a.E - 1)] : (double)l[j];
+        key[j] = l[j] == -__builtin_inff() ? 0 : tk_key(v);
+    }
+    if (grouped) {
         // a group's value as a key of its own (0: none to choose), lane g for group g
         const int per = a.E / a.n_group;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            if constexpr (WIDE) gkey[w][e0 + j] = key[j];
-            else gkey[w][e0 + j] = a.group_best == 2 ? (key[j] ? tk_key(s[j]) : 0) : (u64)key[j];
-        }
+        for (int j = 0; j < VX; ++j) gkey[e0 + j] = a.group_best == 2 && !a.bias ? (key[j] ? tk_key(s[j]) : 0) : key[j];
         __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
         u64 k1 = 0, k2 = 0;
         if (lane < a.n_group)
             for (int i = 0; i < per; ++i) {
-                const u64 k = gkey[w][lane * per + i];
+                const u64 k = gkey[lane * per + i];
                 k2 = max(k2, min(k, k1));
                 k1 = max(k1, k);
             }
@@ -149,95 +199,248 @@ __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
         // kept: fewer than topk_group groups come before it
         int before = 0;
         for (int g = 0; g < a.n_group; ++g) {
-            const u64 o = (u64)__builtin_amdgcn_readlane((int)(uint32_t)gv, g) & 0xffffffffull;
-            const u64 ov = o | ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(gv >> 32), g) << 32);
+            const u64 ov = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)gv, g) |
+                           ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(gv >> 32), g) << 32);
             before += ov > gv || (ov == gv && g < lane);
         }
         const u64 kept = __ballot(before < a.topk_group);
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
+        for (int j = 0; j < VX; ++j)
             if (!((kept >> (min(e0 + j, a.E - 1) / per)) & 1)) key[j] = 0;
     }
-    // topk rounds: the largest key, of equal ones the lowest lane's lowest
-    int id = -1;       // lane r: round r's expert
-    float lv = 0.0f;   // ... and its logit
+    int id = -1;
+    float lv = 0.0f;
     for (int r = 0; r < a.topk; ++r) {
-        Key best = key[0];
+        u64 best = key[0];
 #pragma unroll
-        for (int j = 1; j < VPL; ++j) best = max(best, key[j]);
-        const Key m = tk_max(best, lane);
+        for (int j = 1; j < VX; ++j) best = max(best, key[j]);
+        const u64 m = tk_max(best, lane);
         if (m == 0) break;  // (uniform)
         const int from = __builtin_ctzll(__ballot(best == m));
-        int e = 0;
+        int at = 0;
         float x = 0.0f;
 #pragma unroll
-        for (int j = VPL - 1; j >= 0; --j)
+        for (int j = VX - 1; j >= 0; --j)
             if (key[j] == m) {
-                e = e0 + j;
+                at = j;
                 x = l[j];
             }
-        bool taken = false;
+        at = lane == from ? at : -1;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (lane == from && !taken && key[j] == m) {
-                key[j] = 0;
-                taken = true;
-            }
-        e = __builtin_amdgcn_readlane(e, from);
+        for (int j = 0; j < VX; ++j)
+            if (at == j) key[j] = 0;
+        const int e = __builtin_amdgcn_readlane(e0 + at, from);
         x = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), from));
         if (lane == r) {
             id = e;
             lv = x;
         }
     }
-    // the weights, one lane each, in fp64 (a lane's work for the whole wave: one exp)
-    const bool live = lane < a.topk && id >= 0;
-    double wt;
-    if (a.score == 0) wt = exp((double)lv - (double)mx) / total;
-    else wt = 1.0 / (1.0 + exp(-(double)lv));
-    if (!live) wt = 0.0;
-    if (a.renorm) {
-        const double sum = tk_sum(wt);
-        wt = sum == 0.0 ? 0.0 : wt / sum;
-    }
-    wt *= (double)a.scale;
-    if (lane < a.topk) {
-        const size_t o = (size_t)t * a.topk + lane;
-        a.ids[o] = id;
-        const float f = live ? (float)wt : 0.0f;
-        if (a.wtype == TERNOCL_FP32) ((float *)a.RW)[o] = f;
-        else ((uint16_t *)a.RW)[o] = (uint16_t)(a.wtype == TERNOCL_BF16 ? f2dt<true>(f) : f2dt<false>(f));
-    }
+    tk_write<64>(a, t, lane, id, lv, mx, total, true);
 }
 
-template <int LT, int VPL> void tk_launch(const TkArgs &a, hipStream_t st) {
-    const dim3 g((a.T + kTkWaves - 1) / kTkWaves), b(64 * kTkWaves);
-    const bool grouped = a.topk_group < a.n_group;
-    if (a.bias) {
-        if (grouped) hipLaunchKernelGGL((k_moe_topk<LT, VPL, true, true>), g, b, 0, st, a);
-        else hipLaunchKernelGGL((k_moe_topk<LT, VPL, true, false>), g, b, 0, st, a);
-    } else {
-        if (grouped) hipLaunchKernelGGL((k_moe_topk<LT, VPL, false, true>), g, b, 0, st, a);
-        else hipLaunchKernelGGL((k_moe_topk<LT, VPL, false, false>), g, b, 0, st, a);
+template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
+    constexpr int TPW = 64 / L, VX = VPL * L / 64 > 0 ? VPL * L / 64 : 1;
+    // a wave's values [tokens][L VPL] while groups are valued, tk_exact's keys
+    __shared__ u64 space[kTkWaves][(TPW * L * VPL + 1) / 2 > 64 * VX ? (TPW * L * VPL + 1) / 2 : 64 * VX];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sub = lane % L, tok = lane / L;
+    const int t0 = (blockIdx.x * kTkWaves + w) * TPW, t = t0 + tok;
+    if (t0 >= a.T) return;  // (whole wave; no barrier follows)
+    const bool on = t < a.T;
+    const int tc = min(t, a.T - 1);
+    const float ninf = -__builtin_inff();
+    float l[VPL], bias[VPL];
+    int v[VPL];  // what experts are chosen by (tk_int)
+    tk_logits<VPL>(a, tc, sub, L, l);
+    if (a.bias)
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) bias[j] = a.bias[min(sub + L * j, a.E - 1)];
+    bool odd = false;  // this token needs 64 bits
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        odd |= !(l[j] < __builtin_inff());
+        v[j] = tk_int(l[j]);
     }
+    float mx = ninf;
+    double total = 1.0;
+    const bool two = GROUPED && a.group_best == 2;
+    if (a.score == 0) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) mx = fmaxf(mx, l[j]);
+        mx = tk_lanes<L>(mx, lane, tk_fmax2);
+    }
+    float s[VPL];  // the scores, where choices are made by them
+    if (a.bias || two) {
+        float p = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            if (a.score == 0) s[j] = l[j] == ninf ? 0.0f : __builtin_amdgcn_exp2f((l[j] - mx) * 1.44269504088896341f);
+            else s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504088896341f));
+            p += s[j];
+        }
+        if (a.score == 0) {
+            const float r = 1.0f / tk_lanes<L>(p, lane, tk_add2);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) s[j] *= r;
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const float x = s[j] + bias[j];
+                v[j] = l[j] == ninf ? kNone : tk_int(x);
+                odd |= !(x < __builtin_inff());
+            }
+        }
+    }
+    if (a.score == 0 && !a.renorm) {
+        // the weights' denominator, as exact as they are stored
+        if (a.wtype == TERNOCL_FP32) {
+            double p = 0.0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) p += l[j] == ninf ? 0.0 : exp((double)l[j] - (double)mx);
+            total = tk_dsum<L>(p);
+        } else {
+            float p = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) p += l[j] == ninf ? 0.0f : __builtin_amdgcn_exp2f((l[j] - mx) * 1.44269504088896341f);
+            total = (double)tk_lanes<L>(p, lane, tk_add2);
+        }
+    }
+    if constexpr (GROUPED) {
+        const int per = a.E / a.n_group;
+        int *val = (int *)space[w] + tok * L * VPL;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) val[sub + L * j] = two && !a.bias ? (v[j] == kNone ? kNone : tk_int(s[j])) : v[j];
+        __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+        // lane g values groups g, g + L, ...: their largest one or two (each lane starts at
+        // another member, for the banks)
+        constexpr int GPL = 64 / L;
+        int gv[GPL];
+#pragma unroll
+        for (int k = 0; k < GPL; ++k) {
+            const int g = sub + L * k;
+            int b1 = kNone, b2 = kNone;
+            if (L * k < a.n_group) {  // (uniform)
+                const int *x = val + min(g, a.n_group - 1) * per;
+                int i = sub % per;
+                for (int n = 0; n < per; n += 4) {
+                    int o[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        o[u] = x[i];
+                        i = i + 1 == per ? 0 : i + 1;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int y = n + u < per ? o[u] : kNone;
+                        b2 = max(b2, min(y, b1));
+                        b1 = max(b1, y);
+                    }
+                }
+            }
+            gv[k] = g >= a.n_group ? kNone : two && b2 != kNone ? tk_int(tk_float(b1) + tk_float(b2)) : b1;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < GPL; ++k)
+            if (sub + L * k < a.n_group) val[sub + L * k] = gv[k];
+        __builtin_amdgcn_wave_barrier();
+        // kept: fewer than topk_group groups come before it
+        int before[GPL] = {};
+#pragma unroll 4
+        for (int g = 0; g < a.n_group; ++g) {
+            const int o = val[g];
+#pragma unroll
+            for (int k = 0; k < GPL; ++k) before[k] += o > gv[k] || (o == gv[k] && g < sub + L * k);
+        }
+        u64 kept = 0;
+        int low = 0x7fffffff, high = kNone;  // the least kept, the largest dropped
+#pragma unroll
+        for (int k = 0; k < GPL; ++k) {
+            const bool keep = before[k] < a.topk_group && sub + L * k < a.n_group;
+            const u64 b = __ballot(keep);
+            kept |= L == 64 ? b : ((b >> (L * tok)) & ((1ull << (L & 63)) - 1)) << (L * k);
+            if (keep) low = min(low, gv[k]);
+            else high = max(high, gv[k]);
+        }
+        if (a.bias || two) {
+            const float lo = tk_float(tk_lanes<L>(low, lane, tk_imin2)), hi = tk_float(tk_lanes<L>(high, lane, tk_imax2));
+            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, a.score));
+        }
+        const float inv = 1.0f / (float)per;  // (e + 1/2) / per, e < 512: 2^-10 or more from a whole number
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (!((kept >> (int)(((float)min(sub + L * j, a.E - 1) + 0.5f) * inv)) & 1)) v[j] = kNone;
+    }
+    // the rounds
+    float last = __builtin_inff();
+    int id = -1, pick = kNone;  // lane r: round r's expert and what it was chosen by
+    const int rounds = a.topk + (a.bias ? 1 : 0);
+    for (int r = 0; r < rounds; ++r) {
+        int best = v[0];
+#pragma unroll
+        for (int j = 1; j < VPL; ++j) best = max(best, v[j]);
+        const int m = tk_lanes<L>(best, lane, tk_imax2);
+        if (__ballot(m != kNone) == 0) break;  // (uniform)
+        if (a.bias) {
+            const float x = tk_float(m);
+            odd |= r > 0 && m != kNone && !(last - x > tk_margin(last, a.score));
+            last = x;
+            if (r == a.topk) break;
+        }
+        int e = 1 << 20;
+#pragma unroll
+        for (int j = VPL - 1; j >= 0; --j) e = v[j] == m ? sub + L * j : e;
+        e = tk_lanes<L>(e, lane, tk_imin2);
+        const int at = e - sub;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) v[j] = at == L * j ? kNone : v[j];
+        if (sub == r && m != kNone) {
+            id = e;
+            pick = m;
+        }
+    }
+    float lv = tk_float(pick);
+    if (a.bias) lv = id >= 0 ? tk_logit(a, tc, id) : 0.0f;
+    const u64 redo = __ballot(odd && on);
+    const u64 own = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (L * tok);
+    tk_write<L>(a, t, sub, id, lv, mx, total, on && !(redo & own));
+    if (redo)
+        for (int k = 0; k < TPW; ++k) {
+            const u64 mask = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (L * k);
+            if (redo & mask) tk_exact<VX>(a, t0 + k, lane, space[w]);
+        }
 }
 
-template <int LT> void tk_vpl(const TkArgs &a, hipStream_t st) {
-    if (a.E <= 64) tk_launch<LT, 1>(a, st);
-    else if (a.E <= 128) tk_launch<LT, 2>(a, st);
-    else if (a.E <= 256) tk_launch<LT, 4>(a, st);
-    else tk_launch<LT, 8>(a, st);
+template <int L, int VPL> void tk_launch(const TkArgs &a, hipStream_t st) {
+    const int per = kTkWaves * 64 / L;
+    const dim3 g((a.T + per - 1) / per), b(64 * kTkWaves);
+    if (a.topk_group < a.n_group) hipLaunchKernelGGL((k_moe_topk<L, VPL, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((k_moe_topk<L, VPL, false>), g, b, 0, st, a);
 }
+
+// Tokens from which four share a wave: with fewer, waves are short of SIMDs, and a token's
+// rounds are shorter over 64 lanes.
+constexpr int kTkMany = 4096;
 
 }  // namespace
 
 ternocl_status moe_topk_run(int ltype, const void *logits, long ld, const float *bias, int *ids, int wtype, void *RW, int T,
                             int E, int topk, int score, int n_group, int topk_group, int group_best, int renorm,
                             float scale, hipStream_t st) {
-    const TkArgs a = {logits, bias, ids, RW, ld, T, E, topk, wtype, score, n_group, topk_group, group_best, renorm, scale};
-    if (ltype == TERNOCL_FP32) tk_vpl<TERNOCL_FP32>(a, st);
-    else if (ltype == TERNOCL_BF16) tk_vpl<TERNOCL_BF16>(a, st);
-    else tk_vpl<TERNOCL_FP16>(a, st);
+    const TkArgs a = {logits, bias, ids, RW, ld, ltype, T, E, topk, wtype, score, n_group, topk_group, group_best, renorm, scale};
+    if (T >= kTkMany && topk <= 16) {
+        if (E <= 64) tk_launch<16, 4>(a, st);
+        else if (E <= 128) tk_launch<16, 8>(a, st);
+        else if (E <= 256) tk_launch<16, 16>(a, st);
+        else tk_launch<16, 32>(a, st);
+    } else {
+        if (E <= 64) tk_launch<64, 1>(a, st);
+        else if (E <= 128) tk_launch<64, 2>(a, st);
+        else if (E <= 256) tk_launch<64, 4>(a, st);
+        else tk_launch<64, 8>(a, st);
+    }
     return check_launch();
 }
 
