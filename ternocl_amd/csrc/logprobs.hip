@@ -14,11 +14,11 @@
 // launch.
 //
 // The alternatives: every thread also keeps the largest of each run of its vectors (a
-// "piece").  The topn-th largest of any 256 maxima of disjoint pieces is a bound that
-// at least topn entries reach, and only pieces whose maximum reaches it hold any:
-// those are read again, their entries at or above the bound (about topn of them where
-// values are spread) collected in LDS and ranked by (logit, lowest index).  Where more
-// than kCap reach it (many equal logits), a radix selection over the whole row first
+// "piece").  The topn-th largest of the 256 threads' maxima is a bound that at least topn
+// entries reach, and only pieces whose maximum reaches it hold any: those are read again,
+// their entries at or above the bound (about topn of them where values are spread)
+// collected in LDS and ranked by (logit, lowest index).  Where more than kFlags pieces or
+// kCap entries reach it (many equal logits), a radix selection over the whole row first
 // finds the exact topn-th (value, index) key.
 #include "common.hpp"
 
@@ -229,24 +229,27 @@ struct LpArgs {
     float *maxima;           // [M][chunks][256] (workspace)
 };
 
-__device__ __forceinline__ u64 lp_key(float v, int i) {  // larger: before (v not NaN)
+constexpr int kFlags = 1024;  // pieces read again at most
+struct LpLds {
+    uint32_t thread[kThreads];  // the threads' maxima, in order (lp_ord)
+    u64 cand[kCap];
+    uint32_t flag[kFlags];
+    uint32_t hist[256];
+    int count, flags, need;
+    u64 key;
+};
+// A value's bits as an unsigned integer in the order of the values (-0 as +0).
+__device__ __forceinline__ uint32_t lp_ord(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
-    return ((u64)(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u)) << 32) | (uint32_t)~i;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
+
+__device__ __forceinline__ u64 lp_key(float v, int i) { return ((u64)lp_ord(v) << 32) | (uint32_t)~i; }  // larger: before
 __device__ __forceinline__ float lp_key_value(u64 k) {
     const uint32_t h = (uint32_t)(k >> 32);
     return __uint_as_float(h & 0x80000000u ? h ^ 0x80000000u : ~h);
 }
 
-struct LpLds {
-    float sorted[kThreads];
-    u64 cand[kCap];
-    uint32_t hist[256];
-    int count;
-    float bound;
-    u64 key;
-    int need;
-};
 
 // Calls f(value, index) on every entry of the row, thread by thread.
 template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<LT> &row, F &&f) {
@@ -264,13 +267,13 @@ template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<L
     }
 }
 
-// The row's outputs from its sums and its pieces' maxima: pm [chunks][pieces][256],
-// chunk k's thread t piece p = batches p bpp .. of vectors [k chunk_vecs, ...).
+// The row's outputs from its sums and its pieces' maxima pm [pieces][256]: thread t's piece p
+// holds vectors p span + t + 256 i, i < span / 256 (and, with p = 0, edge entry t).
 template <int LT, bool TOP>
 __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row, int m, const LpSum &s, const float *pm,
-                                          int chunks, int chunk_vecs, int pieces, int bpp, LpLds &L) {
+                                          int pieces, int span, LpLds &L) {
     constexpr int NV = LpVec<LT>::NV;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     const bool empty = s.m == -__builtin_inff() && s.r == 0.0f;
     const bool bad = !(s.r < __builtin_inff()) || s.m == __builtin_inff();
     const float l1 = log1pf(s.r), nan = __builtin_nanf("");
@@ -297,51 +300,77 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
         }
         return;
     }
-    // the bound: the topn-th largest of the 256 threads' maxima
+    // the bound: of the 256 threads' maxima, the topn-th largest's upper 16 bits (topn maxima
+    // at least reach it)
     float v = -__builtin_inff();
-    for (int i = 0; i < chunks * pieces; ++i) v = fmaxf(v, pm[i * kThreads + tid]);
-    L.sorted[tid] = v;
-    if (tid == 0) L.count = 0;
-    __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < kThreads; ++i) {
-        const float o = L.sorted[i];
-        rank += o > v || (o == v && i < tid);
+    for (int p0 = 0; p0 < pieces; p0 += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = pm[min(p0 + i, pieces - 1) * kThreads + tid];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v = fmaxf(v, x[i]);
     }
-    if (rank == a.topn - 1) L.bound = v;
+    L.thread[tid] = lp_ord(v) >> 16;
+    if (tid == 0) L.count = L.flags = 0;
     __syncthreads();
-    const float bound = L.bound;
+    uint32_t o4[4], found = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o4[i] = L.thread[64 * i + lane];
+#pragma unroll
+    for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t t = found | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += __builtin_popcountll(__ballot(o4[i] >= t));
+        if (n >= a.topn) found = t;  // (uniform)
+    }
+    const uint32_t bound = found << 16;  // (of lp_ord; a row with fewer entries than topn above -inf: 0x007f << 16)
+    // the pieces that hold entries at or above it
+    for (int p0 = 0; p0 < pieces; p0 += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = pm[min(p0 + i, pieces - 1) * kThreads + tid];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (p0 + i < pieces && x[i] > -__builtin_inff() && lp_ord(x[i]) >= bound) {
+                const int n = atomicAdd(&L.flags, 1);
+                if (n < kFlags) L.flag[n] = (uint32_t)((p0 + i) * kThreads + tid);
+            }
+    }
+    __syncthreads();
+    const int flags = L.flags, per = span / kThreads + 1;  // (the last: the edge)
     auto take = [&](float x, int i) __attribute__((always_inline)) {
-        if (x >= bound && x > -__builtin_inff()) {
+        if (lp_ord(x) >= bound && x > -__builtin_inff()) {
             const int n = atomicAdd(&L.count, 1);
             if (n < kCap) L.cand[n] = lp_key(x, i);
         }
     };
-    for (int k = 0; k < chunks; ++k) {
-        const int v1 = min(row.nvec, (k + 1) * chunk_vecs);
-        for (int p = 0; p < pieces; ++p) {
-            if (pm[(k * pieces + p) * kThreads + tid] < bound) continue;
-            if (k == 0 && p == 0 && tid < row.edge) {
-                const int i = row.edge_index(tid);
-                take(lp_load1<LT>(row.p, i), i);
-            }
-            const int b0 = k * chunk_vecs + p * bpp * kThreads * kU;
-            const int b1 = min(v1, b0 + bpp * kThreads * kU);
-            for (int w = b0 + tid; w < b1; w += kThreads) {
-                float y[NV];
-                lp_unpack<LT>(row.vec(w), y);
+    if (flags <= kFlags)
+        for (int it = tid; it < flags * per; it += kThreads) {
+            const int f = it / per, j = it - f * per, p = (int)L.flag[f] / kThreads, t = (int)L.flag[f] % kThreads;
+            if (j == per - 1) {
+                if (p == 0 && t < row.edge) {
+                    const int i = row.edge_index(t);
+                    take(lp_load1<LT>(row.p, i), i);
+                }
+            } else {
+                const int w = p * span + t + kThreads * j;
+                if (w < row.nvec) {
+                    float y[NV];
+                    lp_unpack<LT>(row.vec(w), y);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) take(y[i], row.head + w * NV + i);
+                    for (int i = 0; i < NV; ++i) take(y[i], row.head + w * NV + i);
+                }
             }
         }
-    }
     __syncthreads();
     int count = L.count;
-    if (count > kCap) {  // (uniform)
+    if (count > kCap || flags > kFlags) {  // (uniform)
         // the topn-th largest key, 8 bits at a time over the whole row
         u64 prefix = 0;
         int need = a.topn;
         for (int shift = 56; shift >= 0; shift -= 8) {
+            __syncthreads();
             L.hist[tid] = 0;
             __syncthreads();
             lp_scan<LT>(row, [&](float x, int i) __attribute__((always_inline)) {
@@ -359,7 +388,6 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
             __syncthreads();
             prefix = L.key;
             need = L.need;
-            __syncthreads();
         }
         if (tid == 0) L.count = 0;
         __syncthreads();
@@ -376,6 +404,7 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     for (int c = tid; c < count; c += kThreads) {
         const u64 k = L.cand[c];
         int before = 0;
+#pragma unroll 4
         for (int i = 0; i < count; ++i) before += L.cand[i] > k;
         if (before < a.topn) {
             ids[before] = (int)~(uint32_t)k;
@@ -401,7 +430,7 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
     LpSum s = wsum[0];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
-    lp_finish<LT, TOP>(a, row, m, s, pm, 1, pieces * bpp * kThreads * kU, pieces, bpp, reinterpret_cast<LpLds &>(L));
+    lp_finish<LT, TOP>(a, row, m, s, pm, pieces, bpp * kThreads * kU, reinterpret_cast<LpLds &>(L));
 }
 
 template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_part(const LpArgs a) {
@@ -422,19 +451,24 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
 
 template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_join(const LpArgs a) {
     __shared__ std::conditional_t<TOP, LpLds, int> L;
-    __shared__ LpSum total;
-    const int m = blockIdx.x;
+    __shared__ LpSum wsum[kWaves];
+    const int m = blockIdx.x, lane = threadIdx.x & 63;
     const LpRow<LT> row(a.logits, a.ld, m, a.V);
     const float c = a.scale * 1.44269504088896341f;
-    if (threadIdx.x == 0) {
-        LpSum s = a.sums[(size_t)m * a.chunks];
-        for (int k = 1; k < a.chunks; ++k) s = lp_join(s, a.sums[(size_t)m * a.chunks + k], c);
-        total = s;
+    LpSum s = {-__builtin_inff(), 0.0f, 0.0f};
+    for (int k = threadIdx.x; k < a.chunks; k += kThreads) s = lp_join(s, a.sums[(size_t)m * a.chunks + k], c);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const LpSum o = {__shfl_xor(s.m, d, 64), __shfl_xor(s.r, d, 64), __shfl_xor(s.t, d, 64)};
+        s = (lane & d) ? lp_join(o, s, c) : lp_join(s, o, c);  // (the lower lane's first: alike in both)
     }
+    if (lane == 0) wsum[threadIdx.x >> 6] = s;
     __syncthreads();
-    const LpSum s = total;
-    lp_finish<LT, TOP>(a, row, m, s, a.maxima + (size_t)m * a.chunks * kThreads, a.chunks, a.chunk_vecs, 1,
-                       a.chunk_vecs / (kThreads * kU), reinterpret_cast<LpLds &>(L));
+    s = wsum[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
+    lp_finish<LT, TOP>(a, row, m, s, a.maxima + (size_t)m * a.chunks * kThreads, a.chunks, a.chunk_vecs,
+                       reinterpret_cast<LpLds &>(L));
 }
 
 // Workgroups a row is spread over: as many as whole batches give, while all rows stay
