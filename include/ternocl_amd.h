@@ -547,8 +547,10 @@ ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const
  * logits: ltype [M, V] with ld elements from row to row (ld >= V), its rows at any
  * element alignment.  M >= 1, V >= 1, 0 <= topn <= 64, scale > 0 and finite.
  * ws: optional scratch of ternocl_logprobs_ws_bytes(M, V, topn) bytes (0: none used),
- * 16-byte aligned: rows are spread over workgroups where there are few.  NULL or
- * short: one workgroup a row.  The same results, to rounding, either way. */
+ * 16-byte aligned, any contents: rows are spread over workgroups where there are few,
+ * their sums joined by the last (arrival counters in the header, left zero).  NULL or
+ * short: one workgroup a row.  The same results, to rounding, either way, and the same
+ * bits every time.  Calls that share ws must not overlap. */
 size_t ternocl_logprobs_ws_bytes(int M, int V, int topn);
 ternocl_status ternocl_logprobs(int ltype, const void *logits, int64_t ld, const int *tokens, float *logp,
                                 float *entropy, int *top_ids, float *top_logp, int M, int V, int topn, float scale,

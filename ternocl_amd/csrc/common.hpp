@@ -110,6 +110,40 @@ __device__ __forceinline__ uint32_t split_arrive(uint32_t *c, int ksn, int lane)
     return __builtin_amdgcn_readfirstlane(prev);
 }
 
+// A slice's arrival at its tile's counter (lane 0's atomics, broadcast): whether it
+// is the last of ksn.  Two 64-bit words, 0 between calls; the first counts in steps
+// of kKwStep.  A value that no count gives is left from another use of the
+// workspace's memory (these calls' earlier engines took a workspace that nothing
+// had zeroed): every slice of the tile then sees one, and they count again in the
+// second word, by exchanges that take any value but a count of theirs for none.
+// The last arrival zeroes the words.  One atomic addition on a zeroed workspace:
+// counting by exchanges alone, retried whenever another slice arrives, took 4 us
+// more at 7 and 8 slices (M = 43 K = 7040 N = 512 9.0 -> 13.2).
+constexpr uint64_t kKwStep = 0x9E6D3A5171C3B20Full;
+__device__ __forceinline__ bool kw_arrive(uint64_t *c, int ksn, int lane) {
+    bool last = false;
+    if (lane == 0) {
+        const uint64_t seen = __hip_atomic_fetch_add(c, kKwStep, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = seen == (uint64_t)(ksn - 1) * kKwStep;
+        bool count = last;
+        for (int n = 0; n < ksn - 1 && !count; ++n) count = seen == (uint64_t)n * kKwStep;
+        if (!count) {
+            uint64_t e = 0;
+            uint32_t n;
+            do {  // (again only where another of the ksn slices arrived, or after the first guess)
+                n = 0;
+                for (int i = 1; i < ksn; ++i)
+                    if (e == kKwStep + (uint64_t)i) n = (uint32_t)i;
+                last = n == (uint32_t)(ksn - 1);
+            } while (!last && !__hip_atomic_compare_exchange_strong(c + 1, &e, kKwStep + n + 1, __ATOMIC_RELAXED,
+                                                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            if (last) __hip_atomic_store(c + 1, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (last) __hip_atomic_store(c, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return __builtin_amdgcn_readfirstlane((uint32_t)last) != 0;
+}
+
 // The value of lane ^ M (M a power of two below 64): DPP moves for 1, 2, 4 and 8, the
 // row and half swaps for 16 and 32, all VALU; __shfl_xor's ds_bpermute goes through
 // LDS.  The aligned lanes that it moves among must be active.

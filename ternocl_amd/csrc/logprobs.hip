@@ -10,8 +10,8 @@
 // The stream: a workgroup's 256 threads take 16-byte vectors in turn, kU of them in
 // flight per thread; a wave keeps one running maximum for its lanes, raised at most
 // once per batch of kU vectors (r and t = sum d e^d, in base 2, are scaled then).  What
-// bounds it is HBM; a few rows are spread over workgroups, whose sums meet in a second
-// launch.
+// bounds it is HBM; a few rows are spread over workgroups, and the last of a row's to
+// arrive (a counter in the workspace, whatever it held) joins their sums.
 //
 // The alternatives: every thread also keeps the largest of each run of its vectors (a
 // "piece").  The topn-th largest of the 256 threads' maxima is a bound that at least topn
@@ -29,8 +29,9 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kU = 4;      // vectors in flight per thread
-constexpr int kPieces = 32;  // runs of batches per thread at most (LDS)
-constexpr int kCap = 1024; // candidates ranked in LDS
+constexpr int kPieces = 32;  // runs of batches per thread, chunks of a row at most
+constexpr int kPairs = kPieces / 2;
+constexpr int kCap = 512;  // candidates ranked in LDS
 
 template <int LT> struct LpVec {
     static constexpr int NV = LT == TERNOCL_FP32 ? 4 : 8;  // entries of 16 bytes
@@ -112,11 +113,11 @@ __device__ __forceinline__ LpSum lp_join(LpSum a, LpSum b, float c) {
     return o;
 }
 
-// One entry's terms: (2^e2, e2 2^e2).
+// One entry's terms: (2^e2, e2 2^e2).  (e2 from -1000 down, -inf too: 0, and no -inf times 0.)
 __device__ __forceinline__ void lp_term(float x, float m, float c, float &r, float &t) {
-    const float d = (x - m) * c, e = __builtin_amdgcn_exp2f(d);
+    const float y = (x - m) * c, d = y < -1000.0f ? -1000.0f : y, e = __builtin_amdgcn_exp2f(d);
     r += e;
-    t += e > 0.0f ? d * e : 0.0f;
+    t = __builtin_fmaf(d, e, t);
 }
 
 // A wave's running sums: m uniform, r and t a lane's part of the sums relative to m.
@@ -158,12 +159,12 @@ struct LpState {
 };
 
 // Streams vectors [v0, v1) of a row (and, with edge, its edge entries) through this
-// workgroup; pm[p * 256 + tid] = the largest entry of thread tid's piece p (batches of
-// 256 kU vectors, bpp in a piece; the edge belongs to piece 0).  Returns each wave's
-// sums in LDS ws[wave] after a barrier.
-template <int LT, bool TOP>
-__device__ __forceinline__ void lp_stream(const LpRow<LT> &row, int v0, int v1, bool edge, int bpp, float c, float *pm,
-                                          LpSum *wsum) {
+// workgroup; put(p, x): the largest entry of this thread's piece p (bpp batches of 256 kU
+// vectors; the edge belongs to piece 0).  Leaves each wave's sums in LDS, wsum[wave]
+// (a barrier follows before they are read).
+template <int LT, bool TOP, class Put>
+__device__ __forceinline__ void lp_stream(const LpRow<LT> &row, int v0, int v1, bool edge, int bpp, float c, LpSum *wsum,
+                                          Put &&put) {
     constexpr int NV = LpVec<LT>::NV;
     const int tid = threadIdx.x, lane = tid & 63;
     LpState st;
@@ -176,19 +177,20 @@ __device__ __forceinline__ void lp_stream(const LpRow<LT> &row, int v0, int v1, 
         st.add(x, piece, c, lane);
     }
     int b = 0, p = 0;
-    for (int v = v0; v < v1; v += kThreads * kU) {
-        uint4 raw[kU];
+    uint4 raw[kU], ahead[kU];
+    auto fetch = [&](int v, uint4 (&o)[kU]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int i = v + u * kThreads + tid;
-            raw[u] = row.vec(min(i, v1 - 1));
-        }
+        for (int u = 0; u < kU; ++u) o[u] = row.vec(min(v + u * kThreads + tid, v1 - 1));
+    };
+    // a batch from vector v on; part: some of its vectors are past v1
+    auto batch = [&](int v, auto part) __attribute__((always_inline)) {
         float x[kU * NV];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             float y[NV];
             lp_unpack<LT>(raw[u], y);
-            const bool in = v + u * kThreads + tid < v1;
+            raw[u] = ahead[u];
+            const bool in = !decltype(part)::value || v + u * kThreads + tid < v1;
 #pragma unroll
             for (int i = 0; i < NV; ++i) x[u * NV + i] = in ? y[i] : -__builtin_inff();
         }
@@ -200,19 +202,25 @@ __device__ __forceinline__ void lp_stream(const LpRow<LT> &row, int v0, int v1, 
         if constexpr (TOP) {
             piece = fmaxf(piece, tm);
             if (++b == bpp) {
-                pm[p * kThreads + tid] = piece;
+                put(p, piece);
                 piece = -__builtin_inff();
                 b = 0;
                 ++p;
             }
         }
+    };
+    if (v0 < v1) fetch(v0, raw);
+    int v = v0;
+    for (; v + kThreads * kU <= v1; v += kThreads * kU) {
+        if (v + kThreads * kU < v1) fetch(v + kThreads * kU, ahead);
+        batch(v, std::false_type{});
     }
+    if (v < v1) batch(v, std::true_type{});
     if constexpr (TOP) {
-        if (b || p == 0) pm[p * kThreads + tid] = piece;
+        if (b || p == 0) put(p, piece);
     }
     const float r = lp_wave_sum(st.r, lane), t = lp_wave_sum(st.t, lane);
     if (lane == 0) wsum[tid >> 6] = LpSum{st.m, r, t};
-    __syncthreads();
 }
 
 struct LpArgs {
@@ -225,11 +233,12 @@ struct LpArgs {
     int M, V, topn;
     float scale;
     int chunks, chunk_vecs;  // of the split launch
-    LpSum *sums;             // [M][chunks] (workspace)
+    uint64_t *arrived;       // [M][2]: arrival counters (workspace header)
+    float *sums;             // [M][chunks][3] (workspace)
     float *maxima;           // [M][chunks][256] (workspace)
 };
 
-constexpr int kFlags = 1024;  // pieces read again at most
+constexpr int kFlags = 512;  // pieces read again at most
 struct LpLds {
     uint32_t thread[kThreads];  // the threads' maxima, in order (lp_ord)
     u64 cand[kCap];
@@ -267,11 +276,36 @@ template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<L
     }
 }
 
-// The row's outputs from its sums and its pieces' maxima pm [pieces][256]: thread t's piece p
-// holds vectors p span + t + 256 i, i < span / 256 (and, with p = 0, edge entry t).
+// The token asked for and its logit (loaded early: two loads, one after the other).
+template <int LT> struct LpToken {
+    int tok;
+    float x;
+    __device__ __forceinline__ LpToken(const LpArgs &a, const LpRow<LT> &row, int m) : tok(a.tokens ? a.tokens[m] : -1) {
+        if (tok >= a.V) tok = -1;
+        x = lp_load1<LT>(row.p, max(tok, 0));
+    }
+};
+
+// The maxima of a row's pieces, two of one piece row in a load: thread t has pairs t + 256 i
+// of [pieces][128] pairs.
+struct LpMaxima {
+    float x[2 * kPairs];
+    template <class Get> __device__ __forceinline__ void load(int pieces, Get &&get) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const int j = threadIdx.x + kThreads * i;
+            const float2 v = get(min(j, 128 * pieces - 1));
+            x[2 * i] = j < 128 * pieces ? v.x : -__builtin_inff();
+            x[2 * i + 1] = j < 128 * pieces ? v.y : -__builtin_inff();
+        }
+    }
+};
+
+// The row's outputs from its sums and its pieces' maxima, p < pieces: thread t's piece p holds
+// vectors p span + t + 256 i, i < span / 256 (and, with p = 0, edge entry t).
 template <int LT, bool TOP>
-__device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row, int m, const LpSum &s, const float *pm,
-                                          int pieces, int span, LpLds &L) {
+__device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row, int m, const LpSum &s,
+                                          const LpToken<LT> &token, const LpMaxima &pm, int pieces, int span, LpLds &L) {
     constexpr int NV = LpVec<LT>::NV;
     const int tid = threadIdx.x, lane = tid & 63;
     const bool empty = s.m == -__builtin_inff() && s.r == 0.0f;
@@ -279,13 +313,8 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     const float l1 = log1pf(s.r), nan = __builtin_nanf("");
     if (tid == 0) {
         if (a.logp) {
-            const int tok = a.tokens[m];
-            float o = 0.0f;
-            if (tok >= 0 && tok < a.V) {
-                const float x = lp_load1<LT>(row.p, tok);
-                o = bad ? nan : empty ? -__builtin_inff() : (x - s.m) * a.scale - l1;
-            }
-            a.logp[m] = o;
+            const float o = bad ? nan : empty ? -__builtin_inff() : (token.x - s.m) * a.scale - l1;
+            a.logp[m] = token.tok < 0 ? 0.0f : o;
         }
         if (a.entropy)
             a.entropy[m] = bad ? nan : empty ? 0.0f : l1 - s.t * 0.693147180559945309f / (1.0f + s.r);
@@ -300,16 +329,11 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
         }
         return;
     }
-    // the bound: of the 256 threads' maxima, the topn-th largest's upper 16 bits (topn maxima
-    // at least reach it)
-    float v = -__builtin_inff();
-    for (int p0 = 0; p0 < pieces; p0 += 8) {
-        float x[8];
+    // the bound: of 256 threads' maxima (each of its pairs above), the topn-th largest's upper
+    // 16 bits (topn entries at least reach it)
+    float v = pm.x[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = pm[min(p0 + i, pieces - 1) * kThreads + tid];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v = fmaxf(v, x[i]);
-    }
+    for (int i = 1; i < 2 * kPairs; ++i) v = fmaxf(v, pm.x[i]);
     L.thread[tid] = lp_ord(v) >> 16;
     if (tid == 0) L.count = L.flags = 0;
     __syncthreads();
@@ -326,24 +350,28 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     }
     const uint32_t bound = found << 16;  // (of lp_ord; a row with fewer entries than topn above -inf: 0x007f << 16)
     // the pieces that hold entries at or above it
-    for (int p0 = 0; p0 < pieces; p0 += 8) {
-        float x[8];
+    if (lp_ord(v) >= bound)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = pm[min(p0 + i, pieces - 1) * kThreads + tid];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (p0 + i < pieces && x[i] > -__builtin_inff() && lp_ord(x[i]) >= bound) {
+        for (int i = 0; i < 2 * kPairs; ++i)
+            if (pm.x[i] > -__builtin_inff() && lp_ord(pm.x[i]) >= bound) {
                 const int n = atomicAdd(&L.flags, 1);
-                if (n < kFlags) L.flag[n] = (uint32_t)((p0 + i) * kThreads + tid);
+                if (n < kFlags) L.flag[n] = (uint32_t)(2 * (tid + kThreads * (i >> 1)) + (i & 1));
             }
-    }
     __syncthreads();
     const int flags = L.flags, per = span / kThreads + 1;  // (the last: the edge)
-    auto take = [&](float x, int i) __attribute__((always_inline)) {
-        if (lp_ord(x) >= bound && x > -__builtin_inff()) {
-            const int n = atomicAdd(&L.count, 1);
-            if (n < kCap) L.cand[n] = lp_key(x, i);
-        }
+    // those of n entries (indices i0 + their place) into the list, one addition to its count
+    auto take = [&](auto &x, auto n, int i0) __attribute__((always_inline)) {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < decltype(n)::value; ++i) mask |= (uint32_t)(x[i] > -__builtin_inff() && lp_ord(x[i]) >= bound) << i;
+        if (!mask) return;
+        int at = atomicAdd(&L.count, __builtin_popcount(mask));
+#pragma unroll
+        for (int i = 0; i < decltype(n)::value; ++i)
+            if (mask >> i & 1) {
+                if (at < kCap) L.cand[at] = lp_key(x[i], i0 + i);
+                ++at;
+            }
     };
     if (flags <= kFlags)
         for (int it = tid; it < flags * per; it += kThreads) {
@@ -351,15 +379,15 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
             if (j == per - 1) {
                 if (p == 0 && t < row.edge) {
                     const int i = row.edge_index(t);
-                    take(lp_load1<LT>(row.p, i), i);
+                    const float x[1] = {lp_load1<LT>(row.p, i)};
+                    take(x, std::integral_constant<int, 1>{}, i);
                 }
             } else {
                 const int w = p * span + t + kThreads * j;
                 if (w < row.nvec) {
                     float y[NV];
                     lp_unpack<LT>(row.vec(w), y);
-#pragma unroll
-                    for (int i = 0; i < NV; ++i) take(y[i], row.head + w * NV + i);
+                    take(y, std::integral_constant<int, NV>{}, row.head + w * NV);
                 }
             }
         }
@@ -417,69 +445,92 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     }
 }
 
+// A row per workgroup.  LDS: the pieces' maxima [pieces][256].
 template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_row(const LpArgs a, int pieces, int bpp) {
+    extern __shared__ __attribute__((aligned(16))) float lp_pm[];
     __shared__ LpSum wsum[kWaves];
-    __shared__ float pm[TOP ? kPieces * kThreads : 1];
     __shared__ std::conditional_t<TOP, LpLds, int> L;
-    const int m = blockIdx.x;
+    const int m = blockIdx.x, tid = threadIdx.x;
     const LpRow<LT> row(a.logits, a.ld, m, a.V);
+    const LpToken<LT> token(a, row, m);
     const float c = a.scale * 1.44269504088896341f;
     if constexpr (TOP)
-        for (int p = 1; p < pieces; ++p) pm[p * kThreads + threadIdx.x] = -__builtin_inff();
-    lp_stream<LT, TOP>(row, 0, row.nvec, true, bpp, c, pm, wsum);
+        for (int p = 1; p < pieces; ++p) lp_pm[p * kThreads + tid] = -__builtin_inff();
+    lp_stream<LT, TOP>(row, 0, row.nvec, true, bpp, c, wsum, [&](int p, float x) __attribute__((always_inline)) {
+        lp_pm[p * kThreads + tid] = x;
+    });
+    __syncthreads();
     LpSum s = wsum[0];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
-    lp_finish<LT, TOP>(a, row, m, s, pm, pieces, bpp * kThreads * kU, reinterpret_cast<LpLds &>(L));
+    LpMaxima pm;
+    if constexpr (TOP) pm.load(pieces, [&](int j) __attribute__((always_inline)) { return ((const float2 *)lp_pm)[j]; });
+    lp_finish<LT, TOP>(a, row, m, s, token, pm, pieces, bpp * kThreads * kU, reinterpret_cast<LpLds &>(L));
 }
 
-template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_part(const LpArgs a) {
+__device__ __forceinline__ void lp_put(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float lp_get(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// A row over a.chunks workgroups, a chunk a piece of each thread: the one that arrives
+// last has the others' sums and maxima (agent-scope stores, done before the arrival) and
+// finishes the row.
+template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_split(const LpArgs a) {
     __shared__ LpSum wsum[kWaves];
-    const int m = blockIdx.y, k = blockIdx.x;
+    __shared__ std::conditional_t<TOP, LpLds, int> L;
+    __shared__ int flag;
+    const int m = blockIdx.y, k = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const LpRow<LT> row(a.logits, a.ld, m, a.V);
+    const LpToken<LT> token(a, row, m);
     const float c = a.scale * 1.44269504088896341f;
     const int v0 = min(k * a.chunk_vecs, row.nvec), v1 = min(row.nvec, v0 + a.chunk_vecs);
-    const size_t o = (size_t)m * a.chunks + k;
-    lp_stream<LT, TOP>(row, v0, v1, k == 0, a.chunk_vecs, c, a.maxima + o * kThreads, wsum);
-    if (threadIdx.x == 0) {
-        LpSum s = wsum[0];
+    float *sums = a.sums + 3 * (size_t)m * a.chunks, *maxima = a.maxima + (size_t)m * a.chunks * kThreads;
+    lp_stream<LT, TOP>(row, v0, v1, k == 0, a.chunk_vecs, c, wsum, [&](int, float x) __attribute__((always_inline)) {
+        lp_put(maxima + k * kThreads + tid, x);
+    });
+    __syncthreads();
+    LpSum s = wsum[0];
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
-        a.sums[o] = s;
+    for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
+    if (tid == 0) {
+        lp_put(sums + 3 * k, s.m);
+        lp_put(sums + 3 * k + 1, s.r);
+        lp_put(sums + 3 * k + 2, s.t);
     }
-}
-
-template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logprobs_join(const LpArgs a) {
-    __shared__ std::conditional_t<TOP, LpLds, int> L;
-    __shared__ LpSum wsum[kWaves];
-    const int m = blockIdx.x, lane = threadIdx.x & 63;
-    const LpRow<LT> row(a.logits, a.ld, m, a.V);
-    const float c = a.scale * 1.44269504088896341f;
-    LpSum s = {-__builtin_inff(), 0.0f, 0.0f};
-    for (int k = threadIdx.x; k < a.chunks; k += kThreads) s = lp_join(s, a.sums[(size_t)m * a.chunks + k], c);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();  // every wave's stores are done
+    if (tid < 64) {
+        const bool last = kw_arrive(a.arrived + 2 * (size_t)m, a.chunks, lane);
+        if (lane == 0) flag = last;
+    }
+    __syncthreads();
+    if (!flag) return;  // (uniform)
+    LpMaxima pm;
+    if constexpr (TOP)
+        pm.load(a.chunks, [&](int j) __attribute__((always_inline)) {
+            const uint64_t v = __hip_atomic_load((const uint64_t *)maxima + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+        });
+    s = LpSum{-__builtin_inff(), 0.0f, 0.0f};
+    if (lane < a.chunks) s = LpSum{lp_get(sums + 3 * lane), lp_get(sums + 3 * lane + 1), lp_get(sums + 3 * lane + 2)};
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
+    for (int d = 1; d < kPieces; d <<= 1) {
         const LpSum o = {__shfl_xor(s.m, d, 64), __shfl_xor(s.r, d, 64), __shfl_xor(s.t, d, 64)};
         s = (lane & d) ? lp_join(o, s, c) : lp_join(s, o, c);  // (the lower lane's first: alike in both)
     }
-    if (lane == 0) wsum[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = wsum[0];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
-    lp_finish<LT, TOP>(a, row, m, s, a.maxima + (size_t)m * a.chunks * kThreads, a.chunks, a.chunk_vecs,
-                       reinterpret_cast<LpLds &>(L));
+    s = LpSum{__shfl(s.m, 0, 64), __shfl(s.r, 0, 64), __shfl(s.t, 0, 64)};
+    lp_finish<LT, TOP>(a, row, m, s, token, pm, a.chunks, a.chunk_vecs, reinterpret_cast<LpLds &>(L));
 }
 
-// Workgroups a row is spread over: as many as whole batches give, while all rows stay
-// within about two workgroups a CU.
-// (nv: entries of a vector)
+// Workgroups a row is spread over (nv: entries of a vector): as many as whole batches
+// give, while all rows stay within about kSplit workgroups.
+constexpr int kSplit = 1024;
 int lp_chunks(int M, int V, int nv, int &chunk_vecs) {
     const long batch = (long)kThreads * kU;
     const long nb = V < nv ? 1 : ((long)V / nv + batch - 1) / batch;
-    long c = M >= 512 ? 1 : 512 / M;
+    long c = M >= kSplit / 2 ? 1 : kSplit / M;
     if (c > nb) c = nb;
-    if (c < 1) c = 1;
+    if (c > kPieces) c = kPieces;
     const long per = (nb + c - 1) / c;
     chunk_vecs = (int)(per * batch);
     return (int)((nb + per - 1) / per);
@@ -490,20 +541,21 @@ int lp_chunks(int M, int V, int nv, int &chunk_vecs) {
 size_t logprobs_ws_need(int M, int V, int topn) {
     int cv;
     const int c = lp_chunks(M, V, 4, cv);  // (16-bit rows have fewer)
-    return c == 1 ? 0 : kWsHeader + (size_t)M * c * (sizeof(LpSum) + (topn ? 4 * kThreads : 0));
+    return c == 1 ? 0 : kWsHeader + (size_t)M * c * (12 + (topn ? 4 * kThreads : 0)) + 4;
 }
 
 ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *tokens, float *logp, float *entropy,
                             int *top_ids, float *top_logp, int M, int V, int topn, float scale, void *ws,
                             size_t ws_bytes, hipStream_t st) {
-    LpArgs a = {logits, ld, tokens, logp, entropy, top_ids, top_logp, M, V, topn, scale, 1, 0, nullptr, nullptr};
+    LpArgs a = {logits, ld, tokens, logp, entropy, top_ids, top_logp, M, V, topn, scale, 1, 0, nullptr, nullptr, nullptr};
     const int nv = ltype == TERNOCL_FP32 ? 4 : 8;
     const size_t need = logprobs_ws_need(M, V, topn);
-    const bool split = need && ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0;
+    if (need && ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0) a.chunks = lp_chunks(M, V, nv, a.chunk_vecs);
+    const bool split = a.chunks > 1;
     if (split) {
-        a.chunks = lp_chunks(M, V, nv, a.chunk_vecs);
-        a.sums = (LpSum *)((uint8_t *)ws + kWsHeader);
-        a.maxima = (float *)(a.sums + (size_t)M * a.chunks);
+        a.arrived = (uint64_t *)ws;  // (kSplit / 2 rows of 16 bytes: within the header)
+        a.sums = (float *)((uint8_t *)ws + kWsHeader);
+        a.maxima = a.sums + align_up(3 * (size_t)M * a.chunks, 2);
     }
     // pieces of the unsplit launch: at most kPieces runs of batches
     const int nb = (V / nv + kThreads * kU - 1) / (kThreads * kU);
@@ -512,10 +564,10 @@ ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *t
         constexpr int LT = decltype(lt)::value;
         constexpr bool TOP = decltype(top)::value;
         if (split) {
-            hipLaunchKernelGGL((k_logprobs_part<LT, TOP>), dim3(a.chunks, M), dim3(kThreads), 0, st, a);
-            hipLaunchKernelGGL((k_logprobs_join<LT, TOP>), dim3(M), dim3(kThreads), 0, st, a);
+            hipLaunchKernelGGL((k_logprobs_split<LT, TOP>), dim3(a.chunks, M), dim3(kThreads), 0, st, a);
         } else {
-            hipLaunchKernelGGL((k_logprobs_row<LT, TOP>), dim3(M), dim3(kThreads), 0, st, a, pieces, bpp);
+            hipLaunchKernelGGL((k_logprobs_row<LT, TOP>), dim3(M), dim3(kThreads), TOP ? pieces * kThreads * 4 : 0, st, a,
+                               pieces, bpp);
         }
     };
     auto lt = [&](auto top) {
