@@ -11,13 +11,15 @@
 //   * Without a bias the logits themselves order the experts -- softmax and the sigmoid
 //     rise with them, and in exact arithmetic only equal logits give equal scores -- so the
 //     rounds compare fp32 logits, exactly.
-//   * With a bias (and for the sums of two that value a group) v is computed in fp32,
-//     and one more round is made: where two picks in a row, or the last group kept and the
-//     first one dropped, are closer than its error (tk_margin) tells apart, the token is
-//     done again with 64-bit values (tk_exact, the whole wave).  So is a token
-//     with a NaN or +inf among its values.  Of N(0, 1.5) logits over 256 experts about 1
-//     token in 200 is.
+//   * With a bias (and for the sums of two that value a group) v is computed in fp32.
+//     Where two picks in a row are closer than its error (tk_margin) tells apart, the picks
+//     up to the next wider gap are ranked by their 64-bit values; where the last group kept
+//     and the first one dropped are, or a value is NaN or +inf, the token is done again
+//     with 64-bit values (tk_exact, the whole wave).  Of N(0, 1.5) logits over 256 experts,
+//     sigmoid scores, about 1 token in 2000 has close picks, 1 in 16000 close groups.
 #include "common.hpp"
+
+#include <algorithm>
 
 namespace tcl {
 namespace {
@@ -133,6 +135,51 @@ template <int n> __device__ __forceinline__ void tk_logits(const TkArgs &a, int 
     for (int j = 0; j < n; ++j) l[j] = e0 + j * step < a.E ? l[j] : -__builtin_inff();
 }
 
+// n values of 2 or 4 bytes each that lie together, in loads of 16 bytes or all of them (p
+// aligned to that)
+template <int bytes, int n> __device__ __forceinline__ void tk_load(const void *p, uint32_t o[n]) {
+    constexpr int total = bytes * n, step = total < 16 ? total : 16;
+    uint32_t w[(total + 3) / 4];
+#pragma unroll
+    for (int i = 0; i < total / step; ++i) {
+        const uint8_t *q = (const uint8_t *)p + 16 * i;
+        if constexpr (step == 16) {
+            const uint4 v = *(const uint4 *)q;
+            __builtin_memcpy(w + 4 * i, &v, 16);
+        } else if constexpr (step == 8) {
+            const uint2 v = *(const uint2 *)q;
+            __builtin_memcpy(w, &v, 8);
+        } else if constexpr (step == 4) {
+            w[0] = *(const uint32_t *)q;
+        } else {
+            w[0] = *(const uint16_t *)q;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) o[j] = bytes == 4 ? w[j] : (w[j / 2] >> (16 * (j & 1))) & 0xffffu;
+}
+// Logits e0 .. e0 + n - 1 of token t (all of them experts, or none: -inf)
+template <int n> __device__ __forceinline__ void tk_logits_together(const TkArgs &a, int t, int e0, float l[n]) {
+    const size_t i = (size_t)t * a.ld + (e0 < a.E ? e0 : 0);
+    uint32_t w[n];
+    if (a.ltype == TERNOCL_FP32) {
+        tk_load<4, n>((const float *)a.logits + i, w);
+#pragma unroll
+        for (int j = 0; j < n; ++j) l[j] = __uint_as_float(w[j]);
+    } else {
+        tk_load<2, n>((const uint16_t *)a.logits + i, w);
+        if (a.ltype == TERNOCL_BF16) {
+#pragma unroll
+            for (int j = 0; j < n; ++j) l[j] = dt2f<true>(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < n; ++j) l[j] = dt2f<false>(w[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) l[j] = e0 < a.E ? l[j] : -__builtin_inff();
+}
+
 // The outputs of slot r of token t: expert id (-1: none) with logit l.  mx, total: the
 // row's largest logit and its softmax sum; L lanes hold the token's slots.
 template <int L>
@@ -189,6 +236,7 @@ template <int VX> __device__ __forceinline__ void tk_exact(const TkArgs &a, int 
         __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
         u64 k1 = 0, k2 = 0;
         if (lane < a.n_group)
+#pragma unroll 8
             for (int i = 0; i < per; ++i) {
                 const u64 k = gkey[lane * per + i];
                 k2 = max(k2, min(k, k1));
@@ -239,7 +287,9 @@ template <int VX> __device__ __forceinline__ void tk_exact(const TkArgs &a, int 
     tk_write<64>(a, t, lane, id, lv, mx, total, true);
 }
 
-template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
+// GROUPED: 0 no choice of groups; 1 any groups; 2 groups of whole lanes, a power of two of
+// them: lane i holds experts i VPL .. + VPL - 1 then.
+template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
     constexpr int TPW = 64 / L, VX = VPL * L / 64 > 0 ? VPL * L / 64 : 1;
     // a wave's values [tokens][L VPL] while groups are valued, tk_exact's keys
     __shared__ u64 space[kTkWaves][(TPW * L * VPL + 1) / 2 > 64 * VX ? (TPW * L * VPL + 1) / 2 : 64 * VX];
@@ -252,10 +302,21 @@ template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * k
     const float ninf = -__builtin_inff();
     float l[VPL], bias[VPL];
     int v[VPL];  // what experts are chosen by (tk_int)
-    tk_logits<VPL>(a, tc, sub, L, l);
-    if (a.bias)
+    constexpr int E0 = GROUPED == 2 ? VPL : 1, ES = GROUPED == 2 ? 1 : L;  // lane i's experts E0 i + ES j
+    if constexpr (GROUPED == 2) {
+        tk_logits_together<VPL>(a, tc, E0 * sub, l);
+        if (a.bias) {
+            uint32_t w[VPL];
+            tk_load<4, VPL>(a.bias + (E0 * sub < a.E ? E0 * sub : 0), w);
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) bias[j] = a.bias[min(sub + L * j, a.E - 1)];
+            for (int j = 0; j < VPL; ++j) bias[j] = __uint_as_float(w[j]);
+        }
+    } else {
+        tk_logits<VPL>(a, tc, sub, L, l);
+        if (a.bias)
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) bias[j] = a.bias[min(sub + L * j, a.E - 1)];
+    }
     bool odd = false;  // this token needs 64 bits
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
@@ -264,7 +325,7 @@ template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * k
     }
     float mx = ninf;
     double total = 1.0;
-    const bool two = GROUPED && a.group_best == 2;
+    const bool two = GROUPED != 0 && a.group_best == 2;
     if (a.score == 0) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) mx = fmaxf(mx, l[j]);
@@ -307,7 +368,54 @@ template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * k
             total = (double)tk_lanes<L>(p, lane, tk_add2);
         }
     }
-    if constexpr (GROUPED) {
+    if constexpr (GROUPED == 2) {
+        // a group's largest two: a lane's own, then over its lanes
+        const int lpg = a.E / a.n_group / VPL, g = sub / lpg;
+        int b1 = kNone, b2 = kNone;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int y = two && !a.bias ? (v[j] == kNone ? kNone : tk_int(s[j])) : v[j];
+            b2 = max(b2, min(y, b1));
+            b1 = max(b1, y);
+        }
+        auto merge = [&](auto m) __attribute__((always_inline)) {
+            if (lpg <= decltype(m)::value) return;  // (uniform)
+            const int o1 = __float_as_int(lane_xor<decltype(m)::value>(__int_as_float(b1), lane));
+            const int o2 = __float_as_int(lane_xor<decltype(m)::value>(__int_as_float(b2), lane));
+            b2 = max(min(b1, o1), max(b2, o2));
+            b1 = max(b1, o1);
+        };
+        merge(std::integral_constant<int, 1>{});
+        merge(std::integral_constant<int, 2>{});
+        merge(std::integral_constant<int, 4>{});
+        merge(std::integral_constant<int, 8>{});
+        if constexpr (L == 64) {
+            merge(std::integral_constant<int, 16>{});
+            merge(std::integral_constant<int, 32>{});
+        }
+        const int gv = two && b2 != kNone ? tk_int(tk_float(b1) + tk_float(b2)) : b1;
+        // kept: fewer than topk_group groups come before it
+        int *val = (int *)space[w] + tok * L;
+        val[g] = gv;  // (by each of its lanes)
+        __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+        int before = 0;
+        for (int i = 0; i < a.n_group; i += 4) {
+            const int4 o = *(const int4 *)(val + i);
+            before += o.x > gv || (o.x == gv && i < g);
+            before += i + 1 < a.n_group && (o.y > gv || (o.y == gv && i + 1 < g));
+            before += i + 2 < a.n_group && (o.z > gv || (o.z == gv && i + 2 < g));
+            before += i + 3 < a.n_group && (o.w > gv || (o.w == gv && i + 3 < g));
+        }
+        const bool keep = before < a.topk_group, real = g < a.n_group;
+        if (a.bias || two) {
+            const float lo = tk_float(tk_lanes<L>(real && keep ? gv : 0x7fffffff, lane, tk_imin2));
+            const float hi = tk_float(tk_lanes<L>(real && !keep ? gv : kNone, lane, tk_imax2));
+            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, a.score));
+        }
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) v[j] = keep ? v[j] : kNone;
+    }
+    if constexpr (GROUPED == 1) {
         const int per = a.E / a.n_group;
         int *val = (int *)space[w] + tok * L * VPL;
 #pragma unroll
@@ -374,38 +482,71 @@ template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * k
             if (!((kept >> (int)(((float)min(sub + L * j, a.E - 1) + 0.5f) * inv)) & 1)) v[j] = kNone;
     }
     // the rounds
+    // With a bias they go on past topk until a pick is apart from the next value, and the
+    // picks are put in order by their 64-bit values where two are not.
     float last = __builtin_inff();
+    bool close = false, settled = false;  // (alike in a token's lanes)
     int id = -1, pick = kNone;  // lane r: round r's expert and what it was chosen by
-    const int rounds = a.topk + (a.bias ? 1 : 0);
-    for (int r = 0; r < rounds; ++r) {
+    for (int r = 0; a.bias || r < a.topk; ++r) {
         int best = v[0];
 #pragma unroll
         for (int j = 1; j < VPL; ++j) best = max(best, v[j]);
         const int m = tk_lanes<L>(best, lane, tk_imax2);
-        if (__ballot(m != kNone) == 0) break;  // (uniform)
         if (a.bias) {
             const float x = tk_float(m);
-            odd |= r > 0 && m != kNone && !(last - x > tk_margin(last, a.score));
+            const bool apart = m == kNone || last - x > tk_margin(last, a.score);
+            settled |= r >= a.topk && apart;
+            if (r >= a.topk && __ballot(!settled) == 0) break;  // (uniform)
+            if (r == L) {  // more close values than lanes
+                odd |= !settled;
+                break;
+            }
+            close |= !settled && r > 0 && !apart;
             last = x;
-            if (r == a.topk) break;
+        } else if (__ballot(m != kNone) == 0) {
+            break;  // (uniform)
         }
         int e = 1 << 20;
 #pragma unroll
-        for (int j = VPL - 1; j >= 0; --j) e = v[j] == m ? sub + L * j : e;
+        for (int j = VPL - 1; j >= 0; --j) e = v[j] == m ? E0 * sub + ES * j : e;
         e = tk_lanes<L>(e, lane, tk_imin2);
-        const int at = e - sub;
+        const int at = e - E0 * sub;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) v[j] = at == L * j ? kNone : v[j];
-        if (sub == r && m != kNone) {
+        for (int j = 0; j < VPL; ++j) v[j] = at == ES * j ? kNone : v[j];
+        if (sub == r && m != kNone && !settled) {
             id = e;
             pick = m;
         }
     }
     float lv = tk_float(pick);
     if (a.bias) lv = id >= 0 ? tk_logit(a, tc, id) : 0.0f;
+    int slot = sub;
+    if (__ballot(close && !odd && on)) {  // (uniform)
+        double x = 0.0;
+        if (a.score == 0) {
+            double p = 0.0;
+#pragma unroll 4
+            for (int e = sub; e < a.E; e += L) {
+                const float y = tk_logit(a, tc, e);
+                p += y == ninf ? 0.0 : exp((double)y - (double)mx);
+            }
+            x = exp((double)lv - (double)mx) / tk_dsum<L>(p);
+        } else {
+            x = 1.0 / (1.0 + exp(-(double)lv));
+        }
+        x += (double)a.bias[max(id, 0)];
+        int rank = 0;
+        for (int r = 0; r < L; ++r) {
+            const double o = __shfl(x, L * tok + r, 64);
+            const int oe = __shfl(id, L * tok + r, 64);
+            if (__ballot(oe >= 0) == 0) break;  // (uniform: no token has a pick r)
+            rank += oe >= 0 && (o > x || (o == x && oe < id));
+        }
+        if (close && id >= 0) slot = rank;
+    }
     const u64 redo = __ballot(odd && on);
     const u64 own = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (L * tok);
-    tk_write<L>(a, t, sub, id, lv, mx, total, on && !(redo & own));
+    tk_write<L>(a, t, slot, id, lv, mx, total, on && !(redo & own));
     if (redo)
         for (int k = 0; k < TPW; ++k) {
             const u64 mask = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (L * k);
@@ -416,8 +557,13 @@ template <int L, int VPL, bool GROUPED> __global__ void __launch_bounds__(64 * k
 template <int L, int VPL> void tk_launch(const TkArgs &a, hipStream_t st) {
     const int per = kTkWaves * 64 / L;
     const dim3 g((a.T + per - 1) / per), b(64 * kTkWaves);
-    if (a.topk_group < a.n_group) hipLaunchKernelGGL((k_moe_topk<L, VPL, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((k_moe_topk<L, VPL, false>), g, b, 0, st, a);
+    const size_t es = a.ltype == TERNOCL_FP32 ? 4 : 2, part = std::min<size_t>(16, VPL * es);
+    const int members = a.E / a.n_group, lpg = members / VPL;
+    const bool lanes = members % VPL == 0 && (lpg & (lpg - 1)) == 0 && (uintptr_t)a.logits % part == 0 &&
+                       a.ld * es % part == 0 && (uintptr_t)a.bias % std::min(16, VPL * 4) == 0;
+    if (a.topk_group == a.n_group) hipLaunchKernelGGL((k_moe_topk<L, VPL, 0>), g, b, 0, st, a);
+    else if (lanes) hipLaunchKernelGGL((k_moe_topk<L, VPL, 2>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((k_moe_topk<L, VPL, 1>), g, b, 0, st, a);
 }
 
 // Tokens from which four share a wave: with fewer, waves are short of SIMDs, and a token's

@@ -90,6 +90,19 @@ def test_tokens(dev, Tk):
     check(T, x, b, 8, "f32", "sigmoid", 8, 3, 2)
 
 
+@pytest.mark.parametrize("Tk", [4095, 4097])
+@pytest.mark.parametrize("E,n_group,topk_group,group_best", [(256, 8, 4, 2), (160, 5, 2, 2), (512, 16, 3, 1), (60, 15, 7, 1),
+                                                             (128, 4, 2, 2), (96, 3, 2, 1), (64, 1, 1, 1)])
+def test_many_tokens(dev, Tk, E, n_group, topk_group, group_best):
+    """Enough tokens for several to share a wave, their scores close now and then."""
+    import ternocl_amd as T
+    x, b = logits_of(Tk + E, Tk, E, "f32")
+    x[::97, ::3] = x[::97, :1] + 2.0**-23 * torch.arange(len(range(0, E, 3)))
+    x[5, 7], x[9, 1:] = -math.inf, -math.inf
+    check(T, x, b, 6, "f32", "sigmoid", n_group, topk_group, group_best, True, 2.5)
+    check(T, x, None, 6, "bf16", "softmax", n_group, topk_group, group_best, False)
+
+
 @pytest.mark.parametrize("E,n_group,topk_group", [(64, 8, 4), (64, 8, 8), (256, 8, 4), (160, 8, 3), (512, 64, 7), (48, 3, 1),
                                                   (64, 64, 32), (126, 9, 2)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
