@@ -26,6 +26,8 @@
 // the same bits on every run, one barrier a strip.
 #include "common.hpp"
 
+#include <algorithm>
+
 namespace tcl {
 namespace {
 
@@ -81,57 +83,73 @@ template <int j> __device__ __forceinline__ uint32_t g4_bytes(uint32_t a, uint32
     return (lo | hi) ^ 0x80808080u;
 }
 
+// Variants of 64 registers a lane: two workgroups on a CU, their staging and tails apart (M =
+// 1 K = 5120 N = 34816 20.0 -> 18.6 us; the others would spill).
+__host__ __device__ constexpr bool g4_two(int rs, int group, bool zero) { return rs == 1 && group == 128 && !zero; }
+
+// Eight activations, task i (i >= tasks: nothing is stored): the lanes of its group are
+// adjacent, and all of a wave's are here.
+template <bool BF16, int G, bool ZP>
+__device__ __forceinline__ void g4_stage8(const G4Args &a, uint8_t *lds, const G4Lds &l, const uint4 &raw, int i, int tasks) {
+    const int units = a.K / 8, mp = a.M > 4 ? 8 : 4, lane = threadIdx.x & 63, R = 3 * a.M;
+    const int ic = min(i, tasks - 1), m = ic / units, u = ic - m * units;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[2 * j] = dt2f<BF16>(w[j] & 0xffffu);
+        f[2 * j + 1] = dt2f<BF16>(w[j] >> 16);
+    }
+    uint32_t mb = 0;  // the largest |a| by its bits: a NaN is above infinity
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(f[j]) & 0x7fffffffu);
+    mb = __float_as_uint(g4_reduce<G>(__uint_as_float(mb), lane, [](float x, float y) {
+        return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y)));
+    }));
+    const bool bad = mb >= 0x7f800000u;
+    const int e = max((int)(mb >> 23), 1) - 127;
+    uint32_t t[8];
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int q = bad ? 0 : (int)__builtin_rintf(__builtin_ldexpf(f[j], 21 - e));
+        sum += q;
+        t[j] = (uint32_t)q + 0x808080u;
+    }
+    if constexpr (ZP)
+        sum = __float_as_int(g4_reduce<G>(__int_as_float(sum), lane, [](float x, float y) {
+            return __int_as_float(__float_as_int(x) + __float_as_int(y));
+        }));
+    if (i >= tasks) return;
+    const int step = u >> 4, b = (u >> 2) & 3, wd = u & 3;
+    const int q = G == 128 ? b : wd, h = (G == 128 ? wd : b) >> 1, half = (G == 128 ? wd : b) & 1;
+    uint8_t *p = lds + l.digits + ((step * 2 + h) * R + 3 * m) * 64 + q * 16 + half * 8;
+    // odd nibbles' rows 2, 6, 3, 7, then even nibbles' rows 0, 4, 1, 5 (the order of g4_mfma)
+    *(uint2 *)(p) = make_uint2(g4_bytes<2>(t[2], t[6], t[3], t[7]), g4_bytes<2>(t[0], t[4], t[1], t[5]));
+    *(uint2 *)(p + 64) = make_uint2(g4_bytes<1>(t[2], t[6], t[3], t[7]), g4_bytes<1>(t[0], t[4], t[1], t[5]));
+    *(uint2 *)(p + 128) = make_uint2(g4_bytes<0>(t[2], t[6], t[3], t[7]), g4_bytes<0>(t[0], t[4], t[1], t[5]));
+    if ((8 * u) % G == 0) {
+        const int g = 8 * u / G;
+        const float s = bad ? __builtin_nanf("") : __builtin_ldexpf(1.0f, e - 21);
+        ((float *)(lds + l.scales))[g * mp + m] = s;
+        if constexpr (ZP) ((float *)(lds + l.sums))[g * mp + m] = (float)sum * s;
+    }
+}
+
 // Stages the digits, powers of two (and sums) of all M rows.  Task i: activations 8 u ..
 // 8 u + 7 of a row; 16 tasks a 128-row step, so G / 8 adjacent lanes hold a group.
-template <bool BF16, int G, bool ZP>
+template <bool BF16, int RS, int G, bool ZP>
 __device__ __forceinline__ void g4_stage(const G4Args &a, uint8_t *lds, const G4Lds &l) {
-    const int units = a.K / 8, tasks = a.M * units, mp = a.M > 4 ? 8 : 4, lane = threadIdx.x & 63;
-    const int R = 3 * a.M;
-    for (int i0 = 0; i0 < tasks; i0 += blockDim.x) {  // (whole steps: tasks is a multiple of 16)
-        const int i = i0 + threadIdx.x, ic = min(i, tasks - 1);
-        const int m = ic / units, u = ic - m * units;
-        const uint4 raw = *(const uint4 *)(a.A + (size_t)m * a.K + 8 * u);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float f[8];
+    const int tasks = a.M * (a.K / 8), mp = a.M > 4 ? 8 : 4;
+    constexpr int kPass = g4_two(RS, G, ZP) ? 1 : 4;  // passes whose loads are in flight together (registers)
+    const int T = blockDim.x;
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < tasks; i0 += kPass * T) {
+        uint4 raw[kPass];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            f[2 * j] = dt2f<BF16>(w[j] & 0xffffu);
-            f[2 * j + 1] = dt2f<BF16>(w[j] >> 16);
-        }
-        uint32_t mb = 0;  // the largest |a| by its bits: a NaN is above infinity
+        for (int k = 0; k < kPass; ++k) raw[k] = *(const uint4 *)(a.A + 8 * (size_t)min(i0 + k * T, tasks - 1));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(f[j]) & 0x7fffffffu);
-        mb = __float_as_uint(g4_reduce<G>(__uint_as_float(mb), lane, [](float x, float y) {
-            return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y)));
-        }));
-        const bool bad = mb >= 0x7f800000u;
-        const int e = max((int)(mb >> 23), 1) - 127;
-        uint32_t t[8];
-        int sum = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int q = bad ? 0 : (int)__builtin_rintf(__builtin_ldexpf(f[j], 21 - e));
-            sum += q;
-            t[j] = (uint32_t)q + 0x808080u;
-        }
-        if constexpr (ZP)
-            sum = __float_as_int(g4_reduce<G>(__int_as_float(sum), lane, [](float x, float y) {
-                return __int_as_float(__float_as_int(x) + __float_as_int(y));
-            }));
-        if (i >= tasks) continue;
-        const int step = u >> 4, b = (u >> 2) & 3, wd = u & 3;
-        const int q = G == 128 ? b : wd, h = (G == 128 ? wd : b) >> 1, half = (G == 128 ? wd : b) & 1;
-        uint8_t *p = lds + l.digits + ((step * 2 + h) * R + 3 * m) * 64 + q * 16 + half * 8;
-        // odd nibbles' rows 2, 6, 3, 7, then even nibbles' rows 0, 4, 1, 5 (the order of g4_mfma)
-        *(uint2 *)(p) = make_uint2(g4_bytes<2>(t[2], t[6], t[3], t[7]), g4_bytes<2>(t[0], t[4], t[1], t[5]));
-        *(uint2 *)(p + 64) = make_uint2(g4_bytes<1>(t[2], t[6], t[3], t[7]), g4_bytes<1>(t[0], t[4], t[1], t[5]));
-        *(uint2 *)(p + 128) = make_uint2(g4_bytes<0>(t[2], t[6], t[3], t[7]), g4_bytes<0>(t[0], t[4], t[1], t[5]));
-        if ((8 * u) % G == 0) {
-            const int g = 8 * u / G;
-            const float s = bad ? __builtin_nanf("") : __builtin_ldexpf(1.0f, e - 21);
-            ((float *)(lds + l.scales))[g * mp + m] = s;
-            if constexpr (ZP) ((float *)(lds + l.sums))[g * mp + m] = (float)sum * s;
-        }
+        for (int k = 0; k < kPass; ++k)
+            if (i0 - (int)threadIdx.x + k * T < tasks) g4_stage8<BF16, G, ZP>(a, lds, l, raw[k], i0 + k * T, tasks);
     }
     // rows M .. mp - 1: nothing
     for (int i = threadIdx.x; i < a.K / G * mp; i += blockDim.x)
@@ -141,25 +159,53 @@ __device__ __forceinline__ void g4_stage(const G4Args &a, uint8_t *lds, const G4
         }
 }
 
-// One step's weights of a lane: block q of its column, and the scales (zeros) of the
-// step's groups.
-template <int G, bool ZP> struct G4Slot {
-    static constexpr int GS = 128 / G;
+// One step's weights of a lane: block q of its column; and the scales (zeros) of the step's
+// groups, value v of its column (S of group v, then Z) in lane q = v: two or four values a
+// load, handed round by row moves.
+template <bool BF16, int G, bool ZP> struct G4Slot {
+    static constexpr int GS = 128 / G, NV = ZP ? 2 * GS : GS, NL = NV > 4 ? 2 : 1;
     g4_u32x4 w;
-    uint16_t s[GS], z[ZP ? GS : 1];
-    __device__ __forceinline__ void load(const G4Args &a, int step, int n, int q) {
+    uint16_t x[NL];
+    // this lane's first value of step 0 and column 0
+    static __device__ __forceinline__ void base(const G4Args &a, int q, const uint16_t *(&p)[NL]) {
+        if constexpr (NV == 1) p[0] = a.S;
+        else if constexpr (NL == 2) p[0] = a.S + (size_t)q * a.N, p[1] = a.Z + (size_t)q * a.N;
+        else if constexpr (!ZP) p[0] = a.S + (size_t)(q % GS) * a.N;
+        else p[0] = ((q / GS) & 1 ? a.Z : a.S) + (size_t)(q % GS) * a.N;
+    }
+    __device__ __forceinline__ void load(const G4Args &a, const uint16_t *const (&p)[NL], int step, int n, int q) {
         w = __builtin_nontemporal_load((const g4_u32x4 *)(a.B + ((size_t)(4 * step + q) * a.N + n) * 4));
 #pragma unroll
-        for (int j = 0; j < GS; ++j) {
-            s[j] = a.S[(size_t)(step * GS + j) * a.N + n];
-            if constexpr (ZP) z[j] = a.Z[(size_t)(step * GS + j) * a.N + n];
+        for (int i = 0; i < NL; ++i) x[i] = p[i][(size_t)(step * GS) * a.N + n];
+    }
+    // every value of the lane's column: S, then Z, by group
+    __device__ __forceinline__ void values(float (&v)[NV]) const {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const uint32_t f = __float_as_uint(dt2f<BF16>(x[i]));
+            if constexpr (NV == 1) {
+                v[0] = __uint_as_float(f);
+            } else {
+                const auto r = __builtin_amdgcn_permlane16_swap(f, f, false, false);  // even, odd rows' values
+                if constexpr (NV == 2) {
+                    v[0] = __uint_as_float(r[0]);
+                    v[1] = __uint_as_float(r[1]);
+                } else {
+                    const auto e = __builtin_amdgcn_permlane32_swap(r[0], r[0], false, false);  // rows 0, 2
+                    const auto o = __builtin_amdgcn_permlane32_swap(r[1], r[1], false, false);  // rows 1, 3
+                    v[4 * i] = __uint_as_float(e[0]);
+                    v[4 * i + 1] = __uint_as_float(o[0]);
+                    v[4 * i + 2] = __uint_as_float(e[1]);
+                    v[4 * i + 3] = __uint_as_float(o[1]);
+                }
+            }
         }
     }
 };
 
 // RS: sets of four activation rows.
 template <bool BF16, int RS, int G, bool ZP>
-__global__ void __launch_bounds__(64 * kMaxWaves) k_int4_gemv(const G4Args a) {
+__global__ void __launch_bounds__(64 * kMaxWaves, g4_two(RS, G, ZP) ? 8 : 4) k_int4_gemv(const G4Args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int GS = 128 / G, MP = 4 * RS;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
@@ -167,12 +213,21 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_int4_gemv(const G4Args a) {
     const int steps = a.K / 128, strips = a.N / 16, R = 3 * a.M;
     const G4Lds l = g4_lds(a.M, a.K, G, ZP, W);
     const int s0 = steps * w / W, s1 = steps * (w + 1) / W;  // (W <= steps: at least one)
+    // XCD x (workgroups x, x + 8, ...) takes runs of eight strips in a row: four strips share a
+    // 128-byte line of S and Z, which every XCD that reads of it fetches whole (strips dealt
+    // round, M = 1 K = 5120 N = 34816: groups of 64 with zero points 26.0 -> 23.9 us, groups of
+    // 32 33.4 -> 29.1)
+    const int j8 = blockIdx.x >> 3, first = ((j8 >> 3) * 8 + (blockIdx.x & 7)) * 8 + (j8 & 7);
+    if (first >= strips) return;  // (whole workgroup)
     // the loads run kDepth steps ahead of the products, across strips
-    int ls = blockIdx.x, lt = s0;
-    G4Slot<G, ZP> slot[kDepth];
+    int ls = first, lt = s0;
+    typedef G4Slot<BF16, G, ZP> Slot;
+    Slot slot[kDepth];
+    const uint16_t *sp[Slot::NL];
+    Slot::base(a, q, sp);
     auto fetch = [&](int d) __attribute__((always_inline)) {
         if (ls >= strips) return;  // (uniform)
-        slot[d].load(a, lt, 16 * ls + c, q);
+        slot[d].load(a, sp, lt, 16 * ls + c, q);
         if (++lt == s1) {
             lt = s0;
             ls += gridDim.x;
@@ -180,7 +235,7 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_int4_gemv(const G4Args a) {
     };
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) fetch(d);
-    g4_stage<BF16, G, ZP>(a, lds, l);
+    g4_stage<BF16, RS, G, ZP>(a, lds, l);
     g4_barrier();
 
     // matrix row r = lane % 16: digit r % 4 (3: unused) of activation row r / 4
@@ -193,15 +248,11 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_int4_gemv(const G4Args a) {
     const float *scales = (const float *)(lds + l.scales) + q, *sums = (const float *)(lds + l.sums) + q;
     float *red = (float *)(lds + l.red);
     float acc[RS] = {};
-    int strip = blockIdx.x, t = s0, it = 0;
+    int strip = first, t = s0, it = 0;
     auto item = [&](int d) __attribute__((always_inline)) {
         uint32_t w4[4] = {slot[d].w[0], slot[d].w[1], slot[d].w[2], slot[d].w[3]};
-        uint16_t sc[GS], zc[ZP ? GS : 1];
-#pragma unroll
-        for (int j = 0; j < GS; ++j) {
-            sc[j] = slot[d].s[j];
-            if constexpr (ZP) zc[j] = slot[d].z[j];
-        }
+        float sz[Slot::NV];
+        slot[d].values(sz);
         fetch(d);
         if constexpr (G < 128) {
             // lane q's block q (its words 0..3) -> word q of blocks 0..3: a 4 x 4 transpose over q
@@ -246,8 +297,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_int4_gemv(const G4Args a) {
                 const int g = (t * GS + j) * MP + 4 * s;
                 const float f = __builtin_fmaf((float)D[j][0], 65536.0f, __builtin_fmaf((float)D[j][1], 256.0f, (float)D[j][2]));
                 float v = f * scales[g];  // 16 times the group's product
-                if constexpr (ZP) v = __builtin_fmaf(-16.0f * dt2f<BF16>(zc[j]), sums[g], v);
-                acc[s] = __builtin_fmaf(dt2f<BF16>(sc[j]), v, acc[s]);
+                if constexpr (ZP) v = __builtin_fmaf(-16.0f * sz[GS + j], sums[g], v);
+                acc[s] = __builtin_fmaf(sz[j], v, acc[s]);
             }
         }
         if (++t < s1) return;
@@ -303,7 +354,9 @@ ternocl_status int4_gemv_run(int dtype, const void *A, const uint32_t *B, const 
     const G4Args a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other, Bias,
                       M, N, K, postop, out_f32};
     const int waves = g4_waves(K), lds = g4_lds(M, K, group, Z != nullptr, waves).total;
-    const int strips = N / 16, per = lds <= kMaxLds / 2 ? 2 : 1, grid = strips < 256 * per ? strips : 256 * per;
+    // (whole runs of strips over the XCDs)
+    const int strips = N / 16, per = g4_two(M > 4 ? 2 : 1, group, Z != nullptr) && lds <= kMaxLds / 2 ? 2 : 1;
+    const int grid = std::min((strips + 63) / 64 * 64, 256 * per);
     hipError_t e = hipSuccess;
     auto go = [&](auto bf, auto rs, auto g, auto z) {
         auto *k = k_int4_gemv<decltype(bf)::value, decltype(rs)::value, decltype(g)::value, decltype(z)::value>;
