@@ -153,16 +153,11 @@ bool int4_gemv_supports(int M, int K, int group, bool zero);
 ternocl_status int4_gemv_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
                              const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
                              int out_f32, hipStream_t st);
-// kernels (int4_gemm_kw.hip)
-size_t int4_gemm_kw_ws_need(int M, int N, int K);
-ternocl_status int4_gemm_kw_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
-                                const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
-                                int out_f32, void *ws, size_t ws_bytes, hipStream_t st);
-// kernels (int4_gemm_tile.hip)
-bool int4_gemm_tile_wins(int M, int N, int K, int group);
-ternocl_status int4_gemm_tile_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
-                                  const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
-                                  int out_f32, hipStream_t st);
+// kernels (int4_gemm_kw.hip, int4_gemm_tile.hip)
+size_t int4_gemm_ws_need(int M, int N, int K, int group);
+ternocl_status int4_gemm_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                             const void *Other, const void *Bias, int M, int N, int K, int group, int postop, int out_f32,
+                             void *ws, size_t ws_bytes, hipStream_t st);
 // kernels (int4_plain.hip)
 ternocl_status int4_plain_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
                               const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
@@ -701,7 +696,7 @@ static bool int4_group(int group) { return group == 32 || group == 64 || group =
 size_t ternocl_int4_gemm_ws_bytes(int M, int N, int K, int group) {
     if (M < 1 || N < 16 || N % 16 || K < kGS || K % kGS || !int4_group(group)) return 0;
     // (a GEMV takes none; with or without zero points it runs the same shapes but the longest K)
-    return int4_gemv_supports(M, K, group, true) || int4_gemm_tile_wins(M, N, K, group) ? 0 : int4_gemm_kw_ws_need(M, N, K);
+    return int4_gemv_supports(M, K, group, true) ? 0 : int4_gemm_ws_need(M, N, K, group);
 }
 
 ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
@@ -714,11 +709,9 @@ ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, co
     if (((uintptr_t)A & 15) == 0 && int4_gemv_supports(M, K, group, Z != nullptr))
         return int4_gemv_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
     const uintptr_t low = (uintptr_t)A | (uintptr_t)S | (uintptr_t)Z | (uintptr_t)C | (uintptr_t)Other | (uintptr_t)Bias;
-    if ((low & 15) == 0 && int4_gemm_tile_wins(M, N, K, group))
-        return int4_gemm_tile_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
-    if ((low & 15) == 0 && (size_t)256 * K < kMaxBufBytes)
-        return int4_gemm_kw_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, ws, ws_bytes,
-                                (hipStream_t)stream);
+    if ((low & 15) == 0 && (size_t)128 * K < kMaxBufBytes)  // (a tile's rows of A in 32 bits)
+        return int4_gemm_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, ws, ws_bytes,
+                             (hipStream_t)stream);
     return int4_plain_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
 }
 

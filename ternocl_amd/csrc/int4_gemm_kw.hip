@@ -23,6 +23,10 @@
 #include <algorithm>
 
 namespace tcl {
+// (int4_gemm_tile.hip)
+ternocl_status int4_gemm_tile_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                                  const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
+                                  int out_f32, int ksn, float *part, uint64_t *cnt, hipStream_t st);
 namespace {
 
 // The K walk of one wave, units [u0, u1) of its 32 MB rows into acc: kw_walk's way of
@@ -209,31 +213,48 @@ template <class Cfg> hipError_t i4_pick(const I4GemmArgs &a, bool bf, int group,
     return bf ? g(std::true_type{}) : g(std::false_type{});
 }
 
-// ---- host side: tile choice ----------------------------------------------------
+// ---- host side: the choice of tile and K slices ------------------------------------
 
+// A launch's time in us by tile: base, and per round of 256 workgroups slope for each 1024
+// rows of K; for fp16 without zero points / others, groups of 64 and 128 / of 32.  A K
+// split costs 1.2 us and split for each 10^6 of its slices' sums.  Fitted (logarithms, least
+// squares, one fit a class) to 3700 graph-timed calls, M = 9..2048, N = 1024..34816, K =
+// 1024..28672: rms 15% for K over the waves, 8% for the 128 x 256 tiles; the tile chosen by
+// it is 1.4% behind the fastest of all on average (24% at most).  Wider tiles read the
+// activations fewer times; narrower ones fill the chip.  64 x 256, 64 x 128 and 128 x 128
+// tiles with shared activations would gain 0.2% more.
 struct I4Tile {
     int bm, bn;
-    double base, slope;
+    double base[4], slope[4], split;
 };
-constexpr I4Tile kI4Tiles[] = {{32, 32, 4.0, 1.6}, {32, 64, 5.2, 2.2}, {64, 64, 5.0, 3.4}};
+constexpr I4Tile kI4Tiles[] = {{32, 32, {4.2, 4.4, 4.55, 4.7}, {1.77, 1.83, 1.93, 2.12}, 12.4},
+                               {32, 64, {4.6, 4.8, 5.0, 5.2}, {2.54, 2.62, 2.67, 2.95}, 9.2},
+                               {64, 64, {5.3, 5.8, 6.0, 6.2}, {3.6, 4.3, 5.0, 6.2}, 5.5},
+                               {128, 256, {9.2, 9.6, 10.3, 10.45}, {13.95, 18.1, 18.7, 24.6}, 2.05}};
 constexpr int kI4TileCount = sizeof(kI4Tiles) / sizeof(kI4Tiles[0]);
+constexpr int kI4Shared = 3;  // the tile of int4_gemm_tile.hip
 
 struct I4Plan {
     int tile, ks;  // ks: K slices (> 1 needs the workspace)
     double us;
 };
 
-I4Plan i4_plan(int M, int N, int K, bool split) {
+// The cheapest tile and slice count with ws_bytes of workspace.  off: bf16 or zero points.
+I4Plan i4_plan(int M, int N, int K, int group, bool off, size_t ws_bytes) {
     I4Plan best = {-1, 1, 1e30};
+    const int cls = (group == 32 ? 2 : 0) + (off ? 1 : 0);
     for (int i = 0; i < kI4TileCount; ++i) {
         const I4Tile &t = kI4Tiles[i];
         if (t.bm > 32 && t.bm >= 2 * M) continue;  // half the tile's rows idle: a lower one does it
         const long tiles = (long)((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+        if (tiles > 1 << 28) continue;  // (a launch's workgroups)
         for (int ks = 1; ks <= 8; ++ks) {
-            if (ks > 1 && (!split || K / ks < 512 || tiles * ks > 1024 || tiles * 16 > (long)kWsHeader)) break;
+            if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / ks < 512 || tiles * ks > 1024 ||
+                           tiles * 16 > (long)kWsHeader))
+                break;
             const double rounds = (double)((tiles * ks + 255) / 256);
-            double us = t.base * (0.5 + 0.5 * rounds) + t.slope * rounds * K / (1024.0 * ks);
-            if (ks > 1) us += 1.2 + 8e-6 * ks * M * N / 4.0;
+            double us = t.base[cls] + t.slope[cls] * rounds * K / (1024.0 * ks);
+            if (ks > 1) us += 1.2 + t.split * 1e-6 * ks * M * N;
             if (us < best.us - 1e-9) best = {i, ks, us};
         }
     }
@@ -250,22 +271,26 @@ hipError_t i4_run_tile(int tile, const I4GemmArgs &a, bool bf, int group, hipStr
 
 }  // namespace
 
-size_t int4_gemm_kw_ws_need(int M, int N, int K) {
-    const I4Plan p = i4_plan(M, N, K, true);
-    return p.ks == 1 ? 0 : kWsHeader + (size_t)p.ks * M * N * 4;
+// Workspace of a call's K split (0: none), the larger of what it takes by type.
+size_t int4_gemm_ws_need(int M, int N, int K, int group) {
+    int ks = 1;
+    for (int off = 0; off < 2; ++off) ks = std::max(ks, i4_plan(M, N, K, group, off, ~(size_t)0).ks);
+    return ks == 1 ? 0 : kWsHeader + (size_t)ks * M * N * 4;
 }
 
-// (operands 16-byte aligned)
-ternocl_status int4_gemm_kw_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
-                                const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
-                                int out_f32, void *ws, size_t ws_bytes, hipStream_t st) {
-    const bool split = ws && ((uintptr_t)ws & 15) == 0;
-    I4Plan p = i4_plan(M, N, K, split);
-    if (p.ks > 1 && ws_bytes < kWsHeader + (size_t)p.ks * M * N * 4) p = i4_plan(M, N, K, false);
-    const I4GemmArgs a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other,
-                          Bias, M, N, K, postop, out_f32, p.ks,
-                          p.ks > 1 ? (float *)((uint8_t *)ws + kWsHeader) : nullptr, p.ks > 1 ? (uint64_t *)ws : nullptr};
-    return launch_status(i4_run_tile(p.tile, a, dtype == TERNOCL_BF16, group, st));
+// (operands 16-byte aligned; M K and N below 2^31 times a tile's rows and columns)
+ternocl_status int4_gemm_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
+                             const void *Other, const void *Bias, int M, int N, int K, int group, int postop, int out_f32,
+                             void *ws, size_t ws_bytes, hipStream_t st) {
+    const bool bf = dtype == TERNOCL_BF16;
+    const I4Plan p = i4_plan(M, N, K, group, bf || Z, ws && ((uintptr_t)ws & 15) == 0 ? ws_bytes : 0);
+    float *part = p.ks > 1 ? (float *)((uint8_t *)ws + kWsHeader) : nullptr;
+    uint64_t *cnt = p.ks > 1 ? (uint64_t *)ws : nullptr;
+    if (p.tile == kI4Shared)
+        return int4_gemm_tile_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, p.ks, part, cnt, st);
+    const I4GemmArgs a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other, Bias,
+                          M, N, K, postop, out_f32, p.ks, part, cnt};
+    return launch_status(i4_run_tile(p.tile, a, bf, group, st));
 }
 
 }  // namespace tcl

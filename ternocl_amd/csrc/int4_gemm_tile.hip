@@ -26,7 +26,9 @@ struct I4TileArgs {
     void *C;
     const uint16_t *Other;
     const void *Bias;
-    int M, N, K, postop, out_f32;
+    int M, N, K, postop, out_f32, ksn;
+    float *part;     // ksn > 1: [ksn][M][N] slice sums
+    uint64_t *cnt;   // ... and the tiles' arrival counters
 };
 
 // LDS writes are done and every wave is here; global loads in flight stay so.
@@ -37,17 +39,20 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
     constexpr bool OFF = BF16 || ZP;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][Cfg::A_BYTES];
     const int mt = (a.M + Cfg::BM - 1) / Cfg::BM, nt = (a.N + Cfg::BN - 1) / Cfg::BN;
-    int tm, tn;
-    {  // XCD x takes a contiguous range of the tiles, column strip by column strip
-        const int per = (mt * nt + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-        if (t >= mt * nt) return;  // whole workgroup: padding
+    int tm, tn, sl;
+    {  // XCD x takes a contiguous range of the slices' tiles, column strip by column strip
+        const int per = (mt * nt * a.ksn + 7) / 8;
+        int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if (t >= mt * nt * a.ksn) return;  // whole workgroup: padding
+        sl = t / (mt * nt);
+        t -= sl * (mt * nt);
         tn = t / mt;
         tm = t - tn * mt;
     }
     const int m0 = tm * Cfg::BM, n0 = tn * Cfg::BN, mrows = min(Cfg::BM, a.M - m0);
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, q = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % Cfg::WM, wn = wave / Cfg::WM;
-    const int units = a.K / 64;
+    const int units = a.K / 64, u0 = 2 * (int)((long)(units / 2) * sl / a.ksn), u1 = 2 * (int)((long)(units / 2) * (sl + 1) / a.ksn);
     // A: chunk tid + THREADS i of the unit: row / 8, position / 8 swizzled by the row
     const uint16_t *ap[Cfg::LOADS];
     uint32_t ad[Cfg::LOADS];
@@ -145,33 +150,91 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
                         }
         }
     };
-    a_load(0);
-    bs.load(0, 0);
+    a_load(u0);
+    bs.load(u0, 0);
     a_store(0);
-    a_load(1);
-    bs.load(1, 1);
-    for (int u = 0; u < units; u += 2) {  // (K is a multiple of 128)
+    a_load(u0 + 1);
+    bs.load(u0 + 1, 1);
+    for (int u = u0; u < u1; u += 2) {  // (whole 128-row steps)
         unit(u, 0);
         unit(u + 1, 1);
     }
-    epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
-        const int n = n0 + 64 * wn + CB * c;
-        if (n >= a.N) return;
+    const int n = n0 + 64 * wn + CB * c;
+    // this lane's outputs (m, n), (m, n + 1): element r of row block mb
+    auto row_of = [&](int mb, int r) __attribute__((always_inline)) { return 64 * wm + 32 * mb + 8 * (r >> 2) + 4 * q + (r & 3); };
+    if (a.ksn > 1) {  // (uniform) as kw_finish: the last of the tile's slices adds them in order
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = 64 * wm + 32 * mb + 8 * (r >> 2) + 4 * q + (r & 3);
-                if (m >= mrows) continue;
-                const float v[CB] = {acc[mb][0][r], acc[mb][1][r]};
-                kw_store<CB, BF16, decltype(P_)::value, decltype(F_)::value>(a.C, a.Other, a.Bias, a.N, m0 + m, n, v);
+                const int m = row_of(mb, r);
+                if (m >= mrows || n >= a.N) continue;
+                const uint64_t x = (uint64_t)__float_as_uint(acc[mb][0][r]) | ((uint64_t)__float_as_uint(acc[mb][1][r]) << 32);
+                __hip_atomic_store((uint64_t *)(a.part + ((size_t)sl * a.M + m0 + m) * a.N + n), x, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
             }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();  // every wave's sums are stored
+        uint32_t *flag = (uint32_t *)lds[0];
+        if (wave == 0) {
+            const bool last = kw_arrive(a.cnt + 2 * ((size_t)tm * nt + tn), a.ksn, lane);
+            if (lane == 0) *flag = last;
+        }
+        __syncthreads();
+        if (!*flag) return;  // (uniform)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            for (int s = 0; s < a.ksn; ++s) {
+                uint64_t x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    x[r] = __hip_atomic_load((const uint64_t *)(a.part + ((size_t)s * a.M + m0 + min(row_of(mb, r), mrows - 1)) * a.N +
+                                                                min(n, a.N - CB)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float lo = __uint_as_float((uint32_t)x[r]), hi = __uint_as_float((uint32_t)(x[r] >> 32));
+                    acc[mb][0][r] = s ? acc[mb][0][r] + lo : lo;
+                    acc[mb][1][r] = s ? acc[mb][1][r] + hi : hi;
+                }
+            }
+        }
+    }
+    epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
+        constexpr int P = decltype(P_)::value;
+        constexpr bool F32 = decltype(F_)::value;
+        if (n >= a.N) return;
+        float bias[CB] = {0.0f, 0.0f};
+        if constexpr (postop_needs_bias(P))
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                bias[cb] = F32 ? ((const float *)a.Bias)[n + cb] : dt2f<BF16>(((const uint16_t *)a.Bias)[n + cb]);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            // a row block's Other values all in flight (one after the other: 164 against 149 us at M =
+            // 1024 K = 4096 N = 14336, silu(acc) * other)
+            uint32_t o[16] = {};
+            if constexpr (postop_needs_other(P))
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    o[r] = *(const uint32_t *)(a.Other + (size_t)(m0 + min(row_of(mb, r), mrows - 1)) * a.N + n);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = row_of(mb, r);
+                const float x = epi_apply_c<P>(acc[mb][0][r], dt2f<BF16>(o[r] & 0xffffu), bias[0]);
+                const float y = epi_apply_c<P>(acc[mb][1][r], dt2f<BF16>(o[r] >> 16), bias[1]);
+                if (m >= mrows) continue;
+                const size_t i = (size_t)(m0 + m) * a.N + n;
+                if constexpr (F32) *(float2 *)((float *)a.C + i) = make_float2(x, y);
+                else *(uint32_t *)((uint16_t *)a.C + i) = f2dt<BF16>(x) | (f2dt<BF16>(y) << 16);
+            }
+        }
     });
 }
 
 template <class Cfg, bool BF16, int G, bool ZP> hipError_t tile_launch(const I4TileArgs &a, hipStream_t st) {
     const int mt = (a.M + Cfg::BM - 1) / Cfg::BM, nt = (a.N + Cfg::BN - 1) / Cfg::BN;
-    hipLaunchKernelGGL((k_int4_gemm_tile<Cfg, BF16, G, ZP>), dim3(8 * ((mt * nt + 7) / 8)), dim3(Cfg::THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_int4_gemm_tile<Cfg, BF16, G, ZP>), dim3(8 * ((mt * nt * a.ksn + 7) / 8)), dim3(Cfg::THREADS), 0, st, a);
     return hipGetLastError();
 }
 template <class Cfg> hipError_t tile_pick(const I4TileArgs &a, bool bf, int group, hipStream_t st) {
@@ -189,17 +252,13 @@ template <class Cfg> hipError_t tile_pick(const I4TileArgs &a, bool bf, int grou
 
 }  // namespace
 
-// Whether the tiles here are ahead of K over the waves (int4_gemm_kw.hip): where they fill most of the chip.
-bool int4_gemm_tile_wins(int M, int N, int K, int group) {
-    return M > 128 && (long)((M + 127) / 128) * ((N + 255) / 256) >= 128;
-}
-
-// (operands 16-byte aligned)
+// ksn K slices (> 1: their sums in part, the tiles' arrival counters at cnt); operands
+// 16-byte aligned.
 ternocl_status int4_gemm_tile_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
                                   const void *Other, const void *Bias, int M, int N, int K, int group, int postop,
-                                  int out_f32, hipStream_t st) {
-    const I4TileArgs a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other,
-                          Bias, M, N, K, postop, out_f32};
+                                  int out_f32, int ksn, float *part, uint64_t *cnt, hipStream_t st) {
+    const I4TileArgs a = {(const uint16_t *)A, B, (const uint16_t *)S, (const uint16_t *)Z, C, (const uint16_t *)Other, Bias,
+                          M, N, K, postop, out_f32, ksn, part, cnt};
     return launch_status(tile_pick<TileCfg<2, 4>>(a, dtype == TERNOCL_BF16, group, st));
 }
 
