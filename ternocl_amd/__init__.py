@@ -108,10 +108,17 @@ def _dtype_of(t) -> int:
     raise TernoclError(1, f"activations must be float16 or bfloat16, got {t.dtype}")
 
 
+_FLOAT_TYPES: dict = {}  # filled at the first use: torch stays unimported until then
+
+
 def _float_type(t) -> int:
     """The type of a tensor that may be fp32 too (logits, routing weights)."""
-    import torch
-    return FP32 if t.dtype == torch.float32 else _dtype_of(t)
+    v = _FLOAT_TYPES.get(t.dtype)
+    if v is None:
+        import torch
+        _FLOAT_TYPES.update({torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32})
+        v = FP32 if t.dtype == torch.float32 else _dtype_of(t)
+    return v
 
 
 def _nbytes(t) -> int:
@@ -451,7 +458,7 @@ def int4_gemm(A, B, S, Z, C, Other, Bias, M: int, N: int, K: int, group: int = 1
     """C = ct(epi(A x ((q - Z) S))): B int32 [K/32, N, 4] of ``int4_pack``, scales S and zero points Z
     (None: 0) [K/group, N] in A's dtype, the epilogues of ``int2_fp16_upcvt_gemm``.  ``ws``
     (int4_gemm_ws_bytes, 16-byte aligned): the K split of few tiles over a long K."""
-    _check(lib().ternocl_int4_gemm(_dtype_of(A), _ptr(A), _ptr(B), _ptr(S), _ptr(Z), _ptr(C), _ptr(Other), _ptr(Bias),
+    _check(lib().ternocl_int4_gemm(_float_type(A), _ptr(A), _ptr(B), _ptr(S), _ptr(Z), _ptr(C), _ptr(Other), _ptr(Bias),
                                    M, N, K, group, postop, int(bool(out_f32)), _ptr(ws), _nbytes(ws), _stream(stream)))
 
 

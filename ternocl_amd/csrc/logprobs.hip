@@ -128,9 +128,9 @@ struct LpState {
         r = t = 0.0f;
     }
     // n entries of each lane (padding: -inf) whose lane maximum is tm
-    template <int n> __device__ __forceinline__ void add(const float (&x)[n], float tm, float c, int lane) {
+    template <int n> __device__ __forceinline__ void add(float (&x)[n], float tm, float c, int lane) {
         const float wm = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(lp_wave_max(tm, lane))));
-        if (wm > m) {  // (uniform) a new maximum: one of its entries is left out below
+        if (wm > m) {  // (uniform) a new maximum
             if (m != -__builtin_inff()) {
                 // the lanes' sums so far, and the old maximum's own term in lane 0
                 const float d = (m - wm) * c, f = __builtin_amdgcn_exp2f(d);
@@ -139,14 +139,13 @@ struct LpState {
                 r = f * old;
             }
             m = wm;
-            const bool skip = lane == __builtin_ctzll(__ballot(tm == wm));
-            bool done = !skip;
+            bool done = lane != __builtin_ctzll(__ballot(tm == wm));  // one of its entries is left out
 #pragma unroll
             for (int i = 0; i < n; ++i) {
-                if (!done && x[i] == wm) done = true;
-                else lp_term(x[i], m, c, r, t);
+                const bool hit = !done && x[i] == wm;
+                x[i] = hit ? -__builtin_inff() : x[i];
+                done |= hit;
             }
-            return;
         }
         if (m == -__builtin_inff()) {  // only -inf so far (or NaN: its r must show it)
 #pragma unroll
@@ -276,15 +275,11 @@ template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<L
     }
 }
 
-// The token asked for and its logit (loaded early: two loads, one after the other).
-template <int LT> struct LpToken {
-    int tok;
-    float x;
-    __device__ __forceinline__ LpToken(const LpArgs &a, const LpRow<LT> &row, int m) : tok(a.tokens ? a.tokens[m] : -1) {
-        if (tok >= a.V) tok = -1;
-        x = lp_load1<LT>(row.p, max(tok, 0));
-    }
-};
+// The token asked for (-1: none).
+__device__ __forceinline__ int lp_token(const LpArgs &a, int m) {
+    const int tok = a.tokens ? a.tokens[m] : -1;
+    return tok < a.V ? tok : -1;
+}
 
 // The maxima of a row's pieces, two of one piece row in a load: thread t has pairs t + 256 i
 // of [pieces][128] pairs.
@@ -305,7 +300,7 @@ struct LpMaxima {
 // vectors p span + t + 256 i, i < span / 256 (and, with p = 0, edge entry t).
 template <int LT, bool TOP>
 __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row, int m, const LpSum &s,
-                                          const LpToken<LT> &token, const LpMaxima &pm, int pieces, int span, LpLds &L) {
+                                          int tok, float tok_x, const LpMaxima &pm, int pieces, int span, LpLds &L) {
     constexpr int NV = LpVec<LT>::NV;
     const int tid = threadIdx.x, lane = tid & 63;
     const bool empty = s.m == -__builtin_inff() && s.r == 0.0f;
@@ -313,8 +308,8 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     const float l1 = log1pf(s.r), nan = __builtin_nanf("");
     if (tid == 0) {
         if (a.logp) {
-            const float o = bad ? nan : empty ? -__builtin_inff() : (token.x - s.m) * a.scale - l1;
-            a.logp[m] = token.tok < 0 ? 0.0f : o;
+            const float o = bad ? nan : empty ? -__builtin_inff() : (tok_x - s.m) * a.scale - l1;
+            a.logp[m] = tok < 0 ? 0.0f : o;
         }
         if (a.entropy)
             a.entropy[m] = bad ? nan : empty ? 0.0f : l1 - s.t * 0.693147180559945309f / (1.0f + s.r);
@@ -340,8 +335,8 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     uint32_t o4[4], found = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o4[i] = L.thread[64 * i + lane];
-#pragma unroll
-    for (int bit = 15; bit >= 0; --bit) {
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {  // (rolled, as below: a few rows' call is as long as its code takes to fetch)
         const uint32_t t = found | (1u << bit);
         int n = 0;
 #pragma unroll
@@ -350,13 +345,14 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     }
     const uint32_t bound = found << 16;  // (of lp_ord; a row with fewer entries than topn above -inf: 0x007f << 16)
     // the pieces that hold entries at or above it
-    if (lp_ord(v) >= bound)
+    uint32_t hits = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * kPairs; ++i)
-            if (pm.x[i] > -__builtin_inff() && lp_ord(pm.x[i]) >= bound) {
-                const int n = atomicAdd(&L.flags, 1);
-                if (n < kFlags) L.flag[n] = (uint32_t)(2 * (tid + kThreads * (i >> 1)) + (i & 1));
-            }
+    for (int i = 0; i < 2 * kPairs; ++i) hits |= (uint32_t)(pm.x[i] > -__builtin_inff() && lp_ord(pm.x[i]) >= bound) << i;
+    while (hits) {
+        const int i = __builtin_ctz(hits), n = atomicAdd(&L.flags, 1);
+        if (n < kFlags) L.flag[n] = (uint32_t)(2 * (tid + kThreads * (i >> 1)) + (i & 1));
+        hits &= hits - 1;
+    }
     __syncthreads();
     const int flags = L.flags, per = span / kThreads + 1;  // (the last: the edge)
     // those of n entries (indices i0 + their place) into the list, one addition to its count
@@ -452,7 +448,7 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
     __shared__ std::conditional_t<TOP, LpLds, int> L;
     const int m = blockIdx.x, tid = threadIdx.x;
     const LpRow<LT> row(a.logits, a.ld, m, a.V);
-    const LpToken<LT> token(a, row, m);
+    const int tok = lp_token(a, m);  // (used only after the stream)
     const float c = a.scale * 1.44269504088896341f;
     if constexpr (TOP)
         for (int p = 1; p < pieces; ++p) lp_pm[p * kThreads + tid] = -__builtin_inff();
@@ -463,9 +459,10 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
     LpSum s = wsum[0];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) s = lp_join(s, wsum[i], c);
+    const float tok_x = lp_load1<LT>(row.p, max(tok, 0));
     LpMaxima pm;
     if constexpr (TOP) pm.load(pieces, [&](int j) __attribute__((always_inline)) { return ((const float2 *)lp_pm)[j]; });
-    lp_finish<LT, TOP>(a, row, m, s, token, pm, pieces, bpp * kThreads * kU, reinterpret_cast<LpLds &>(L));
+    lp_finish<LT, TOP>(a, row, m, s, tok, tok_x, pm, pieces, bpp * kThreads * kU, reinterpret_cast<LpLds &>(L));
 }
 
 __device__ __forceinline__ void lp_put(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -480,7 +477,7 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
     __shared__ int flag;
     const int m = blockIdx.y, k = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const LpRow<LT> row(a.logits, a.ld, m, a.V);
-    const LpToken<LT> token(a, row, m);
+    const int tok = lp_token(a, m);  // (used only after the stream)
     const float c = a.scale * 1.44269504088896341f;
     const int v0 = min(k * a.chunk_vecs, row.nvec), v1 = min(row.nvec, v0 + a.chunk_vecs);
     float *sums = a.sums + 3 * (size_t)m * a.chunks, *maxima = a.maxima + (size_t)m * a.chunks * kThreads;
@@ -505,6 +502,7 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
     }
     __syncthreads();
     if (!flag) return;  // (uniform)
+    const float tok_x = lp_load1<LT>(row.p, max(tok, 0));
     LpMaxima pm;
     if constexpr (TOP)
         pm.load(a.chunks, [&](int j) __attribute__((always_inline)) {
@@ -513,13 +511,15 @@ template <int LT, bool TOP> __global__ void __launch_bounds__(kThreads) k_logpro
         });
     s = LpSum{-__builtin_inff(), 0.0f, 0.0f};
     if (lane < a.chunks) s = LpSum{lp_get(sums + 3 * lane), lp_get(sums + 3 * lane + 1), lp_get(sums + 3 * lane + 2)};
-#pragma unroll
-    for (int d = 1; d < kPieces; d <<= 1) {
-        const LpSum o = {__shfl_xor(s.m, d, 64), __shfl_xor(s.r, d, 64), __shfl_xor(s.t, d, 64)};
-        s = (lane & d) ? lp_join(o, s, c) : lp_join(s, o, c);  // (the lower lane's first: alike in both)
+    {  // the chunks' sums, one a lane, relative to the largest maximum (lp_join, all at once)
+        const float top = lp_wave_max(s.m, lane);
+        const bool one = lane == __builtin_ctzll(__ballot(s.m == top));  // (its own term left out)
+        const bool none = s.m == -__builtin_inff();
+        const float d = none ? 0.0f : (s.m - top) * c, f = none ? 0.0f : __builtin_amdgcn_exp2f(d), n = 1.0f + s.r;
+        const float r = none || one ? s.r : f * n, t = one ? s.t : f > 0.0f ? f * (s.t + d * n) : 0.0f;
+        s = LpSum{top, lp_wave_sum(r, lane), lp_wave_sum(t, lane)};
     }
-    s = LpSum{__shfl(s.m, 0, 64), __shfl(s.r, 0, 64), __shfl(s.t, 0, 64)};
-    lp_finish<LT, TOP>(a, row, m, s, token, pm, a.chunks, a.chunk_vecs, reinterpret_cast<LpLds &>(L));
+    lp_finish<LT, TOP>(a, row, m, s, tok, tok_x, pm, a.chunks, a.chunk_vecs, reinterpret_cast<LpLds &>(L));
 }
 
 // Workgroups a row is spread over (nv: entries of a vector): as many as whole batches
