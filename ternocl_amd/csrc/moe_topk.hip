@@ -6,8 +6,10 @@
 //   of those (renormalised), times scale.
 //
 // L lanes take a token (64 / L tokens a wave), lane i of them holding experts i, i + L, ...
-// topk rounds pick the largest value (a maximum over the lanes), the lowest index that has
-// it (a minimum over those), and drop it.
+// With L = 64, topk rounds pick the largest value (a maximum over the lanes), the lowest index
+// that has it (a minimum over those), and drop it: the shortest way for one token.  With L =
+// 16 the values that can be among the topk go to a list that is ranked at once: a third
+// of the rounds' instructions.
 //   * Without a bias the logits themselves order the experts -- softmax and the sigmoid
 //     rise with them, and in exact arithmetic only equal logits give equal scores -- so the
 //     rounds compare fp32 logits, exactly.
@@ -291,8 +293,9 @@ template <int VX> __device__ __forceinline__ void tk_exact(const TkArgs &a, int 
 // them: lane i holds experts i VPL .. + VPL - 1 then.
 template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
     constexpr int TPW = 64 / L, VX = VPL * L / 64 > 0 ? VPL * L / 64 : 1;
-    // a wave's values [tokens][L VPL] while groups are valued, tk_exact's keys
-    __shared__ u64 space[kTkWaves][(TPW * L * VPL + 1) / 2 > 64 * VX ? (TPW * L * VPL + 1) / 2 : 64 * VX];
+    // a wave's values [tokens][L VPL] while groups are valued; its tokens' lists [32] and
+    // picks in order [16]; tk_exact's keys
+    __shared__ __attribute__((aligned(16))) u64 space[kTkWaves][std::max({(TPW * L * VPL + 1) / 2, 64 * VX, L == 16 ? 192 : 0})];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sub = lane % L, tok = lane / L;
     const int t0 = (blockIdx.x * kTkWaves + w) * TPW, t = t0 + tok;
@@ -414,6 +417,16 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         }
 #pragma unroll
         for (int j = 0; j < VPL; ++j) v[j] = keep ? v[j] : kNone;
+        if constexpr (L == 16) {
+            // dealt to the lanes as without groups: kept ones fill a few lanes otherwise
+            int *deal = (int *)space[w] + tok * L * VPL;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < VPL; j += 4) *(int4 *)(deal + VPL * sub + j) = make_int4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) v[j] = deal[sub + L * j];
+        }
     }
     if constexpr (GROUPED == 1) {
         const int per = a.E / a.n_group;
@@ -481,41 +494,111 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         for (int j = 0; j < VPL; ++j)
             if (!((kept >> (int)(((float)min(sub + L * j, a.E - 1) + 0.5f) * inv)) & 1)) v[j] = kNone;
     }
-    // the rounds
-    // With a bias they go on past topk until a pick is apart from the next value, and the
-    // picks are put in order by their 64-bit values where two are not.
-    float last = __builtin_inff();
-    bool close = false, settled = false;  // (alike in a token's lanes)
-    int id = -1, pick = kNone;  // lane r: round r's expert and what it was chosen by
-    for (int r = 0; a.bias || r < a.topk; ++r) {
+    bool close = false;  // picks to be put in order by their 64-bit values (alike in a token's lanes)
+    int id = -1, pick = kNone;  // lane r: the r-th largest value's expert, and the value
+    if constexpr (L == 16) {
+        // The need-th largest of the 16 lanes' maxima is a bound that at least need values
+        // reach (13 or so of 256 for need = 10): those go to a list, whose 64-bit keys (value,
+        // lowest index) are ranked each against all.  More than kList: tk_exact.
+        constexpr int kList = 32;
+        const int need = a.topk + (a.bias ? 2 : 0);  // (<= 16)
         int best = v[0];
 #pragma unroll
         for (int j = 1; j < VPL; ++j) best = max(best, v[j]);
-        const int m = tk_lanes<L>(best, lane, tk_imax2);
-        if (a.bias) {
-            const float x = tk_float(m);
-            const bool apart = m == kNone || last - x > tk_margin(last, a.score);
-            settled |= r >= a.topk && apart;
-            if (r >= a.topk && __ballot(!settled) == 0) break;  // (uniform)
-            if (r == L) {  // more close values than lanes
-                odd |= !settled;
-                break;
+        int above = 0;
+        auto turn = [&](auto i) __attribute__((always_inline)) {  // (row_ror i)
+            above += __builtin_amdgcn_mov_dpp(best, 0x120 + decltype(i)::value, 0xf, 0xf, true) > best;
+        };
+        turn(std::integral_constant<int, 1>{}), turn(std::integral_constant<int, 2>{}), turn(std::integral_constant<int, 3>{});
+        turn(std::integral_constant<int, 4>{}), turn(std::integral_constant<int, 5>{}), turn(std::integral_constant<int, 6>{});
+        turn(std::integral_constant<int, 7>{}), turn(std::integral_constant<int, 8>{}), turn(std::integral_constant<int, 9>{});
+        turn(std::integral_constant<int, 10>{}), turn(std::integral_constant<int, 11>{}), turn(std::integral_constant<int, 12>{});
+        turn(std::integral_constant<int, 13>{}), turn(std::integral_constant<int, 14>{}), turn(std::integral_constant<int, 15>{});
+        const int bound = max(tk_lanes<L>(above < need ? best : 0x7fffffff, lane, tk_imin2), kNone + 1);
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) count += v[j] >= bound;
+        // places in the list: the counts of the lanes before (row_shr 1, 2, 4, 8: 0 comes in)
+        int place = count;
+        place += __builtin_amdgcn_update_dpp(0, place, 0x111, 0xf, 0xf, true);
+        place += __builtin_amdgcn_update_dpp(0, place, 0x112, 0xf, 0xf, true);
+        place += __builtin_amdgcn_update_dpp(0, place, 0x114, 0xf, 0xf, true);
+        place += __builtin_amdgcn_update_dpp(0, place, 0x118, 0xf, 0xf, true);
+        const int total_n = tk_lanes<L>(place, lane, tk_imax2);  // (the last lane's)
+        place -= count;
+        odd |= total_n > kList;
+        u64 *list = space[w] + tok * kList, *order = space[w] + TPW * kList + tok * L;
+        __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+        list[sub] = list[sub + L] = order[sub] = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (v[j] >= bound) {
+                if (place < kList) list[place] = ((u64)((uint32_t)v[j] ^ 0x80000000u) << 32) | (uint32_t)~(sub + L * j);
+                ++place;
             }
-            close |= !settled && r > 0 && !apart;
-            last = x;
-        } else if (__ballot(m != kNone) == 0) {
-            break;  // (uniform)
+        __builtin_amdgcn_wave_barrier();
+        const u64 k0 = list[sub], k1 = list[sub + L];
+        int r0 = 0, r1 = 0;
+        for (int i = 0; i < kList; i += 2) {
+            if (__ballot(i < total_n) == 0) break;  // (uniform)
+            const ulonglong2 o = *(const ulonglong2 *)(list + i);
+            r0 += (o.x > k0) + (o.y > k0);
+            r1 += (o.x > k1) + (o.y > k1);
         }
-        int e = 1 << 20;
+        if (k0 && r0 < L) order[r0] = k0;
+        if (k1 && r1 < L) order[r1] = k1;
+        __builtin_amdgcn_wave_barrier();
+        const u64 k = order[sub];
+        int last = a.topk - 1;  // the last pick
+        if (a.bias) {
+            // a pick too close to the next one (the 16th: not known)
+            const u64 next = order[min(sub + 1, L - 1)];
+            const float x = tk_float((int)((uint32_t)(k >> 32) ^ 0x80000000u)), y = tk_float((int)((uint32_t)(next >> 32) ^ 0x80000000u));
+            const bool amb = k != 0 && (sub == L - 1 ? total_n > L : next != 0 && !(x - y > tk_margin(x, a.score)));
+            const uint32_t near = (uint32_t)(__ballot(amb) >> (L * tok)) & 0xffffu;
+            last = __builtin_ctz(~near & ~((1u << (a.topk - 1)) - 1));  // (16: none of them is apart)
+            odd |= last >= L;
+            close = (near & ((1u << min(last, L - 1)) - 1)) != 0;
+        }
+        if (k && sub <= last) {
+            id = (int)~(uint32_t)k;
+            pick = (int)((uint32_t)(k >> 32) ^ 0x80000000u);
+        }
+    } else {
+        // topk rounds: the largest value, of equal ones the lowest index.  With a bias they go on
+        // until a pick is apart from the next value.
+        float last = __builtin_inff();
+        bool settled = false;  // (alike in a token's lanes)
+        for (int r = 0; a.bias || r < a.topk; ++r) {
+            int best = v[0];
 #pragma unroll
-        for (int j = VPL - 1; j >= 0; --j) e = v[j] == m ? E0 * sub + ES * j : e;
-        e = tk_lanes<L>(e, lane, tk_imin2);
-        const int at = e - E0 * sub;
+            for (int j = 1; j < VPL; ++j) best = max(best, v[j]);
+            const int m = tk_lanes<L>(best, lane, tk_imax2);
+            if (a.bias) {
+                const float x = tk_float(m);
+                const bool apart = m == kNone || last - x > tk_margin(last, a.score);
+                settled |= r >= a.topk && apart;
+                if (r >= a.topk && __ballot(!settled) == 0) break;  // (uniform)
+                if (r == L) {  // more close values than lanes
+                    odd |= !settled;
+                    break;
+                }
+                close |= !settled && r > 0 && !apart;
+                last = x;
+            } else if (__ballot(m != kNone) == 0) {
+                break;  // (uniform)
+            }
+            int e = 1 << 20;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) v[j] = at == ES * j ? kNone : v[j];
-        if (sub == r && m != kNone && !settled) {
-            id = e;
-            pick = m;
+            for (int j = VPL - 1; j >= 0; --j) e = v[j] == m ? E0 * sub + ES * j : e;
+            e = tk_lanes<L>(e, lane, tk_imin2);
+            const int at = e - E0 * sub;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) v[j] = at == ES * j ? kNone : v[j];
+            if (sub == r && m != kNone && !settled) {
+                id = e;
+                pick = m;
+            }
         }
     }
     float lv = tk_float(pick);
@@ -576,7 +659,7 @@ ternocl_status moe_topk_run(int ltype, const void *logits, long ld, const float 
                             int E, int topk, int score, int n_group, int topk_group, int group_best, int renorm,
                             float scale, hipStream_t st) {
     const TkArgs a = {logits, bias, ids, RW, ld, ltype, T, E, topk, wtype, score, n_group, topk_group, group_best, renorm, scale};
-    if (T >= kTkMany && topk <= 16) {
+    if (T >= kTkMany && topk + (bias ? 2 : 0) <= 16) {
         if (E <= 64) tk_launch<16, 4>(a, st);
         else if (E <= 128) tk_launch<16, 8>(a, st);
         else if (E <= 256) tk_launch<16, 16>(a, st);
