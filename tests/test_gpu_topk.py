@@ -101,6 +101,27 @@ def test_many_tokens(dev, Tk, E, n_group, topk_group, group_best):
     x[5, 7], x[9, 1:] = -math.inf, -math.inf
     check(T, x, b, 6, "f32", "sigmoid", n_group, topk_group, group_best, True, 2.5)
     check(T, x, None, 6, "bf16", "softmax", n_group, topk_group, group_best, False)
+    if topk_group * (E // n_group) >= 20:
+        check(T, x[:500], b, 14, "f32", "sigmoid", n_group, topk_group, group_best)
+        check(T, x[:500], b, 15, "f32", "sigmoid", n_group, topk_group, group_best)
+        check(T, x[:500], None, 16, "f32", "softmax", n_group, topk_group, group_best)
+        check(T, x[:500], None, 17, "f32", "softmax", n_group, topk_group, group_best)
+
+
+@pytest.mark.parametrize("biased", [False, True])
+def test_equal_and_uneven_rows(dev, biased):
+    """Rows of one value, of few, and with all large values in the same places of every 16."""
+    import ternocl_amd as T
+    g = torch.Generator().manual_seed(4)
+    x = torch.zeros(40, 256)
+    x[10:20] = torch.randint(0, 3, (10, 256), generator=g).float()
+    x[20:30] = torch.randn(10, 256, generator=g)
+    x[20:30, 3::16] += 8
+    x[30:] = torch.randn(10, 256, generator=g) - 300
+    b = torch.randint(-1, 2, (256,), generator=g) * 0.25 if biased else None
+    for score in ("softmax", "sigmoid"):
+        check(T, x, b, 8, "f32", score)
+        check(T, x, b, 8, "f32", score, 8, 2, 1)
 
 
 @pytest.mark.parametrize("E,n_group,topk_group", [(64, 8, 4), (64, 8, 8), (256, 8, 4), (160, 8, 3), (512, 64, 7), (48, 3, 1),
