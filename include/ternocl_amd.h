@@ -490,10 +490,12 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
  *          value (NULL: 0)
  * Codes, activations and zero points are multiplied as they are and summed in fp32
  * (or exact integers) per group; nothing is rounded to DT before the epilogue.  A
- * row of A that holds an infinity or a NaN gives infinities or NaN.
+ * row of A that holds an infinity or a NaN has infinities or NaN for its sums, before
+ * the epilogue; no other row is changed by it.
  * N % 16 == 0, K % 128 == 0, any M >= 1.  B starts on 16 bytes.  M <= 8 runs the
- * decode GEMV and larger M the matrix-core GEMM where the other operands are
- * 16-byte aligned too, a plain kernel otherwise.
+ * decode GEMV (A 16-byte aligned; K M up to some 50000), other calls a matrix-core
+ * GEMM where every operand is 16-byte aligned, a plain kernel (several times slower)
+ * otherwise.
  * ws / ws_bytes: optional device scratch of ternocl_int4_gemm_ws_bytes(M, N, K,
  * group) bytes (0: none used), 16-byte aligned, laid out and used as
  * ternocl_int2_fp16_upcvt_gemm's: a deterministic K split of few tiles over a long
@@ -527,7 +529,7 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
  * weights.  Weights whose sum is 0 renormalise to 0.
  * logits: ltype [T, E] (TERNOCL_FP16, _BF16 or _FP32) with ld elements from row to
  * row (ld >= E); wtype: the same three.
- * T >= 1, 1 <= E <= 512, 1 <= n_group <= 64 dividing E, 1 <= topk_group <= n_group,
+ * 1 <= T <= 2^25, 1 <= E <= 512, 1 <= n_group <= 64 dividing E, 1 <= topk_group <= n_group,
  * group_best <= E / n_group, 1 <= topk <= min(64, topk_group * E / n_group). */
 ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const float *bias, int *ids, int wtype,
                                 void *RW, int T, int E, int topk, int score, int n_group, int topk_group,
@@ -545,7 +547,7 @@ ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const
  * over get id -1 and -inf.  A row of -inf alone gives logp -inf, entropy 0, ids -1; a
  * row with a NaN or +inf gives NaN, ids -1.
  * logits: ltype [M, V] with ld elements from row to row (ld >= V), its rows at any
- * element alignment.  M >= 1, V >= 1, 0 <= topn <= 64, scale > 0 and finite.
+ * element alignment.  1 <= M <= 2^23, V >= 1, 0 <= topn <= 64, scale > 0 and finite.
  * ws: optional scratch of ternocl_logprobs_ws_bytes(M, V, topn) bytes (0: none used),
  * 16-byte aligned, any contents: rows are spread over workgroups where there are few,
  * their sums joined by the last (arrival counters in the header, left zero).  NULL or

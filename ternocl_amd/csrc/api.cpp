@@ -728,8 +728,9 @@ ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const
     if (score != 0 && score != 1) FAIL(TERNOCL_ERR_INVALID_ARG, "score must be 0 (softmax) or 1 (sigmoid)");
     if (renorm != 0 && renorm != 1) FAIL(TERNOCL_ERR_INVALID_ARG, "renorm must be 0 or 1");
     if (!std::isfinite(scale)) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be finite");
-    if (T < 1 || E < 1 || E > 512) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need T >= 1 and 1 <= E <= 512");
+    if (T < 1 || T > 1 << 25 || E < 1 || E > 512) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need 1 <= T <= 2^25 and 1 <= E <= 512");
     if (ld < E) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ld must be at least E");
+    if ((uintptr_t)logits % (ltype == TERNOCL_FP32 ? 4 : 2)) FAIL(TERNOCL_ERR_INVALID_ARG, "logits must be aligned to its element");
     if (n_group < 1 || n_group > 64 || E % n_group) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "n_group must be 1..64 and divide E");
     if (topk_group < 1 || topk_group > n_group) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "topk_group must be 1..n_group");
     if (group_best < 1 || group_best > 2 || group_best > E / n_group)
@@ -755,7 +756,7 @@ ternocl_status ternocl_logprobs(int ltype, const void *logits, int64_t ld, const
     if (topn && (!top_ids || !top_logp)) FAIL(TERNOCL_ERR_INVALID_ARG, "topn > 0 writes top_ids and top_logp: both must be non-null");
     if (!logp && !entropy && !topn) FAIL(TERNOCL_ERR_INVALID_ARG, "nothing to compute: logp, entropy and topn are all absent");
     if (!(scale > 0.0f) || !std::isfinite(scale)) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be positive and finite");
-    if (M < 1 || V < 1) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "M and V must be positive");
+    if (M < 1 || M > 1 << 23 || V < 1) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need 1 <= M <= 2^23 and V >= 1");
     if (ld < V) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ld must be at least V");
     const uintptr_t es = ltype == TERNOCL_FP32 ? 4 : 2;
     if ((uintptr_t)logits % es) FAIL(TERNOCL_ERR_INVALID_ARG, "logits must be aligned to its element");

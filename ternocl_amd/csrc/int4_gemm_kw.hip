@@ -247,7 +247,7 @@ I4Plan i4_plan(int M, int N, int K, int group, bool off, size_t ws_bytes) {
         const I4Tile &t = kI4Tiles[i];
         if (t.bm > 32 && t.bm >= 2 * M) continue;  // half the tile's rows idle: a lower one does it
         const long tiles = (long)((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-        if (tiles > 1 << 28) continue;  // (a launch's workgroups)
+        if (tiles > 8000000) continue;  // (a launch's threads: 32 bits)
         for (int ks = 1; ks <= 8; ++ks) {
             if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / ks < 512 || tiles * ks > 1024 ||
                            tiles * 16 > (long)kWsHeader))
@@ -284,6 +284,10 @@ ternocl_status int4_gemm_run(int dtype, const void *A, const uint32_t *B, const 
                              void *ws, size_t ws_bytes, hipStream_t st) {
     const bool bf = dtype == TERNOCL_BF16;
     const I4Plan p = i4_plan(M, N, K, group, bf || Z, ws && ((uintptr_t)ws & 15) == 0 ? ws_bytes : 0);
+    if (p.tile < 0) {
+        set_error("M x N needs more tiles than a launch holds");
+        return TERNOCL_ERR_UNSUPPORTED_SHAPE;
+    }
     float *part = p.ks > 1 ? (float *)((uint8_t *)ws + kWsHeader) : nullptr;
     uint64_t *cnt = p.ks > 1 ? (uint64_t *)ws : nullptr;
     if (p.tile == kI4Shared)

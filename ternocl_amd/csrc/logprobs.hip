@@ -538,10 +538,14 @@ int lp_chunks(int M, int V, int nv, int &chunk_vecs) {
 
 }  // namespace
 
-size_t logprobs_ws_need(int M, int V, int topn) {
+static size_t lp_ws(int M, int V, int topn, int nv) {
     int cv;
-    const int c = lp_chunks(M, V, 4, cv);  // (16-bit rows have fewer)
+    const int c = lp_chunks(M, V, nv, cv);
     return c == 1 ? 0 : kWsHeader + (size_t)M * c * (12 + (topn ? 4 * kThreads : 0)) + 4;
+}
+size_t logprobs_ws_need(int M, int V, int topn) {  // (whichever the type)
+    const size_t a = lp_ws(M, V, topn, 4), b = lp_ws(M, V, topn, 8);
+    return a > b ? a : b;
 }
 
 ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *tokens, float *logp, float *entropy,
@@ -549,7 +553,7 @@ ternocl_status logprobs_run(int ltype, const void *logits, long ld, const int *t
                             size_t ws_bytes, hipStream_t st) {
     LpArgs a = {logits, ld, tokens, logp, entropy, top_ids, top_logp, M, V, topn, scale, 1, 0, nullptr, nullptr, nullptr};
     const int nv = ltype == TERNOCL_FP32 ? 4 : 8;
-    const size_t need = logprobs_ws_need(M, V, topn);
+    const size_t need = lp_ws(M, V, topn, nv);
     if (need && ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0) a.chunks = lp_chunks(M, V, nv, a.chunk_vecs);
     const bool split = a.chunks > 1;
     if (split) {

@@ -221,3 +221,23 @@ def test_ops_match_direct_calls(dev):
         torch.ops.ternocl.int4_gemm(A.cuda(), B, S.cuda(), None, 32, None, None, 3, False)  # no bias
     torch.library.opcheck(torch.ops.ternocl.int4_gemm.default, (A.cuda(), B, S.cuda(), Z.cuda(), 32, None, None, 0, False),
                           test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("M", [2, 12])
+def test_offsets_past_32_bits(dev, M):
+    """Weights of more than 2^32 bytes: the columns at both ends."""
+    import ternocl_amd as T
+    K, N, group = 4096, (1 << 21) + 48 * 1024, 128
+    A, _, _, _, dt = make(5, M, K, 16, group, True, False)
+    A = A.cuda()
+    B = torch.randint(-2**31, 2**31 - 1, (K // 32, N, 4), dtype=torch.int32, device="cuda")
+    S = (torch.rand((K // group, N), device="cuda") * 0.01 + 0.005).to(dt)
+    assert B.numel() * 4 > 2**32
+    C = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    T.int4_gemm(A, B, S, None, C, None, None, M, N, K, group, 0, True)
+    torch.cuda.synchronize()
+    for n0 in (0, N // 2, N - 64):
+        cols = slice(n0, n0 + 64)
+        W = T.int4_unpack(B[:, cols].contiguous().cpu().numpy().view(np.uint32), K)
+        want, d = gold(A.cpu(), torch.from_numpy(W), S[:, cols].cpu(), None, group, None, None, 0)
+        assert ((C[:, cols].cpu().double() - want).abs() <= 2.0**-24 * want.abs() + d).all()

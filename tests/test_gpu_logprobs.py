@@ -236,6 +236,22 @@ def test_op_graph_and_stream(dev):
     torch.library.opcheck(op.default, (x, t, 10, 0.9), test_utils=("test_schema", "test_faketensor"))
 
 
+def test_offsets_past_32_bits(dev):
+    """Rows past 2^32 bytes and 2^31 elements: the first and the last."""
+    import ternocl_amd as T
+    M, V = 15000, 151680
+    x = torch.randn((M, V), dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2**31
+    t = torch.randint(0, V, (M,), dtype=torch.int32, device="cuda")
+    lp, H = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    ids, tl = torch.empty((M, 3), dtype=torch.int32, device="cuda"), torch.empty((M, 3), device="cuda")
+    T.logprobs(x, t, lp, H, ids, tl, M, V, topn=3)
+    for r in ([0, 1], [M // 2, M // 2 + 1], [M - 2, M - 1]):
+        glp, gH, gids, gtl = gold(x[r].cpu(), t[r].cpu(), 3, 1.0)
+        assert torch.equal(ids[r].cpu(), gids) and torch.allclose(lp[r].cpu().double(), glp, atol=1e-4)
+        assert torch.allclose(H[r].cpu().double(), gH, atol=1e-4) and torch.allclose(tl[r].cpu().double(), gtl, atol=1e-4)
+
+
 @pytest.mark.parametrize("Tk", [1, 5, 70])
 def test_decode_step(dev, Tk):
     """The calls as a model makes them: router logits -> moe_topk -> the ternary MoE layer -> a 4-bit head ->

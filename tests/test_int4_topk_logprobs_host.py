@@ -77,7 +77,7 @@ def _topk(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(ltype=3), INVALID), (dict(wtype=-1), INVALID), (dict(logits=None), INVALID), (dict(ids=None), INVALID),
     (dict(RW=None), INVALID), (dict(score=2), INVALID), (dict(renorm=2), INVALID), (dict(scale=float("nan")), INVALID),
-    (dict(scale=float("inf")), INVALID), (dict(T=0), SHAPE), (dict(E=0), SHAPE), (dict(E=513, ld=513), SHAPE),
+    (dict(scale=float("inf")), INVALID), (dict(T=0), SHAPE), (dict(T=2**25 + 1), SHAPE), (dict(logits=4098), INVALID), (dict(ltype=0, logits=4097), INVALID), (dict(E=0), SHAPE), (dict(E=513, ld=513), SHAPE),
     (dict(ld=63), SHAPE), (dict(n_group=0), SHAPE), (dict(n_group=5), SHAPE), (dict(E=128, ld=128, n_group=128), SHAPE),
     (dict(n_group=4, topk_group=5), SHAPE), (dict(topk_group=0), SHAPE), (dict(group_best=0), SHAPE),
     (dict(group_best=3), SHAPE), (dict(n_group=64, topk_group=8, group_best=2), SHAPE), (dict(topk=0), SHAPE),
@@ -98,7 +98,7 @@ def _logprobs(**kw):
     (dict(ltype=7), INVALID), (dict(logits=None), INVALID), (dict(logits=4098), INVALID), (dict(ltype=0, logits=4097), INVALID),
     (dict(tokens=None), INVALID), (dict(logp=None), INVALID), (dict(topn=65), INVALID), (dict(topn=-1), INVALID),
     (dict(top_ids=None), INVALID), (dict(top_logp=None), INVALID), (dict(scale=0.0), INVALID), (dict(scale=-1.0), INVALID),
-    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(M=0), SHAPE), (dict(V=0), SHAPE),
+    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(M=0), SHAPE), (dict(M=2**23 + 1), SHAPE), (dict(V=0), SHAPE),
     (dict(ld=999), SHAPE), (dict(tokens=None, logp=None, entropy=None, topn=0), INVALID)])
 def test_logprobs_refusals(kw, status):
     assert _logprobs(**kw) == status
