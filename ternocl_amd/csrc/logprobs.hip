@@ -113,11 +113,11 @@ __device__ __forceinline__ LpSum lp_join(LpSum a, LpSum b, float c) {
     return o;
 }
 
-// One entry's terms: (2^e2, e2 2^e2).  (e2 from -1000 down, -inf too: 0, and no -inf times 0.)
+// One entry's terms: (2^e2, e2 2^e2).  (No -inf times 0; a NaN stays one in r.)
 __device__ __forceinline__ void lp_term(float x, float m, float c, float &r, float &t) {
-    const float y = (x - m) * c, d = y < -1000.0f ? -1000.0f : y, e = __builtin_amdgcn_exp2f(d);
+    const float d = (x - m) * c, e = __builtin_amdgcn_exp2f(d);
     r += e;
-    t = __builtin_fmaf(d, e, t);
+    t = __builtin_fmaf(fmaxf(d, -1000.0f), e, t);
 }
 
 // A wave's running sums: m uniform, r and t a lane's part of the sums relative to m.
