@@ -491,7 +491,8 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
  * Codes, activations and zero points are multiplied as they are and summed in fp32
  * (or exact integers) per group; nothing is rounded to DT before the epilogue.  A
  * row of A that holds an infinity or a NaN has infinities or NaN for its sums, before
- * the epilogue; no other row is changed by it.
+ * the epilogue; no other row is changed by it.  (bf16: so may a row that holds values
+ * past 2^112, whose sums over a group leave fp32.)
  * N % 16 == 0, K % 128 == 0, any M >= 1.  B starts on 16 bytes.  M <= 8 runs the
  * decode GEMV (A 16-byte aligned; K M up to some 50000), other calls a matrix-core
  * GEMM where every operand is 16-byte aligned, a plain kernel (several times slower)
@@ -521,8 +522,9 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
  *   ids   = the topk largest v among them, in falling order (equal values: the
  *           lowest index first, groups too)
  *   RW    = scale * s[ids], with renorm divided by the sum of the chosen s first
- * Choices are made on v as in 64-bit arithmetic; sums and weights are fp64,
- * rounded to fp32, then to wtype.  An expert whose logit or v is -inf is never chosen and
+ * Choices are made on v as in 64-bit arithmetic, without a bias on the logits, which
+ * order the experts as s does and also tell apart what rounds to one s; sums and weights
+ * are fp64, rounded to fp32, then to wtype.  An expert whose logit or v is -inf is never chosen and
  * adds nothing to its group's value; slots left without an expert get id -1 and
  * weight 0 (which the MoE entries skip).  A group without experts to choose counts
  * as -inf.  A NaN ranks first, and a softmax row with a NaN or +inf logit has NaN
@@ -547,7 +549,7 @@ ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const
  * over get id -1 and -inf.  A row of -inf alone gives logp -inf, entropy 0, ids -1; a
  * row with a NaN or +inf gives NaN, ids -1.
  * logits: ltype [M, V] with ld elements from row to row (ld >= V), its rows at any
- * element alignment.  1 <= M <= 2^23, V >= 1, 0 <= topn <= 64, scale > 0 and finite.
+ * element alignment.  1 <= M <= 2^23, V >= 1, 0 <= topn <= 64, 2^-100 <= scale <= 2^100.
  * ws: optional scratch of ternocl_logprobs_ws_bytes(M, V, topn) bytes (0: none used),
  * 16-byte aligned, any contents: rows are spread over workgroups where there are few,
  * their sums joined by the last (arrival counters in the header, left zero).  NULL or

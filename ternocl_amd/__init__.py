@@ -476,6 +476,8 @@ def int4_unpack(B, K: int):
     """B uint32 [K/32, N, 4] -> int8 [K, N] (ternocl_int4_unpack, on the host)."""
     import numpy as np
     B = np.ascontiguousarray(B, dtype=np.uint32)
+    if B.ndim != 3 or B.shape[0] != K // 32 or B.shape[2] != 4:
+        raise TernoclError(1, f"int4_unpack: B must be [K/32, N, 4], got {list(B.shape)} with K = {K}")
     W = np.empty((K, B.shape[1]), np.int8)
     _check(lib().ternocl_int4_unpack(_cptr(B), _cptr(W), K, B.shape[1]))
     return W

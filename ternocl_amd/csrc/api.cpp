@@ -755,7 +755,8 @@ ternocl_status ternocl_logprobs(int ltype, const void *logits, int64_t ld, const
     if (topn < 0 || topn > 64) FAIL(TERNOCL_ERR_INVALID_ARG, "topn must be 0..64");
     if (topn && (!top_ids || !top_logp)) FAIL(TERNOCL_ERR_INVALID_ARG, "topn > 0 writes top_ids and top_logp: both must be non-null");
     if (!logp && !entropy && !topn) FAIL(TERNOCL_ERR_INVALID_ARG, "nothing to compute: logp, entropy and topn are all absent");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be positive and finite");
+    // (outside, a difference of two logits or scale * log2 e leaves fp32's range where the product does not)
+    if (!(scale >= 0x1p-100f) || scale > 0x1p100f) FAIL(TERNOCL_ERR_INVALID_ARG, "scale must be 2^-100..2^100");
     if (M < 1 || M > 1 << 23 || V < 1) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need 1 <= M <= 2^23 and V >= 1");
     if (ld < V) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ld must be at least V");
     const uintptr_t es = ltype == TERNOCL_FP32 ? 4 : 2;

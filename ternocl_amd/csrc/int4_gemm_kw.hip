@@ -79,7 +79,7 @@ __device__ __forceinline__ void i4_walk(uint8_t *abuf, const uint16_t *A, const 
                 if constexpr (OFF) {
                     float z = BF16 ? 24.0f : 0.0f;
                     if constexpr (ZP) z += i4_scale<CB, BF16>(bs.zr[s][g], cb);
-                    of[g][cb] = -sc[g][cb] * z;
+                    of[g][cb] = -z;
                 }
             }
         }
@@ -114,8 +114,9 @@ __device__ __forceinline__ void i4_walk(uint8_t *abuf, const uint16_t *A, const 
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int g = G < 64 ? i >> 1 : 0;
-                            acc[mb][cb][r] = __builtin_fmaf(part[mb][cb][r], sc[g][cb], acc[mb][cb][r]);
-                            if constexpr (OFF) acc[mb][cb][r] = __builtin_fmaf(sums[mb][r], of[g][cb], acc[mb][cb][r]);
+                            float v = part[mb][cb][r];
+                            if constexpr (OFF) v = __builtin_fmaf(sums[mb][r], of[g][cb], v);
+                            acc[mb][cb][r] = __builtin_fmaf(v, sc[g][cb], acc[mb][cb][r]);
                         }
         }
     };
@@ -278,7 +279,7 @@ size_t int4_gemm_ws_need(int M, int N, int K, int group) {
     return ks == 1 ? 0 : kWsHeader + (size_t)ks * M * N * 4;
 }
 
-// (operands 16-byte aligned; M K and N below 2^31 times a tile's rows and columns)
+// (operands 16-byte aligned; 128 K below 2^31)
 ternocl_status int4_gemm_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
                              const void *Other, const void *Bias, int M, int N, int K, int group, int postop, int out_f32,
                              void *ws, size_t ws_bytes, hipStream_t st) {

@@ -116,7 +116,7 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
                 if constexpr (OFF) {
                     float z = BF16 ? 24.0f : 0.0f;
                     if constexpr (ZP) z += i4_scale<CB, BF16>(bs.zr[s][g], cb);
-                    of[g][cb] = -sc[g][cb] * z;
+                    of[g][cb] = -z;
                 }
             }
         }
@@ -145,8 +145,9 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int g = G < 64 ? i >> 1 : 0;
-                            acc[mb][cb][r] = __builtin_fmaf(part[mb][cb][r], sc[g][cb], acc[mb][cb][r]);
-                            if constexpr (OFF) acc[mb][cb][r] = __builtin_fmaf(sums[mb][r], of[g][cb], acc[mb][cb][r]);
+                            float v = part[mb][cb][r];
+                            if constexpr (OFF) v = __builtin_fmaf(sums[mb][r], of[g][cb], v);
+                            acc[mb][cb][r] = __builtin_fmaf(v, sc[g][cb], acc[mb][cb][r]);
                         }
         }
     };

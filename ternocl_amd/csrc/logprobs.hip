@@ -275,6 +275,9 @@ template <int LT, class F> __device__ __forceinline__ void lp_scan(const LpRow<L
     }
 }
 
+// scale (x - m), finite wherever that is in fp32 (halves: the difference may be past its range).
+__device__ __forceinline__ float lp_scaled(float x, float m, float scale) { return (0.5f * x - 0.5f * m) * (2.0f * scale); }
+
 // The token asked for (-1: none).
 __device__ __forceinline__ int lp_token(const LpArgs &a, int m) {
     const int tok = a.tokens ? a.tokens[m] : -1;
@@ -308,7 +311,7 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
     const float l1 = log1pf(s.r), nan = __builtin_nanf("");
     if (tid == 0) {
         if (a.logp) {
-            const float o = bad ? nan : empty ? -__builtin_inff() : (tok_x - s.m) * a.scale - l1;
+            const float o = bad ? nan : empty ? -__builtin_inff() : lp_scaled(tok_x, s.m, a.scale) - l1;
             a.logp[m] = tok < 0 ? 0.0f : o;
         }
         if (a.entropy)
@@ -432,7 +435,7 @@ __device__ __forceinline__ void lp_finish(const LpArgs &a, const LpRow<LT> &row,
         for (int i = 0; i < count; ++i) before += L.cand[i] > k;
         if (before < a.topn) {
             ids[before] = (int)~(uint32_t)k;
-            out[before] = (lp_key_value(k) - s.m) * a.scale - l1;
+            out[before] = lp_scaled(lp_key_value(k), s.m, a.scale) - l1;
         }
     }
     for (int i = count + tid; i < a.topn; i += kThreads) {

@@ -181,6 +181,19 @@ def test_extremes(dev, M):
         assert ((got - want).abs() <= 2.0**-23 * want.abs() + d + 2.0**-113).all()
 
 
+@pytest.mark.parametrize("M", [1, 8, 20, 300])
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+def test_largest_scales(dev, M, zero, group):
+    """Scales near the end of bf16's range: sums that they bring back into fp32 are no infinities on the way."""
+    import ternocl_amd as T
+    A, W, S, Z, dt = make(6, M, 256, 272, group, True, zero)
+    A, S = (A.double() * 2.0**-100).to(dt), (S.double() * 2.0**131).to(dt)
+    got = run(T, A, W, S, Z, group, None, None, 0, True).cpu().double()
+    want, d = gold(A, W, S, Z, group, None, None, 0)
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + d).all()
+
+
 @pytest.mark.parametrize("M", [1, 4, 24, 200])
 def test_graph_and_stream(dev, M):
     """Captured on a side stream and replayed with new inputs between eager calls, its workspace reused."""

@@ -196,6 +196,32 @@ def test_scales(dev, scale):
     check(T, x, t, 8, scale)
 
 
+@pytest.mark.parametrize("ws", [True, False])
+@pytest.mark.parametrize("scale", [2.0**-100, 2.0**100])
+def test_scale_limits(dev, scale, ws):
+    """Both ends of the scales, logits to match, and logits whose difference is past fp32's range."""
+    import ternocl_amd as T
+    x, t = rows(12, 3, 40001, "f32")
+    x = x / scale
+    if scale < 1:
+        x[1, 100], x[1, 200], t[1] = 3e38, -3e38, 200
+        x[2, 100], x[2, 200], x[2, 40000], t[2] = 3e38, -3e38, 3e38, 200
+    check(T, x, t, 8, scale, ws=ws)
+
+
+@pytest.mark.parametrize("scale", [0.25, 1.0])
+def test_widest_difference(dev, scale):
+    """The type's lowest value beside its largest: listed with its ln p where that is in fp32."""
+    import ternocl_amd as T
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[-big, big, 0.0, -big, -math.inf]])
+    lp, H, ids, tl = call(T, x, torch.tensor([3], dtype=torch.int32), 5, scale)
+    want = [0.0, -big * scale, -2 * big * scale, -2 * big * scale, -math.inf]
+    want = [w if w >= -big else -math.inf for w in want]
+    assert ids.tolist() == [[1, 2, 0, 3, -1]] and H.tolist() == [0.0]
+    assert lp.item() == want[3] and tl.tolist() == [want]
+
+
 def test_parts_may_be_left_out(dev):
     import ternocl_amd as T
     x, t = rows(6, 3, 12345, "f16")

@@ -98,7 +98,8 @@ def _logprobs(**kw):
     (dict(ltype=7), INVALID), (dict(logits=None), INVALID), (dict(logits=4098), INVALID), (dict(ltype=0, logits=4097), INVALID),
     (dict(tokens=None), INVALID), (dict(logp=None), INVALID), (dict(topn=65), INVALID), (dict(topn=-1), INVALID),
     (dict(top_ids=None), INVALID), (dict(top_logp=None), INVALID), (dict(scale=0.0), INVALID), (dict(scale=-1.0), INVALID),
-    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(M=0), SHAPE), (dict(M=2**23 + 1), SHAPE), (dict(V=0), SHAPE),
+    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(scale=2.0**101), INVALID),
+    (dict(scale=2.0**-101), INVALID), (dict(M=0), SHAPE), (dict(M=2**23 + 1), SHAPE), (dict(V=0), SHAPE),
     (dict(ld=999), SHAPE), (dict(tokens=None, logp=None, entropy=None, topn=0), INVALID)])
 def test_logprobs_refusals(kw, status):
     assert _logprobs(**kw) == status
@@ -117,6 +118,11 @@ def test_python_refusals():
     x = torch.zeros(2, 8)
     with pytest.raises(T.TernoclError):
         T.moe_topk(x, None, x, x, 2, 8, 2, score="tanh", stream=0)
+    B = np.zeros((2, 3, 4), np.uint32)
+    assert T.int4_unpack(B, 64).shape == (64, 3)
+    for b, K in ((B, 96), (B, 32), (B[:, :, :2], 64), (B[0], 32)):  # (never read past B)
+        with pytest.raises(T.TernoclError):
+            T.int4_unpack(b, K)
     with pytest.raises(T.TernoclError):
         T.logprobs(x.double(), None, None, x, None, None, 2, 8, stream=0)
 
