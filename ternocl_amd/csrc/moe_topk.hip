@@ -6,7 +6,7 @@
 //   of those (renormalised), times scale.
 //
 // L lanes take a token (64 / L tokens a wave), lane i of them holding experts i, i + L, ...
-// With L = 16 (up to 16 choices, 14 with a bias) the values that can be among the topk go to
+// With L = 16 (up to 16 choices, 15 with a bias) the values that can be among the topk go to
 // a list that is ranked at once; with L = 64 topk rounds pick the largest value (a maximum
 // over the lanes), the lowest index that has it (a minimum over those), and drop it, at
 // three times the instructions (T = 1 E = 64, 8 choices 4.0 against 3.1 us, T = 4000 E =
@@ -70,8 +70,10 @@ constexpr int kTkWaves = 4;
 // A sigmoid: its argument's two roundings (times s (1 - s) |l|, below 0.23), the
 // exponential's and the reciprocal's last places, below 2^-22 together.  A softmax term:
 // 37 additions of its row's sum at most, each term's argument (E |l - max| <= ln 512) and
-// last place, below 56 x 2^-24 < 2^-18.  The bias's addition: 2^-24 |v|.
-__device__ __forceinline__ float tk_margin(float v, int score) { return (score == 0 ? 0x1p-17f : 0x1p-21f) + 0x1p-22f * fabsf(v); }
+// last place, below 56 x 2^-24 < 2^-18 of the row's largest.  The bias's addition: 2^-24 |v|.
+// s: twice the scores' part, kSigmoidError or 2^-17 of the largest term.
+constexpr float kSigmoidError = 0x1p-21f;
+__device__ __forceinline__ float tk_margin(float v, float s) { return s + 0x1p-22f * fabsf(v); }
 
 // A value's bits as an integer in the order of the values (-0 as +0), kNone for -inf; and
 // back.  (Integer comparisons: fmaxf quiets its operands first, twice the instructions.)
@@ -115,6 +117,17 @@ __device__ __forceinline__ float tk_logit(const TkArgs &a, int t, int e) {
     if (a.ltype == TERNOCL_FP32) return ((const float *)a.logits)[i];
     const uint32_t h = ((const uint16_t *)a.logits)[i];
     return a.ltype == TERNOCL_BF16 ? dt2f<true>(h) : dt2f<false>(h);
+}
+// The softmax sum of token t in 64 bits, relative to its largest logit mx: L lanes, the logits
+// read again (the double exponentials of 32 experts a lane would hold it at 2 waves a SIMD)
+template <int L> __device__ __forceinline__ double tk_total(const TkArgs &a, int t, int sub, float mx) {
+    double p = 0.0;
+#pragma unroll 4
+    for (int e = sub; e < a.E; e += L) {
+        const float y = tk_logit(a, t, e);
+        p += y == -__builtin_inff() ? 0.0 : exp((double)y - (double)mx);
+    }
+    return tk_dsum<L>(p);
 }
 // Logits e0, e0 + step, ... of token t (-inf past the last expert), all loads in flight
 template <int n> __device__ __forceinline__ void tk_logits(const TkArgs &a, int t, int e0, int step, float l[n]) {
@@ -291,8 +304,10 @@ template <int VX> __device__ __forceinline__ void tk_exact(const TkArgs &a, int 
 }
 
 // GROUPED: 0 no choice of groups; 1 any groups; 2 groups of whole lanes, a power of two of
-// them: lane i holds experts i VPL .. + VPL - 1 then.
-template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kTkWaves) k_moe_topk(const TkArgs a) {
+// them: lane i holds experts i VPL .. + VPL - 1 then.  Many tokens of 257 experts and more are
+// four waves a SIMD only in 128 registers (up to 216 without the bound: that call 33.4 -> 23.6
+// us, E = 512 10 choices without a bias 14.0 -> 11.5).
+template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kTkWaves, L == 16 && VPL == 32 ? 4 : 1) k_moe_topk(const TkArgs a) {
     constexpr int TPW = 64 / L, VX = VPL * L / 64 > 0 ? VPL * L / 64 : 1;
     // a wave's values [tokens][L VPL] while groups are valued; its tokens' lists [32] and
     // picks in order [16]; tk_exact's keys
@@ -305,6 +320,10 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
     const int tc = min(t, a.T - 1);
     const float ninf = -__builtin_inff();
     float l[VPL], bias[VPL];
+    auto load_bias = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) bias[j] = a.bias[min(sub + L * j, a.E - 1)];
+    };
     int v[VPL];  // what experts are chosen by (tk_int)
     constexpr int E0 = GROUPED == 2 ? VPL : 1, ES = GROUPED == 2 ? 1 : L;  // lane i's experts E0 i + ES j
     if constexpr (GROUPED == 2) {
@@ -317,9 +336,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         }
     } else {
         tk_logits<VPL>(a, tc, sub, L, l);
-        if (a.bias)
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) bias[j] = a.bias[min(sub + L * j, a.E - 1)];
+        if (VPL < 32 && a.bias) load_bias();
     }
     bool odd = false;  // this token needs 64 bits
 #pragma unroll
@@ -335,7 +352,19 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         for (int j = 0; j < VPL; ++j) mx = fmaxf(mx, l[j]);
         mx = tk_lanes<L>(mx, lane, tk_fmax2);
     }
+    if (a.score == 0 && !a.renorm) {
+        // the weights' denominator, as exact as they are stored
+        if (a.wtype == TERNOCL_FP32) {
+            total = tk_total<L>(a, tc, sub, mx);
+        } else {
+            float p = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) p += l[j] == ninf ? 0.0f : __builtin_amdgcn_exp2f((l[j] - mx) * 1.44269504088896341f);
+            total = (double)tk_lanes<L>(p, lane, tk_add2);
+        }
+    }
     float s[VPL];  // the scores, where choices are made by them
+    float err = kSigmoidError;  // (tk_margin)
     if (a.bias || two) {
         float p = 0.0f;
 #pragma unroll
@@ -348,28 +377,19 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
             const float r = 1.0f / tk_lanes<L>(p, lane, tk_add2);
 #pragma unroll
             for (int j = 0; j < VPL; ++j) s[j] *= r;
+            err = 0x1p-17f * r;
         }
         if (a.bias) {
+            if constexpr (VPL >= 32 && GROUPED != 2) {  // (registers)
+                __builtin_amdgcn_sched_barrier(0);
+                load_bias();
+            }
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
                 const float x = s[j] + bias[j];
                 v[j] = l[j] == ninf ? kNone : tk_int(x);
                 odd |= !(x < __builtin_inff());
             }
-        }
-    }
-    if (a.score == 0 && !a.renorm) {
-        // the weights' denominator, as exact as they are stored
-        if (a.wtype == TERNOCL_FP32) {
-            double p = 0.0;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) p += l[j] == ninf ? 0.0 : exp((double)l[j] - (double)mx);
-            total = tk_dsum<L>(p);
-        } else {
-            float p = 0.0f;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) p += l[j] == ninf ? 0.0f : __builtin_amdgcn_exp2f((l[j] - mx) * 1.44269504088896341f);
-            total = (double)tk_lanes<L>(p, lane, tk_add2);
         }
     }
     if constexpr (GROUPED == 2) {
@@ -414,7 +434,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         if (a.bias || two) {
             const float lo = tk_float(tk_lanes<L>(real && keep ? gv : 0x7fffffff, lane, tk_imin2));
             const float hi = tk_float(tk_lanes<L>(real && !keep ? gv : kNone, lane, tk_imax2));
-            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, a.score));
+            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, err));
         }
 #pragma unroll
         for (int j = 0; j < VPL; ++j) v[j] = keep ? v[j] : kNone;
@@ -435,30 +455,51 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
 #pragma unroll
         for (int j = 0; j < VPL; ++j) val[sub + L * j] = two && !a.bias ? (v[j] == kNone ? kNone : tk_int(s[j])) : v[j];
         __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
-        // lane g values groups g, g + L, ...: their largest one or two (each lane starts at
-        // another member, for the banks)
+        // lane g + part 2^sh values part `part` of group g (of groups g, g + L, ... where they are
+        // more than the lanes): the largest one or two of every parts-th member, from another
+        // one on in each group and token, for the banks.  (T = 16384, one of two groups of 196,
+        // 4 choices: a lane a group 43.6, this 33.4 us)
         constexpr int GPL = 64 / L;
         int gv[GPL];
+        const int sh = min(32 - __builtin_clz(a.n_group - 1), L == 64 ? 6 : 4), parts = L >> sh;  // (n_group > 1)
+        const int g0 = sub & ((1 << sh) - 1), part = sub >> sh, members = (per - part + parts - 1) / parts;
 #pragma unroll
         for (int k = 0; k < GPL; ++k) {
-            const int g = sub + L * k;
+            const int g = g0 + L * k;
             int b1 = kNone, b2 = kNone;
             if (L * k < a.n_group) {  // (uniform)
                 const int *x = val + min(g, a.n_group - 1) * per;
-                int i = sub % per;
-                for (int n = 0; n < per; n += 4) {
+                const int begin = min(part, per - 1);
+                int i = begin + parts * max(min(g + tok, members - 1), 0);
+                for (int n = 0; n * parts < per; n += 4) {
                     int o[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         o[u] = x[i];
-                        i = i + 1 == per ? 0 : i + 1;
+                        i = i + parts < per ? i + parts : begin;
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int y = n + u < per ? o[u] : kNone;
+                        const int y = n + u < members ? o[u] : kNone;
                         b2 = max(b2, min(y, b1));
                         b1 = max(b1, y);
                     }
+                }
+            }
+            auto merge = [&](auto m) __attribute__((always_inline)) {
+                if (decltype(m)::value < 1 << sh) return;  // (uniform)
+                const int o1 = __float_as_int(lane_xor<decltype(m)::value>(__int_as_float(b1), lane));
+                const int o2 = __float_as_int(lane_xor<decltype(m)::value>(__int_as_float(b2), lane));
+                b2 = max(min(b1, o1), max(b2, o2));
+                b1 = max(b1, o1);
+            };
+            if (k == 0) {  // (further groups: parts is 1)
+                merge(std::integral_constant<int, 2>{});
+                merge(std::integral_constant<int, 4>{});
+                merge(std::integral_constant<int, 8>{});
+                if constexpr (L == 64) {
+                    merge(std::integral_constant<int, 16>{});
+                    merge(std::integral_constant<int, 32>{});
                 }
             }
             gv[k] = g >= a.n_group ? kNone : two && b2 != kNone ? tk_int(tk_float(b1) + tk_float(b2)) : b1;
@@ -466,8 +507,10 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < GPL; ++k)
-            if (sub + L * k < a.n_group) val[sub + L * k] = gv[k];
+            if (part == 0 && g0 + L * k < a.n_group) val[g0 + L * k] = gv[k];
         __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < GPL; ++k) gv[k] = sub + L * k < a.n_group ? val[sub + L * k] : kNone;
         // kept: fewer than topk_group groups come before it
         int before[GPL] = {};
 #pragma unroll 4
@@ -488,45 +531,75 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         }
         if (a.bias || two) {
             const float lo = tk_float(tk_lanes<L>(low, lane, tk_imin2)), hi = tk_float(tk_lanes<L>(high, lane, tk_imax2));
-            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, a.score));
+            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, err));
         }
+        // (experts past E: none anyway)
         const float inv = 1.0f / (float)per;  // (e + 1/2) / per, e < 512: 2^-10 or more from a whole number
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
-            if (!((kept >> (int)(((float)min(sub + L * j, a.E - 1) + 0.5f) * inv)) & 1)) v[j] = kNone;
+            if (!((kept >> ((int)__builtin_fmaf((float)sub, inv, ((float)(L * j) + 0.5f) * inv) & 63)) & 1)) v[j] = kNone;
     }
     bool close = false;  // picks to be put in order by their 64-bit values (alike in a token's lanes)
     int id = -1, pick = kNone;  // lane r: the r-th largest value's expert, and the value
     if constexpr (L == 16) {
         // The need-th largest of the 16 lanes' maxima is a bound that at least need values
-        // reach (13 or so of 256 for need = 10): those go to a list, whose 64-bit keys (value,
-        // lowest index) are ranked each against all.  More than kList: tk_exact.
+        // reach (15 or so of 256 for need = 10): those go to a list, whose 64-bit keys (value,
+        // lowest index) are ranked each against all.  Where more than kList reach it (for need =
+        // 14 every second time, for 16 nearly always), the need-th largest of the lanes' two
+        // largest is the bound; still more (equal values): tk_exact.
         constexpr int kList = 32;
-        const int need = a.topk + (a.bias ? 2 : 0);  // (<= 16)
+        const int need = min(a.topk + (a.bias ? 2 : 0), L);
         int best = v[0];
 #pragma unroll
         for (int j = 1; j < VPL; ++j) best = max(best, v[j]);
         int above = 0;
-        auto turn = [&](auto i) __attribute__((always_inline)) {  // (row_ror i)
-            above += __builtin_amdgcn_mov_dpp(best, 0x120 + decltype(i)::value, 0xf, 0xf, true) > best;
+        auto turns = [](auto &&turn) __attribute__((always_inline)) {  // (row_ror i)
+            turn(std::integral_constant<int, 0x121>{}), turn(std::integral_constant<int, 0x122>{});
+            turn(std::integral_constant<int, 0x123>{}), turn(std::integral_constant<int, 0x124>{});
+            turn(std::integral_constant<int, 0x125>{}), turn(std::integral_constant<int, 0x126>{});
+            turn(std::integral_constant<int, 0x127>{}), turn(std::integral_constant<int, 0x128>{});
+            turn(std::integral_constant<int, 0x129>{}), turn(std::integral_constant<int, 0x12a>{});
+            turn(std::integral_constant<int, 0x12b>{}), turn(std::integral_constant<int, 0x12c>{});
+            turn(std::integral_constant<int, 0x12d>{}), turn(std::integral_constant<int, 0x12e>{});
+            turn(std::integral_constant<int, 0x12f>{});
         };
-        turn(std::integral_constant<int, 1>{}), turn(std::integral_constant<int, 2>{}), turn(std::integral_constant<int, 3>{});
-        turn(std::integral_constant<int, 4>{}), turn(std::integral_constant<int, 5>{}), turn(std::integral_constant<int, 6>{});
-        turn(std::integral_constant<int, 7>{}), turn(std::integral_constant<int, 8>{}), turn(std::integral_constant<int, 9>{});
-        turn(std::integral_constant<int, 10>{}), turn(std::integral_constant<int, 11>{}), turn(std::integral_constant<int, 12>{});
-        turn(std::integral_constant<int, 13>{}), turn(std::integral_constant<int, 14>{}), turn(std::integral_constant<int, 15>{});
-        const int bound = max(tk_lanes<L>(above < need ? best : 0x7fffffff, lane, tk_imin2), kNone + 1);
-        int count = 0;
+        turns([&](auto i) __attribute__((always_inline)) {
+            above += __builtin_amdgcn_mov_dpp(best, decltype(i)::value, 0xf, 0xf, true) > best;
+        });
+        int bound = max(tk_lanes<L>(above < need ? best : 0x7fffffff, lane, tk_imin2), kNone + 1);
+        int place, total_n;
+        auto places = [&]() __attribute__((always_inline)) {
+            int count = 0;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) count += v[j] >= bound;
-        // places in the list: the counts of the lanes before (row_shr 1, 2, 4, 8: 0 comes in)
-        int place = count;
-        place += __builtin_amdgcn_update_dpp(0, place, 0x111, 0xf, 0xf, true);
-        place += __builtin_amdgcn_update_dpp(0, place, 0x112, 0xf, 0xf, true);
-        place += __builtin_amdgcn_update_dpp(0, place, 0x114, 0xf, 0xf, true);
-        place += __builtin_amdgcn_update_dpp(0, place, 0x118, 0xf, 0xf, true);
-        const int total_n = tk_lanes<L>(place, lane, tk_imax2);  // (the last lane's)
-        place -= count;
+            for (int j = 0; j < VPL; ++j) count += v[j] >= bound;
+            // places in the list: the counts of the lanes before (row_shr 1, 2, 4, 8: 0 comes in)
+            place = count;
+            place += __builtin_amdgcn_update_dpp(0, place, 0x111, 0xf, 0xf, true);
+            place += __builtin_amdgcn_update_dpp(0, place, 0x112, 0xf, 0xf, true);
+            place += __builtin_amdgcn_update_dpp(0, place, 0x114, 0xf, 0xf, true);
+            place += __builtin_amdgcn_update_dpp(0, place, 0x118, 0xf, 0xf, true);
+            total_n = tk_lanes<L>(place, lane, tk_imax2);  // (the last lane's)
+            place -= count;
+        };
+        places();
+        if (__ballot(total_n > kList)) {  // (uniform)
+            int b1 = kNone, b2 = kNone, n1 = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                b2 = max(b2, min(v[j], b1));
+                b1 = max(b1, v[j]);
+            }
+            int n2 = b1 > b2;
+            turns([&](auto i) __attribute__((always_inline)) {
+                const int o1 = __builtin_amdgcn_mov_dpp(b1, decltype(i)::value, 0xf, 0xf, true);
+                const int o2 = __builtin_amdgcn_mov_dpp(b2, decltype(i)::value, 0xf, 0xf, true);
+                n1 += (o1 > b1) + (o2 > b1);
+                n2 += (o1 > b2) + (o2 > b2);
+            });
+            const int low = min(n1 < need ? b1 : 0x7fffffff, n2 < need ? b2 : 0x7fffffff);
+            bound = max(tk_lanes<L>(low, lane, tk_imin2), kNone + 1);
+            places();
+        }
         odd |= total_n > kList;
         u64 *list = space[w] + tok * kList, *order = space[w] + TPW * kList + tok * L;
         __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
@@ -555,7 +628,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
             // a pick too close to the next one (the 16th: not known)
             const u64 next = order[min(sub + 1, L - 1)];
             const float x = tk_float((int)((uint32_t)(k >> 32) ^ 0x80000000u)), y = tk_float((int)((uint32_t)(next >> 32) ^ 0x80000000u));
-            const bool amb = k != 0 && (sub == L - 1 ? total_n > L : next != 0 && !(x - y > tk_margin(x, a.score)));
+            const bool amb = k != 0 && (sub == L - 1 ? total_n > L : next != 0 && !(x - y > tk_margin(x, err)));
             const uint32_t near = (uint32_t)(__ballot(amb) >> (L * tok)) & 0xffffu;
             last = __builtin_ctz(~near & ~((1u << (a.topk - 1)) - 1));  // (16: none of them is apart)
             odd |= last >= L;
@@ -577,7 +650,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
             const int m = tk_lanes<L>(best, lane, tk_imax2);
             if (a.bias) {
                 const float x = tk_float(m);
-                const bool apart = m == kNone || last - x > tk_margin(last, a.score);
+                const bool apart = m == kNone || last - x > tk_margin(last, err);
                 settled |= r >= a.topk && apart;
                 if (r >= a.topk && __ballot(!settled) == 0) break;  // (uniform)
                 if (r == L) {  // more close values than lanes
@@ -608,13 +681,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
     if (__ballot(close && !odd && on)) {  // (uniform)
         double x = 0.0;
         if (a.score == 0) {
-            double p = 0.0;
-#pragma unroll 4
-            for (int e = sub; e < a.E; e += L) {
-                const float y = tk_logit(a, tc, e);
-                p += y == ninf ? 0.0 : exp((double)y - (double)mx);
-            }
-            x = exp((double)lv - (double)mx) / tk_dsum<L>(p);
+            x = exp((double)lv - (double)mx) / tk_total<L>(a, tc, sub, mx);
         } else {
             x = 1.0 / (1.0 + exp(-(double)lv));
         }
@@ -656,7 +723,7 @@ ternocl_status moe_topk_run(int ltype, const void *logits, long ld, const float 
                             int E, int topk, int score, int n_group, int topk_group, int group_best, int renorm,
                             float scale, hipStream_t st) {
     const TkArgs a = {logits, bias, ids, RW, ld, ltype, T, E, topk, wtype, score, n_group, topk_group, group_best, renorm, scale};
-    if (topk + (bias ? 2 : 0) <= 16) {  // (the lists' bound: one of 16 lanes' maxima)
+    if (topk + (bias ? 1 : 0) <= 16) {  // (16 lanes hold the picks, with a bias the next one too)
         if (E <= 64) tk_launch<16, 4>(a, st);
         else if (E <= 128) tk_launch<16, 8>(a, st);
         else if (E <= 256) tk_launch<16, 16>(a, st);

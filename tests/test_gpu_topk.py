@@ -137,6 +137,23 @@ def test_groups(dev, E, n_group, topk_group, score, biased, group_best):
     check(T, x, b if biased else None, min(6, topk_group * (E // n_group)), "f32", score, n_group, topk_group, group_best, True, 2.5)
 
 
+@pytest.mark.parametrize("E,n_group,topk_group", [(392, 2, 1), (418, 2, 1), (330, 3, 2), (510, 6, 2), (126, 2, 1), (34, 2, 1),
+                                                  (306, 17, 5), (320, 64, 9), (500, 50, 30), (512, 1, 1), (91, 1, 1), (60, 1, 1)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_wide_groups_and_many_choices(dev, E, n_group, topk_group, biased):
+    """Groups of no power of two, a lane's part of each; lists of nearly as many choices as lanes."""
+    import ternocl_amd as T
+    x, b = logits_of(E, 103, E, "f32")
+    b = b if biased else None
+    for score in ("softmax", "sigmoid"):
+        for topk in (13, 14, 15, 16):
+            check(T, x, b, topk, "f32", score, n_group, topk_group, 1 + topk % 2, topk % 3 == 0)
+    y = x.half().float() * 4  # (some equal)
+    check(T, y, b, 15, "bf16", "softmax", n_group, topk_group, 2, False)
+    y[::5] = y[::5].round()  # (many)
+    check(T, y, b, 15, "f32", "sigmoid", n_group, topk_group, 1)
+
+
 def test_close_scores(dev):
     """Scores closer than fp32 tells apart are ordered as in 64 bits; equal ones by index."""
     import ternocl_amd as T
