@@ -17,6 +17,13 @@
 //   * A lane's B fragments are word i of block q of a 64-row unit (16 bytes a column and
 //     unit); in groups of 32 rows both halves of a fragment must lie in one block: words
 //     2 q and 2 q + 1 of each.
+//
+// Why K over the waves: a wave decodes its own weights once and needs no barrier, and few rows
+// give too few tiles for a wave each.  M = 24 K = 14336 N = 4096 bf16 (30 MB, 6.0 us of a
+// large copy): 15.6 us a call, of which the walk's stream is 8.5, its first loads, the waves'
+// and the slices' meeting the rest.  The more columns' activations a row block reads through
+// L2, the more the walk waits for them (M = 200 K = N = 5120: VALU 34% of a wave's time, waits
+// 32%, MFMAs 27%); int4_gemm_tile.hip takes over there.
 #include "gemm_kw.hpp"
 #include "int4_decode.hpp"
 

@@ -1,6 +1,15 @@
 // int4_gemm_tile.hip -- GEMM of hundreds of rows and more on 4-bit weights with group
 // scales for gfx950 (ternocl_int4_gemm): the same sums as int4_gemm_kw.hip on 128 x 256
 // tiles whose eight waves share the activations in LDS.
+//
+// A wave's 64 x 64 part: each decoded fragment feeds two row blocks and each activation
+// fragment two column blocks, with group sums (part) and the tile's (acc) in 128 registers;
+// two buffers of 64 rows of K and one barrier a unit; the activations two units ahead in
+// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 145.6 us a call, 826 TFLOP/s,
+// 71% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
+// decode and group sums on the VALU.  Groups of 32 at bf16 or with zero points are VALU-bound:
+// per 64-row unit of a wave 256 FMAs join group sums and offsets, 64 operations decode, for 24
+// MFMAs, a third of them the offsets' (M = 200 K = N = 5120: 44.4 us, 236 TFLOP/s).
 #include "gemm_kw.hpp"
 #include "int4_decode.hpp"
 

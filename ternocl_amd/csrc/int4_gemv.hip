@@ -24,6 +24,11 @@
 // columns x 4 blocks of 32 rows), with kDepth steps of weights in flight across strips.
 // The waves' sums meet in LDS, added in wave order by one wave while the others go on:
 // the same bits on every run, one barrier a strip.
+//
+// What bounds it is the weight stream: M = 4 K = 4096 N = 151680 fp16, 320 MB, 60.8 us a call,
+// 5.3 TB/s (a large copy 4.9); M = 1 K = 5120 N = 34816 bf16, groups of 64 with zero points, 100
+// MB, 22.3 us, 4.5 TB/s.  A small call is launch and first loads: M = 1 K = N = 4096 4.9 us
+// for 8.7 MB.
 #include "common.hpp"
 
 #include <algorithm>

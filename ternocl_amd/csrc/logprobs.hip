@@ -20,6 +20,10 @@
 // collected in LDS and ranked by (logit, lowest index).  Where more than kFlags pieces or
 // kCap entries reach it (many equal logits), a radix selection over the whole row first
 // finds the exact topn-th (value, index) key.
+//
+// V = 151680, 20 alternatives: 512 rows fp32 61.6 us, 5.0 TB/s (a large copy's rate), bf16
+// 46.1 us (VALU and exponentials); one row 10.0 us (latency: the stream, the arrival, the
+// alternatives, and the code's fetch).
 #include "common.hpp"
 
 namespace tcl {

@@ -20,6 +20,10 @@
 //     and the first one dropped are, or a value is NaN or +inf, the token is done again
 //     with 64-bit values (tk_exact, the whole wave).  Of N(0, 1.5) logits over 256 experts,
 //     sigmoid scores, about 1 token in 2000 has close picks, 1 in 16000 close groups.
+//
+// What bounds it: launch and latency for few tokens (T = 1 E = 128 3.2 us, T = 2048 E = 64 4.2
+// us), VALU issue for many (T = 16384 E = 256 fp32, 8 of 4 of 8 groups with a bias: 14.7 us, 1.2
+// TB/s; without either, bf16: 7.2 us).
 #include "common.hpp"
 
 #include <algorithm>
