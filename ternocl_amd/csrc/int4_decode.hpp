@@ -7,27 +7,36 @@
 namespace tcl {
 namespace {
 
-// A word's 8 codes as B fragment dwords (rows 2 d, 2 d + 1 in dword d): q in fp16, q + 24
-// in bf16.
+// A word's 8 codes as B fragment dwords (rows 2 d, 2 d + 1 in dword d): with OFF q + 24, a
+// nibble in the upper mantissa bits under the exponent of 16; without (fp16 alone has the
+// packed arithmetic for it) q.
 struct I4Const {
     uint32_t lo, hi, xlo, xhi;
 };
-template <bool BF16> __device__ __forceinline__ I4Const i4_const() {
-    I4Const k = BF16 ? I4Const{0x00780078u, 0u, 0x41c041c0u, 0u} : I4Const{0x000f000fu, 0x00f000f0u, 0x64086408u, 0x64806480u};
+template <bool BF16, bool OFF> __device__ __forceinline__ I4Const i4_const() {
+    static_assert(OFF || !BF16);
+    I4Const k = BF16  ? I4Const{0x00780078u, 0u, 0x41c041c0u, 0u}
+                : OFF ? I4Const{0x03c003c0u, 0u, 0x4e004e00u, 0u}
+                      : I4Const{0x000f000fu, 0x00f000f0u, 0x64086408u, 0x64806480u};
     asm("" : "+s"(k.lo));
     asm("" : "+s"(k.xlo));
-    if constexpr (!BF16) {
+    if constexpr (!OFF) {
         asm("" : "+s"(k.hi));
         asm("" : "+s"(k.xhi));
     }
     return k;
 }
-template <bool BF16> __device__ __forceinline__ void i4_decode(uint32_t x, const I4Const &k, uint32_t b[4]) {
+template <bool BF16, bool OFF> __device__ __forceinline__ void i4_decode(uint32_t x, const I4Const &k, uint32_t b[4]) {
     if constexpr (BF16) {
         b[0] = ((x << 3) & k.lo) ^ k.xlo;
         b[1] = ((x >> 1) & k.lo) ^ k.xlo;
         b[2] = ((x >> 5) & k.lo) ^ k.xlo;
         b[3] = ((x >> 9) & k.lo) ^ k.xlo;
+    } else if constexpr (OFF) {
+        b[0] = ((x << 6) & k.lo) ^ k.xlo;
+        b[1] = ((x << 2) & k.lo) ^ k.xlo;
+        b[2] = ((x >> 2) & k.lo) ^ k.xlo;
+        b[3] = ((x >> 6) & k.lo) ^ k.xlo;
     } else {
         const uint32_t y = x >> 8;
         const uint32_t p[4] = {(x & k.lo) ^ k.xlo, (x & k.hi) ^ k.xhi, (y & k.lo) ^ k.xlo, (y & k.hi) ^ k.xhi};

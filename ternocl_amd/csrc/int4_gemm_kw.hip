@@ -7,20 +7,21 @@
 // Codes go to the matrix cores as small integers of the activations' type, so that the
 // products are exact and nothing is rounded but fp32 sums; a scale group's sums are
 // kept apart (part) and join the tile's by one FMA with S per output.
-//   * fp16: a nibble under the exponent of 1024 (or, in the upper half of a byte, 16
-//     times it), less 1032 (a sixteenth, less 72): q itself, nine operations a word of 8
-//     codes.
-//   * bf16 has no packed arithmetic here: a nibble in the upper mantissa bits under the
-//     exponent of 16 reads q + 24, eight operations a word.  24 (and Z, in both types)
-//     times the group's sum of activations is taken off: that sum for a lane's rows comes
-//     out of a matrix instruction against ones, once per row block for all columns.
+//   * fp16 without zero points: a nibble under the exponent of 1024 (or, in the upper half of
+//     a byte, 16 times it), less 1032 (a sixteenth, less 72): q itself, nine operations a
+//     word of 8 codes.
+//   * bf16 has no packed arithmetic here, and zero points need the activations' sums anyway:
+//     a nibble in the upper mantissa bits under the exponent of 16 reads q + 24, eight
+//     operations a word.  24 + Z times the group's sum of activations is taken off: that sum
+//     for a lane's rows comes out of a matrix instruction against ones, once per row block for
+//     all columns.
 //   * A lane's B fragments are word i of block q of a 64-row unit (16 bytes a column and
 //     unit); in groups of 32 rows both halves of a fragment must lie in one block: words
 //     2 q and 2 q + 1 of each.
 //
 // Why K over the waves: a wave decodes its own weights once and needs no barrier, and few rows
 // give too few tiles for a wave each.  M = 24 K = 14336 N = 4096 bf16 (30 MB, 6.0 us of a
-// large copy): 15.6 us a call, of which the walk's stream is 8.5, its first loads, the waves'
+// large copy): 15.4 us a call, of which the walk's stream is 8.5, its first loads, the waves'
 // and the slices' meeting the rest.  The more columns' activations a row block reads through
 // L2, the more the walk waits for them (M = 200 K = N = 5120: VALU 34% of a wave's time, waits
 // 32%, MFMAs 27%); int4_gemm_tile.hip takes over there.
@@ -59,7 +60,7 @@ __device__ __forceinline__ void i4_walk(uint8_t *abuf, const uint16_t *A, const 
         const int j = G < 64 ? 4 * (i >> 1) + 2 * q + (i & 1) : 4 * q + i;
         ar[i] = (uint32_t)(c * 128 + ((j ^ (c & 7)) << 4));
     }
-    const I4Const k4 = i4_const<BF16>();
+    const I4Const k4 = i4_const<BF16, OFF>();
     const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
     const uint32_t ones[4] = {one, one, one, one};
     auto a_store = [&](int p) __attribute__((always_inline)) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ void i4_walk(uint8_t *abuf, const uint16_t *A, const 
             for (int g = 0; g < I4Src<CB, PF, G, ZP>::GU; ++g) {
                 sc[g][cb] = i4_scale<CB, BF16>(bs.sr[s][g], cb);
                 if constexpr (OFF) {
-                    float z = BF16 ? 24.0f : 0.0f;
+                    float z = 24.0f;
                     if constexpr (ZP) z += i4_scale<CB, BF16>(bs.zr[s][g], cb);
                     of[g][cb] = -z;
                 }
@@ -109,7 +110,7 @@ __device__ __forceinline__ void i4_walk(uint8_t *abuf, const uint16_t *A, const 
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 uint32_t b[4];
-                i4_decode<BF16>(w[cb][i], k4, b);
+                i4_decode<BF16, OFF>(w[cb][i], k4, b);
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) part[mb][cb] = kw_mfma<BF16>(af[i & 1][mb], b, first ? f32x16_t{} : part[mb][cb]);
             }

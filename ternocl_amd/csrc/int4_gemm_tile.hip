@@ -5,11 +5,11 @@
 // A wave's 64 x 64 part: each decoded fragment feeds two row blocks and each activation
 // fragment two column blocks, with group sums (part) and the tile's (acc) in 128 registers;
 // two buffers of 64 rows of K and one barrier a unit; the activations two units ahead in
-// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 145.6 us a call, 826 TFLOP/s,
-// 71% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
+// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 142.8 us a call, 842 TFLOP/s,
+// 72% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
 // decode and group sums on the VALU.  Groups of 32 at bf16 or with zero points are VALU-bound:
 // per 64-row unit of a wave 256 FMAs join group sums and offsets, 64 operations decode, for 24
-// MFMAs, a third of them the offsets' (M = 200 K = N = 5120: 44.4 us, 236 TFLOP/s).
+// MFMAs, a third of them the offsets' (M = 200 K = N = 5120: 45.1 us, 232 TFLOP/s).
 #include "gemm_kw.hpp"
 #include "int4_decode.hpp"
 
@@ -94,7 +94,7 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
     bs.units = units;
     bs.q = q;
     bs.col = (uint32_t)min(n0 + 64 * wn + CB * c, a.N - CB);
-    const I4Const k4 = i4_const<BF16>();
+    const I4Const k4 = i4_const<BF16, OFF>();
     const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
     const uint32_t ones[4] = {one, one, one, one};
     f32x16_t acc[MB][CB], part[MB][CB], sums[OFF ? MB : 1];
@@ -114,20 +114,15 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
         a_store(s ^ 1);
         a_load(u + 2);
         uint32_t w[CB][4];
-        float sc[GU][CB], of[GU][CB];
+        typename KwVec<CB>::S sr[GU], zr[GU];
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
+        for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[cb][i] = bs.w[s][cb][i];
 #pragma unroll
-            for (int g = 0; g < GU; ++g) {
-                sc[g][cb] = i4_scale<CB, BF16>(bs.sr[s][g], cb);
-                if constexpr (OFF) {
-                    float z = BF16 ? 24.0f : 0.0f;
-                    if constexpr (ZP) z += i4_scale<CB, BF16>(bs.zr[s][g], cb);
-                    of[g][cb] = -z;
-                }
-            }
+        for (int g = 0; g < GU; ++g) {
+            sr[g] = bs.sr[s][g];
+            if constexpr (ZP) zr[g] = bs.zr[s][g];
         }
         bs.load(u + 2, s);
         __builtin_amdgcn_sched_barrier(0);
@@ -142,22 +137,26 @@ template <class Cfg, bool BF16, int G, bool ZP> __global__ void __launch_bounds_
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 uint32_t b[4];
-                i4_decode<BF16>(w[cb][i], k4, b);
+                i4_decode<BF16, OFF>(w[cb][i], k4, b);
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) part[mb][cb] = kw_mfma<BF16>(af[i & 1][mb], b, first ? f32x16_t{} : part[mb][cb]);
             }
             if (last)
 #pragma unroll
-                for (int cb = 0; cb < CB; ++cb)
+                for (int cb = 0; cb < CB; ++cb) {
+                    const int g = G < 64 ? i >> 1 : 0;
+                    const float sc = i4_scale<CB, BF16>(sr[g], cb);
+                    float of = -24.0f;
+                    if constexpr (ZP) of -= i4_scale<CB, BF16>(zr[g], cb);
 #pragma unroll
                     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int g = G < 64 ? i >> 1 : 0;
                             float v = part[mb][cb][r];
-                            if constexpr (OFF) v = __builtin_fmaf(sums[mb][r], of[g][cb], v);
-                            acc[mb][cb][r] = __builtin_fmaf(v, sc[g][cb], acc[mb][cb][r]);
+                            if constexpr (OFF) v = __builtin_fmaf(sums[mb][r], of, v);
+                            acc[mb][cb][r] = __builtin_fmaf(v, sc, acc[mb][cb][r]);
                         }
+                }
         }
     };
     a_load(u0);
