@@ -5,8 +5,8 @@
 // A wave's 64 x 64 part: each decoded fragment feeds two row blocks and each activation
 // fragment two column blocks, with group sums (part) and the tile's (acc) in 128 registers;
 // two buffers of 64 rows of K and one barrier a unit; the activations two units ahead in
-// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 142.8 us a call, 842 TFLOP/s,
-// 72% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
+// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 143 to 146 us a call, by box, 830
+// TFLOP/s, 71% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
 // decode and group sums on the VALU.  Groups of 32 at bf16 or with zero points are VALU-bound:
 // per 64-row unit of a wave 256 FMAs join group sums and offsets, 64 operations decode, for 24
 // MFMAs, a third of them the offsets' (M = 200 K = N = 5120: 45.1 us, 232 TFLOP/s).
