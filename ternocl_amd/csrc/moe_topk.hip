@@ -635,7 +635,8 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
             const bool amb = k != 0 && (sub == L - 1 ? total_n > L : next != 0 && !(x - y > tk_margin(x, err)));
             const uint32_t near = (uint32_t)(__ballot(amb) >> (L * tok)) & 0xffffu;
             last = __builtin_ctz(~near & ~((1u << (a.topk - 1)) - 1));  // (16: none of them is apart)
-            odd |= last >= L;
+            // (close ones up to the list's end: those below the bound may be close too, and larger in 64 bits)
+            odd |= last >= L || (last == total_n - 1 && bound > kNone + 1);
             close = (near & ((1u << min(last, L - 1)) - 1)) != 0;
         }
         if (k && sub <= last) {

@@ -246,3 +246,28 @@ def test_op_graph_and_stream(dev):
     with pytest.raises(RuntimeError):
         op(x, None, 4, torch.float32, "softmax", 7, 1, 1, True, 1.0)
     torch.library.opcheck(op.default, (x, b, *args), test_utils=("test_schema", "test_faketensor"))
+
+
+def close_ones(seed, Tk, E, close, score, at):
+    """Logits and biases that bring `close` experts of every token within some 2^-24 of `at`, the others at least
+    a tenth below: bias[e] = fp32(at - s(l[e])) for one row l, whose logits differ by up to 2 units of 2^-23 from
+    token to token."""
+    g = torch.Generator().manual_seed(seed)
+    row = torch.randn(E, generator=g) * 1.5
+    x = row * (1 + torch.randint(-2, 3, (Tk, E), generator=g) * 2.0**-23)
+    s = torch.softmax(row.double(), 0) if score == "softmax" else torch.sigmoid(row.double())
+    low = torch.rand(E, generator=g).double() * 0.5 + 0.1
+    low[torch.randperm(E, generator=g)[:close]] = 0
+    return x, (at - low - s).float()
+
+
+@pytest.mark.parametrize("E,topk", [(16, 1), (16, 8), (60, 2), (64, 4), (64, 15), (200, 1), (256, 8), (384, 2), (64, 17)])
+@pytest.mark.parametrize("close", [3, 5, 8, 12, 999])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("at", [0.9, -0.3])
+def test_few_close_scores(dev, E, topk, close, score, at):
+    """A few experts closer than fp32 tells apart, or all of them: the choice is the 64-bit one also where the
+    close ones go past those that were to be ranked."""
+    import ternocl_amd as T
+    x, b = close_ones(E + topk, 120, E, min(close, E), score, at)
+    check(T, x, b, topk, "f32", score)
