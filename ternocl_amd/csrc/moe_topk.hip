@@ -90,6 +90,23 @@ __device__ __forceinline__ float tk_float(int k) {
     return k == kNone ? -__builtin_inff() : __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
 
+// A group's value, and the error of that: its scores' (err, tk_margin's s) and, of its one or
+// two additions of a bias and of their sum, 2^-24 each of the terms, which may be far larger
+// than the sum (1.25 times that: of the error's own roundings).  b2: kNone where one value counts.
+struct TkGroup {
+    int value;
+    float error;
+};
+__device__ __forceinline__ TkGroup tk_group(int b1, int b2, float err) {
+    const float x = tk_float(b1), y = b2 == kNone ? 0.0f : tk_float(b2);
+    return {tk_int(x + y), __builtin_fmaf(fabsf(y), 0x1.4p-23f, __builtin_fmaf(fabsf(x), 0x1.4p-23f, err))};
+}
+// Whether a group may be on the other side of mid, a value between the least kept and the
+// largest dropped one: where none is, exactly those kept are the largest.
+__device__ __forceinline__ bool tk_group_close(int value, float error, float mid) {
+    return value != kNone && !(fabsf(tk_float(value) - mid) > error);
+}
+
 // Sum, maximum, minimum over the L lanes of a token
 template <int L, class V, class Op> __device__ __forceinline__ V tk_lanes(V v, int lane, Op op) {
     auto x = [&](auto m) __attribute__((always_inline)) {
@@ -421,7 +438,8 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
             merge(std::integral_constant<int, 16>{});
             merge(std::integral_constant<int, 32>{});
         }
-        const int gv = two && b2 != kNone ? tk_int(tk_float(b1) + tk_float(b2)) : b1;
+        const TkGroup gr = tk_group(b1, two ? b2 : kNone, err);
+        const int gv = gr.value;
         // kept: fewer than topk_group groups come before it
         int *val = (int *)space[w] + tok * L;
         val[g] = gv;  // (by each of its lanes)
@@ -438,7 +456,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         if (a.bias || two) {
             const float lo = tk_float(tk_lanes<L>(real && keep ? gv : 0x7fffffff, lane, tk_imin2));
             const float hi = tk_float(tk_lanes<L>(real && !keep ? gv : kNone, lane, tk_imax2));
-            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, err));
+            odd |= real && tk_group_close(gv, gr.error, 0.5f * lo + 0.5f * hi);
         }
 #pragma unroll
         for (int j = 0; j < VPL; ++j) v[j] = keep ? v[j] : kNone;
@@ -465,6 +483,7 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         // 4 choices: a lane a group 43.6, this 33.4 us)
         constexpr int GPL = 64 / L;
         int gv[GPL];
+        TkGroup gr[GPL];
         const int sh = min(32 - __builtin_clz(a.n_group - 1), L == 64 ? 6 : 4), parts = L >> sh;  // (n_group > 1)
         const int g0 = sub & ((1 << sh) - 1), part = sub >> sh, members = (per - part + parts - 1) / parts;
 #pragma unroll
@@ -506,12 +525,13 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
                     merge(std::integral_constant<int, 32>{});
                 }
             }
-            gv[k] = g >= a.n_group ? kNone : two && b2 != kNone ? tk_int(tk_float(b1) + tk_float(b2)) : b1;
+            gr[k] = {kNone, 0.0f};
+            if (k == 0 || L * k < a.n_group) gr[k] = tk_group(b1, two ? b2 : kNone, err);  // (past the last group: that again)
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < GPL; ++k)
-            if (part == 0 && g0 + L * k < a.n_group) val[g0 + L * k] = gv[k];
+            if (part == 0 && g0 + L * k < a.n_group) val[g0 + L * k] = gr[k].value;
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < GPL; ++k) gv[k] = sub + L * k < a.n_group ? val[sub + L * k] : kNone;
@@ -535,7 +555,9 @@ template <int L, int VPL, int GROUPED> __global__ void __launch_bounds__(64 * kT
         }
         if (a.bias || two) {
             const float lo = tk_float(tk_lanes<L>(low, lane, tk_imin2)), hi = tk_float(tk_lanes<L>(high, lane, tk_imax2));
-            odd |= hi != ninf && !(lo - hi > 2.0f * tk_margin(lo, err));
+#pragma unroll
+            for (int k = 0; k < GPL; ++k)
+                if (k == 0 || L * k < a.n_group) odd |= tk_group_close(gr[k].value, gr[k].error, 0.5f * lo + 0.5f * hi);
         }
         // (experts past E: none anyway)
         const float inv = 1.0f / (float)per;  // (e + 1/2) / per, e < 512: 2^-10 or more from a whole number

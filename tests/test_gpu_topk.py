@@ -271,3 +271,26 @@ def test_few_close_scores(dev, E, topk, close, score, at):
     import ternocl_amd as T
     x, b = close_ones(E + topk, 120, E, min(close, E), score, at)
     check(T, x, b, topk, "f32", score)
+
+
+@pytest.mark.parametrize("E,n_group,topk_group", [(16, 8, 4), (64, 8, 4), (126, 9, 4), (256, 8, 3), (320, 64, 20), (512, 16, 7)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [0.5, 50.0, 1000.0])
+def test_groups_of_opposite_biases(dev, E, n_group, topk_group, score, size):
+    """Best twos of opposite sign, whose sums are far smaller than their terms and nearly equal: the groups kept are
+    those of 64 bits.  (s1 + s2 = c in every group, up to 2^-22 to 2^-10 of c by token; biases w and -w, w = size..2 size.)"""
+    import ternocl_amd as T
+    g = torch.Generator().manual_seed(E + n_group)
+    Tk, per = 150, E // n_group
+    part = torch.rand((n_group, 1), generator=g).double() * 0.6 + 0.2
+    part = torch.cat((part, 1 - part), 1)
+    pair = torch.log(part) if score == "softmax" else torch.logit(part * 0.9)
+    x = torch.full((Tk, n_group, per), -6.0)
+    away = 2.0 ** (-22 + 12 * torch.rand((Tk, 1, 1), generator=g))
+    x[:, :, :2] = pair.float() * (1 + torch.randn((Tk, n_group, 2), generator=g) * away)
+    b = torch.full((n_group, per), -4.0 * size)
+    b[:, 0] = size * (1 + torch.rand(n_group, generator=g))
+    b[:, 1] = -b[:, 0]
+    order = torch.rand((n_group, per), generator=g).argsort(1)
+    x, b = x.gather(2, order.expand(Tk, -1, -1)), b.gather(1, order)
+    check(T, x.reshape(Tk, E), b.reshape(E), min(6, topk_group * per), "f32", score, n_group, topk_group, 2)
