@@ -99,7 +99,9 @@ struct TkGroup {
 };
 __device__ __forceinline__ TkGroup tk_group(int b1, int b2, float err) {
     const float x = tk_float(b1), y = b2 == kNone ? 0.0f : tk_float(b2);
-    return {tk_int(x + y), __builtin_fmaf(fabsf(y), 0x1.4p-23f, __builtin_fmaf(fabsf(x), 0x1.4p-23f, err))};
+    // (of two values above -inf the sum is no -inf, no empty group's value, in 64 bits)
+    constexpr int kLowest = (int)0x80800000u;  // tk_int(-FLT_MAX)
+    return {max(tk_int(x + y), min(b2, kLowest)), __builtin_fmaf(fabsf(y), 0x1.4p-23f, __builtin_fmaf(fabsf(x), 0x1.4p-23f, err))};
 }
 // Whether a group may be on the other side of mid, a value between the least kept and the
 // largest dropped one: where none is, exactly those kept are the largest.

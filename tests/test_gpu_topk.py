@@ -294,3 +294,19 @@ def test_groups_of_opposite_biases(dev, E, n_group, topk_group, score, size):
     order = torch.rand((n_group, per), generator=g).argsort(1)
     x, b = x.gather(2, order.expand(Tk, -1, -1)), b.gather(1, order)
     check(T, x.reshape(Tk, E), b.reshape(E), min(6, topk_group * per), "f32", score, n_group, topk_group, 2)
+
+
+@pytest.mark.parametrize("E", [16, 24, 60, 64, 100])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_at_the_lowest_value(dev, E, score):
+    """A group whose experts all have a bias of fp32's lowest value is worth the sum of two of them, below fp32's range,
+    and still comes before a group without experts."""
+    import ternocl_amd as T
+    x, b = logits_of(E, 20, E, "f32")
+    per, low = E // 4, torch.finfo(torch.float32).min
+    x[:10, per:2 * per] = -math.inf
+    b[2 * per:] = low
+    b[3 * per:] /= 1 + torch.arange(1, per + 1) * 2.0**-10  # (a little above it)
+    for kept in (1, 2, 3):
+        for topk in {min(15, kept * per), min(64, kept * per)}:
+            check(T, x, b, topk, "f32", score, 4, kept, 2)
