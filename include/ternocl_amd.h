@@ -524,11 +524,12 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
  *   RW    = scale * s[ids], with renorm divided by the sum of the chosen s first
  * Choices are made on v as in 64-bit arithmetic, without a bias on the logits, which
  * order the experts as s does and also tell apart what rounds to one s; sums and weights
- * are fp64, rounded to fp32, then to wtype.  An expert whose logit or v is -inf is never chosen and
- * adds nothing to its group's value; slots left without an expert get id -1 and
- * weight 0 (which the MoE entries skip).  A group without experts to choose counts
- * as -inf.  A NaN ranks first, and a softmax row with a NaN or +inf logit has NaN
- * weights.  Weights whose sum is 0 renormalise to 0.
+ * are fp64, rounded to fp32, then to wtype, but for the softmax sum under 16-bit weights
+ * that are not renormalised: fp32, within 2^-18 of its value.  An expert whose logit or v
+ * is -inf is never chosen and adds nothing to its group's value; slots left without an
+ * expert get id -1 and weight 0 (which the MoE entries skip).  A group without experts to
+ * choose counts as -inf.  A NaN ranks first, and a softmax row with a NaN or +inf logit
+ * has NaN weights.  Weights whose sum is 0 renormalise to 0.
  * logits: ltype [T, E] (TERNOCL_FP16, _BF16 or _FP32) with ld elements from row to
  * row (ld >= E); wtype: the same three.
  * 1 <= T <= 2^25, 1 <= E <= 512, 1 <= n_group <= 64 dividing E, 1 <= topk_group <= n_group,

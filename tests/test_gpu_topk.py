@@ -310,3 +310,26 @@ def test_groups_at_the_lowest_value(dev, E, score):
     for kept in (1, 2, 3):
         for topk in {min(15, kept * per), min(64, kept * per)}:
             check(T, x, b, topk, "f32", score, 4, kept, 2)
+
+
+@pytest.mark.parametrize("E,topk", [(64, 8), (200, 8), (512, 20)])
+def test_weights_as_they_are(dev, E, topk):
+    """Weights of a softmax that is not renormalised: fp32 ones over a 64-bit sum, 16-bit ones over an fp32 sum within
+    2^-18 of it.  (Most logits of a row lie together, so that the 32-bit terms are off the same way: |l - max| <= 6.5
+    in two roundings and a constant, 2.5 x 2^-24 of it each, 2 x 2^-24 for the exponential and 37 x 2^-24 for the
+    additions of 32 in a lane and 16 lanes are 55 x 2^-24.)"""
+    import ternocl_amd as T
+    g = torch.Generator().manual_seed(E)
+    Tk = 1500
+    x = -(2 + 4 * torch.rand((Tk, 1), generator=g)) * (1 + torch.randint(0, 256, (Tk, E), generator=g) * 2.0**-20)
+    x[:, ::E // topk] = torch.rand((Tk, len(range(0, E, E // topk))), generator=g) * 0.5
+    check(T, x, None, topk, "f32", renorm=False)
+    ids = torch.empty((Tk, topk), dtype=torch.int32, device="cuda")
+    want, w = gold(x, None, topk, "softmax", 1, 1, 1, False, 1.0)
+    for wt in ("f16", "bf16"):
+        RW = torch.empty((Tk, topk), dtype=NAMES[wt], device="cuda")
+        T.moe_topk(x.cuda(), None, ids, RW, Tk, E, topk, "softmax", renorm=False)
+        torch.cuda.synchronize()
+        assert torch.equal(ids.cpu(), want)
+        u = torch.finfo(NAMES[wt]).eps / 2
+        assert ((RW.cpu().double() - w).abs() <= ((1 + u) * (1 + 2.0**-24) * (1 + 2.0**-18 + 2.0**-36) - 1) * w).all()
