@@ -16,8 +16,9 @@
 //   values down to 2^-11 and bf16 values down to 2^-14 of their group's largest are t
 //   exactly; smaller ones are within 2^-22 of that largest.
 // * Per group and column: three int32 sums to one fp32 (exact digits, two roundings),
-//   times the activations' power of two and S.  Zero points take Z times the group's
-//   sum of t off.  A group with an infinity or NaN gets NaN for its power of two.
+//   times a sixteenth of the activations' power of two, and S.  Zero points take Z times
+//   the group's sum of activations off.  A group with an infinity or NaN gets NaN for its
+//   power of two.
 //
 // Work split: a workgroup stages the activations' digits in LDS once and walks 16-column
 // strips; its waves take parts of K, in 128-row steps (one 16-byte load a lane: 16
@@ -112,7 +113,7 @@ __device__ __forceinline__ void g4_stage8(const G4Args &a, uint8_t *lds, const G
         return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y)));
     }));
     const bool bad = mb >= 0x7f800000u;
-    const int e = max((int)(mb >> 23), 1) - 127;
+    const int e = max((int)(mb >> 23), 15) - 127;  // (2^-112 at least: bf16's multiples of 2^-133 are t exactly there)
     uint32_t t[8];
     int sum = 0;
 #pragma unroll
@@ -135,9 +136,10 @@ __device__ __forceinline__ void g4_stage8(const G4Args &a, uint8_t *lds, const G
     *(uint2 *)(p + 128) = make_uint2(g4_bytes<0>(t[2], t[6], t[3], t[7]), g4_bytes<0>(t[0], t[4], t[1], t[5]));
     if ((8 * u) % G == 0) {
         const int g = 8 * u / G;
-        const float s = bad ? __builtin_nanf("") : __builtin_ldexpf(1.0f, e - 21);
-        ((float *)(lds + l.scales))[g * mp + m] = s;
-        if constexpr (ZP) ((float *)(lds + l.sums))[g * mp + m] = (float)sum * s;
+        // (a sixteenth for the weights' 16: nothing on the way to a sum is larger than it is)
+        ((float *)(lds + l.scales))[g * mp + m] = bad ? __builtin_nanf("") : __builtin_ldexpf(1.0f, e - 25);
+        if constexpr (ZP)
+            ((float *)(lds + l.sums))[g * mp + m] = bad ? __builtin_nanf("") : __builtin_ldexpf((float)sum, e - 21);
     }
 }
 
@@ -301,8 +303,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves, g4_two(RS, G, ZP) ? 8 : 4) k_i
             for (int j = 0; j < GS; ++j) {
                 const int g = (t * GS + j) * MP + 4 * s;
                 const float f = __builtin_fmaf((float)D[j][0], 65536.0f, __builtin_fmaf((float)D[j][1], 256.0f, (float)D[j][2]));
-                float v = f * scales[g];  // 16 times the group's product
-                if constexpr (ZP) v = __builtin_fmaf(-16.0f * sz[GS + j], sums[g], v);
+                float v = f * scales[g];  // the group's product
+                if constexpr (ZP) v = __builtin_fmaf(-sz[GS + j], sums[g], v);
                 acc[s] = __builtin_fmaf(sz[j], v, acc[s]);
             }
         }
@@ -322,7 +324,6 @@ __global__ void __launch_bounds__(64 * kMaxWaves, g4_two(RS, G, ZP) ? 8 : 4) k_i
             for (int s = 0; s < RS; ++s) {
                 v[s] = r[s * 64 + lane];
                 for (int k = 1; k < W; ++k) v[s] += r[(k * RS + s) * 64 + lane];
-                v[s] *= 0.0625f;
             }
             epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
 #pragma unroll

@@ -254,3 +254,50 @@ def test_offsets_past_32_bits(dev, M):
         W = T.int4_unpack(B[:, cols].contiguous().cpu().numpy().view(np.uint32), K)
         want, d = gold(A.cpu(), torch.from_numpy(W), S[:, cols].cpu(), None, group, None, None, 0)
         assert ((C[:, cols].cpu().double() - want).abs() <= 2.0**-24 * want.abs() + d).all()
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 20, 300])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_largest_zero_points(dev, M, group):
+    """Zero points up to bf16's largest: rows and groups of zeros stay zero, sums within fp32 stay finite."""
+    import ternocl_amd as T
+    A, W, S, Z, dt = make(7, M, 256, 272, group, True, True)
+    g = torch.Generator().manual_seed(8)
+    Z = (Z.sign() * 2.0**124 * (1 + 14 * torch.rand(Z.shape, generator=g))).to(dt)
+    Z[:, :8] = torch.finfo(dt).max
+    A = (A.double() * 2.0**-60).to(dt)
+    A[0] = 0
+    A[:, 128:] = 0
+    got = run(T, A, W, S, Z, group, None, None, 0, True).cpu().double()
+    want, d = gold(A, W, S, Z, group, None, None, 0)
+    assert (got[0] == 0).all()
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + d).all()
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 20, 300])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_largest_sums(dev, M, group):
+    """Sums in the last octaves of fp32's range are no infinities at any number of rows (bf16; positive terms, so
+    that no partial sum is larger)."""
+    import ternocl_amd as T
+    A, W, S, _, dt = make(9, M, 256, 272, group, True, False, "positive")
+    W = W.abs().clamp(1, 7)
+    A, S = (A.double() * 2.0**60).to(dt), (S.double() * 2.0**62.5).to(dt)
+    got = run(T, A, W, S, None, group, None, None, 0, True).cpu().double()
+    want, d = gold(A, W, S, None, group, None, None, 0)
+    assert 2.0**125 < want.max() < 2.0**127.5
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + d).all()
+
+
+@pytest.mark.parametrize("M", [1, 8])
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("exp", [-110, -124, -130])
+def test_smallest_activations(dev, M, zero, exp):
+    """The decode rows' fixed point at the lower end of bf16, subnormal values among the activations."""
+    import ternocl_amd as T
+    A, W, S, Z, dt = make(10, M, 256, 32, 128, True, zero)
+    A, S = (A.double() * 2.0**exp).to(dt), (S.double() * 2.0**100).to(dt)
+    got = run(T, A, W, S, Z, 128, None, None, 0, True).cpu().double()
+    want, d = gold(A, W, S, Z, 128, None, None, 0)
+    # (a group's sum is a multiple of 2^-149 within half a unit, two of them with Z: times S, two groups)
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + d + 4 * 2.0**-149 * S.double().max()).all()
