@@ -488,11 +488,14 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
  *   group: rows per scale, 32, 64 or 128
  *   S    : DT [K/group, N] scales;  Z: DT [K/group, N] zero points, any finite
  *          value (NULL: 0)
- * Codes, activations and zero points are multiplied as they are and summed in fp32
- * (or exact integers) per group; nothing is rounded to DT before the epilogue.  A
- * row of A that holds an infinity or a NaN has infinities or NaN for its sums, before
- * the epilogue; no other row is changed by it.  (bf16: so may a row that holds values
- * past 2^112, whose sums over a group leave fp32.)
+ * Products are summed in fp32 (or exact integers) per group; nothing is rounded to DT
+ * before the epilogue.  M <= 8 (the GEMV below) rounds activations to within 2^-22 of
+ * the largest of their row and group first: fp16 values down to 2^-11 of that one and
+ * bf16 values down to 2^-14 are exact, far smaller ones are lost beside it, also where
+ * it meets codes equal to their zero point and adds nothing itself.
+ * A row of A that holds an infinity or a NaN has infinities or NaN for its sums, before
+ * the epilogue; no other row is changed by it.  So may a row whose sums over a group, or
+ * these times a zero point, leave fp32 (bf16 values past 2^112).
  * N % 16 == 0, K % 128 == 0, any M >= 1.  B starts on 16 bytes.  M <= 8 runs the
  * decode GEMV (A 16-byte aligned; K M up to some 50000), other calls a matrix-core
  * GEMM where every operand is 16-byte aligned, a plain kernel (several times slower)

@@ -301,3 +301,31 @@ def test_smallest_activations(dev, M, zero, exp):
     want, d = gold(A, W, S, Z, 128, None, None, 0)
     # (a group's sum is a multiple of 2^-149 within half a unit, two of them with Z: times S, two groups)
     assert ((got - want).abs() <= 2.0**-24 * want.abs() + d + 4 * 2.0**-149 * S.double().max()).all()
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 9, 33, 200])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_largest_activation_on_zero_codes(dev, M, bf16, group):
+    """One activation of each group far above the others, on weights of 0.  Up to 8 rows: each activation within 2^-22 of
+    its group's largest, the exact ones (2^-14 of it and more, and 0) as they are.  More rows at fp16: nothing is lost."""
+    import ternocl_amd as T
+    K, N = 512, 96
+    A, W, S, _, dt = make(12, M, K, N, group, bf16, False)
+    g = torch.Generator().manual_seed(13)
+    far = 2.0 ** -torch.randint(4, 31, (M, K // group, 1), generator=g)  # (of the largest, by row and group)
+    A = (A.view(M, K // group, group) * 1000 * far).reshape(M, K)
+    A[:, 5::group] = 20000.0
+    A = A.to(dt)
+    W[5::group] = 0
+    got = run(T, A, W, S, None, group, None, None, 0, True).cpu().double()
+    a, w = A.double(), W.double() * S.double().repeat_interleave(group, 0)
+    want = a @ w
+    d = (160 + K / 64) * 2.0**-24 * (a.abs() @ w.abs())
+    if M <= 8:
+        step = 2.0 ** (a.abs().view(M, K // group, group).amax(2).log2().floor() - 21)
+        off = torch.where(a % step.repeat_interleave(group, 1) == 0, 0.0, step.repeat_interleave(group, 1) / 2)
+        d += off @ w.abs()
+    elif bf16:  # (codes with an offset of 24, the largest activations' products with it taken off again)
+        d += (160 + K / 64) * 2.0**-24 * 32 * (a.abs() @ S.double().repeat_interleave(group, 0))
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + d).all()
