@@ -492,7 +492,10 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
  * before the epilogue.  M <= 8 (the GEMV below) rounds activations to within 2^-22 of
  * the largest of their row and group first: fp16 values down to 2^-11 of that one and
  * bf16 values down to 2^-14 are exact, far smaller ones are lost beside it, also where
- * it meets codes equal to their zero point and adds nothing itself.
+ * it meets codes equal to their zero point and adds nothing itself.  More rows of bf16
+ * or with zero points take codes as q + 24 and 24 + Z times a group's sum of activations
+ * off again (the 16-byte aligned engines): the fp32 roundings of sums of |a| (|q - Z| +
+ * 32) |S|, not of |a| |q - Z| |S|.
  * A row of A that holds an infinity or a NaN has infinities or NaN for its sums, before
  * the epilogue; no other row is changed by it.  So may a row whose sums over a group, or
  * these times a zero point, leave fp32 (bf16 values past 2^112).
