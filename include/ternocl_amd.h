@@ -506,8 +506,8 @@ ternocl_status ternocl_int2_moe_decode_noalloc(int dtype, const void *X, const i
  * ws / ws_bytes: optional device scratch of ternocl_int4_gemm_ws_bytes(M, N, K,
  * group) bytes (0: none used), 16-byte aligned, laid out and used as
  * ternocl_int2_fp16_upcvt_gemm's: a deterministic K split of few tiles over a long
- * K, fp32 slice sums added in slice order; its counters take any contents.  NULL
- * or short: unsplit. */
+ * K, fp32 slice sums added in slice order; its counters take any contents (up to some
+ * 6 us faster where they are zero, as each call leaves them).  NULL or short: unsplit. */
 size_t ternocl_int4_gemm_ws_bytes(int M, int N, int K, int group);
 ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z,
                                  void *C, const void *Other, const void *Bias, int M, int N, int K, int group,
@@ -559,7 +559,8 @@ ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const
  * element alignment.  1 <= M <= 2^23, V >= 1, 0 <= topn <= 64, 2^-100 <= scale <= 2^100.
  * ws: optional scratch of ternocl_logprobs_ws_bytes(M, V, topn) bytes (0: none used),
  * 16-byte aligned, any contents: rows are spread over workgroups where there are few,
- * their sums joined by the last (arrival counters in the header, left zero).  NULL or
+ * their sums joined by the last (arrival counters in the header, left zero; a header of
+ * other contents makes the call up to some 20 us longer).  NULL or
  * short: one workgroup a row.  The same results, to rounding, either way, and the same
  * bits every time.  Calls that share ws must not overlap. */
 size_t ternocl_logprobs_ws_bytes(int M, int V, int topn);

@@ -118,7 +118,8 @@ __device__ __forceinline__ uint32_t split_arrive(uint32_t *c, int ksn, int lane)
 // second word, by exchanges that take any value but a count of theirs for none.
 // The last arrival zeroes the words.  One atomic addition on a zeroed workspace:
 // counting by exchanges alone, retried whenever another slice arrives, took 4 us
-// more at 7 and 8 slices (M = 43 K = 7040 N = 512 9.0 -> 13.2).
+// more at 7 and 8 slices (M = 43 K = 7040 N = 512 9.0 -> 13.2), and takes 18 to 21 us more for
+// the 32 arrivals of a row of log probabilities.
 constexpr uint64_t kKwStep = 0x9E6D3A5171C3B20Full;
 __device__ __forceinline__ bool kw_arrive(uint64_t *c, int ksn, int lane) {
     bool last = false;

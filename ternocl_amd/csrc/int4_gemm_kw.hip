@@ -23,8 +23,9 @@
 // give too few tiles for a wave each.  M = 24 K = 14336 N = 4096 bf16 (30 MB, 6.0 us of a
 // large copy): 15.4 us a call, of which the walk's stream is 8.5, its first loads, the waves'
 // and the slices' meeting the rest.  The more columns' activations a row block reads through
-// L2, the more the walk waits for them (M = 200 K = N = 5120: VALU 34% of a wave's time, waits
-// 32%, MFMAs 27%); int4_gemm_tile.hip takes over there.
+// L2, the more the walk waits for them (M = 100 K = N = 5120 fp16, 64 x 64 tiles: VALU 35% of a
+// wave's time, waits for loads 29%, for issue 19%, MFMAs busy 23%); int4_gemm_tile.hip takes over
+// where i4_plan puts it ahead.
 #include "gemm_kw.hpp"
 #include "int4_decode.hpp"
 

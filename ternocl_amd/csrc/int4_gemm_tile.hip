@@ -5,11 +5,13 @@
 // A wave's 64 x 64 part: each decoded fragment feeds two row blocks and each activation
 // fragment two column blocks, with group sums (part) and the tile's (acc) in 128 registers;
 // two buffers of 64 rows of K and one barrier a unit; the activations two units ahead in
-// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 143 to 146 us a call, by box, 830
-// TFLOP/s, 71% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, the rest goes to
-// decode and group sums on the VALU.  Groups of 32 at bf16 or with zero points are VALU-bound:
-// per 64-row unit of a wave 256 FMAs join group sums and offsets, 64 operations decode, for 24
-// MFMAs, a third of them the offsets' (M = 200 K = N = 5120: 45.1 us, 232 TFLOP/s).
+// registers.  M = 1024 K = 4096 N = 14336 fp16, groups of 128: 141 to 149 us a call, by box, 807 to
+// 853 TFLOP/s, about 70% of a large matrix product's; its 448 tiles on 256 CUs leave 12% idle, and of a
+// wave's time VALU (decode, group sums) is 31%, waits for loads and barriers 30%, for issue 32%, MFMAs
+// busy 22%.  Groups of 32 at bf16 or with zero points: per 64-row unit of a wave 256 FMAs join group
+// sums and offsets, 64 operations decode, for 24 MFMAs, a third of them the offsets'; VALU 34%, the two
+// waits 30% and 31%, MFMAs 14% of a wave's time, with one wave a SIMD (M = 200 K = N = 5120: 45 us, 233
+// TFLOP/s).
 #include "gemm_kw.hpp"
 #include "int4_decode.hpp"
 

@@ -22,8 +22,10 @@
 // finds the exact topn-th (value, index) key.
 //
 // V = 151680, 20 alternatives: 512 rows fp32 61.6 us, 5.0 TB/s (a large copy's rate), bf16
-// 46.1 us (VALU and exponentials); one row 10.0 us (latency: the stream, the arrival, the
-// alternatives, and the code's fetch).
+// 46.1 us (a row a workgroup, two waves a SIMD, too few to put VALU beside loads: 39% of a wave's
+// time each, the SIMDs' VALU busy 54% of it); one row 10.2 us (latency: the stream, the arrival, the
+// alternatives, and the code's fetch).  On counters that were not left at zero the split rows
+// take 18 to 21 us more (kw_arrive counts its up to 32 arrivals by exchanges).
 #include "common.hpp"
 
 namespace tcl {

@@ -16,14 +16,17 @@
 //     rounds compare fp32 logits, exactly.
 //   * With a bias (and for the sums of two that value a group) v is computed in fp32.
 //     Where two picks in a row are closer than its error (tk_margin) tells apart, the picks
-//     up to the next wider gap are ranked by their 64-bit values; where the last group kept
-//     and the first one dropped are, or a value is NaN or +inf, the token is done again
-//     with 64-bit values (tk_exact, the whole wave).  Of N(0, 1.5) logits over 256 experts,
+//     up to the next wider gap are ranked by their 64-bit values; where there is none before
+//     the list's end, where groups kept and dropped may be the other way round (TkGroup), or a
+//     value is NaN or +inf, the token is done again with 64-bit values (tk_exact, the whole
+//     wave).  Of N(0, 1.5) logits over 256 experts,
 //     sigmoid scores, about 1 token in 2000 has close picks, 1 in 16000 close groups.
 //
-// What bounds it: launch and latency for few tokens (T = 1 E = 128 3.2 us, T = 2048 E = 64 4.2
-// us), VALU issue for many (T = 16384 E = 256 fp32, 8 of 4 of 8 groups with a bias: 14.7 us, 1.2
-// TB/s; without either, bf16: 7.2 us).
+// What bounds it: launch and latency for few tokens (T = 1 E = 128 3.2 us, T = 2048 E = 64 4.0
+// us).  For many, the latency of a wave's dependent steps: T = 16384 E = 256 fp32, 8 of 4 of 8
+// groups with a bias, 12.4 us, 15 to 17.7 where some token takes 64 bits; a wave's time is 18% VALU,
+// 48% waits for loads and LDS, 23% waits for issue, and the SIMDs' VALU is busy 28% of it.  Without
+// either, bf16: 7.2 us (17%, 58%, 18%).
 #include "common.hpp"
 
 #include <algorithm>

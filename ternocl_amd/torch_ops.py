@@ -312,7 +312,10 @@ def _(X, ids, RW, E, Bg, Sg, Bu, Su, Bd, Sd):
 # ---- the calls around those layers -----------------------------------------------------
 # They launch on the current stream of their tensors' device, whichever device is
 # current.  Their workspaces need no zeroing: one is allocated per call, so that a
-# captured graph keeps its own and two graphs, or two streams, never share one.
+# captured graph keeps its own and two graphs, or two streams, never share one.  Where
+# its memory held another tensor since the last such call, the arrival counters are not
+# zero and the kernel takes longer: 1 to 2 us for the K splits of the 4-bit products' usual
+# shapes (6 at most), 18 to 21 us for few rows of log probabilities.
 
 def _scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
