@@ -517,6 +517,56 @@ ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, co
 ternocl_status ternocl_int4_pack(const int8_t *W, uint32_t *B, int K, int N);
 ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
 
+/* ---- norm and 8-bit rows ---------------------------------------------------------
+ * What comes before a layer's products (no reference counterpart): the residual's
+ * addition, the root-mean-square norm and the activations in 8 bits, in one pass:
+ *   h = x + r (R NULL: x),  n = h (woff + w) / sqrt(mean_k h^2 + eps)
+ *   H = DT(h)   [M, K], may be X or R itself;  NULL: not written
+ *   Y = DT(n)   [M, K];  NULL: not written
+ *   quant 0: no codes (Q and SQ not written, Y non-null)
+ *   quant 1: Q int8 [M, K], SQ fp32 [M]: a scale for each row, for ternocl_int8_gemm:
+ *     SQ = max_k |n| / 127, Q = rne(n / SQ) of the unrounded n (a code is the one that
+ *     64-bit arithmetic gives).  A row of zeros has scale 0 and codes 0; a row with an
+ *     infinity or a NaN scale NaN and codes 0, so that its products are NaN and no other
+ *     row's change.
+ *   quant 2: Q and SQ of ternocl_quant_a(Y), bit for bit (SQ DT [K/128, ternocl_ldsa(M)],
+ *     pad columns not written), for ternocl_int2_int8_gemm; K % 128 == 0.
+ * X, R: DT [M, K] with ldx, ldr >= K elements from row to row.  W: [K] of wtype
+ * (TERNOCL_FP16, _BF16 or _FP32; NULL: a weight of 1, woff not read); woff: 0, or 1 for
+ * weights kept about zero; eps > 0.  Sums and norms are 64-bit; H and Y are rounded to
+ * fp32, then to DT.  1 <= M <= 2^23, K >= 1.  Rows of 8-element multiples up to K = 32768
+ * whose pointers and pitches are multiples of 16 bytes (Q: 8) take a kernel that reads
+ * each element once, others a slower one.  No output overlaps another tensor but H as said. */
+ternocl_status ternocl_rmsnorm(int dtype, const void *X, int64_t ldx, const void *R, int64_t ldr, int wtype, const void *W,
+                               float woff, float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K,
+                               void *stream);
+/* The codes and scales alone (quant 1 of n = x): what goes into an MLP's second product. */
+ternocl_status ternocl_quant_rows(int dtype, const void *X, int64_t ldx, int8_t *Q, float *SQ, int M, int K, void *stream);
+
+/* ---- int8 GEMV / GEMM -------------------------------------------------------------
+ * Products of 8-bit integers with a scale for each token and each channel, for the
+ * projections that a model of ternary layers keeps at 8 bits (no reference counterpart;
+ * C, Other, Bias, epilogues and workspace are those of ternocl_int2_fp16_upcvt_gemm):
+ *   C[m,n] = ct(epi((sum_k A[m,k] B[k,n]) SB[n] SA[m]))
+ *   A    : int8 [M, K], SA: fp32 [M] (ternocl_rmsnorm, ternocl_quant_rows)
+ *   B    : int8 [K/16][N][16], 16 rows of a column together; SB: fp32 [N]
+ * Sums are exact (any int8 values, -128 too), rounded once to fp32, multiplied by SB[n],
+ * then by SA[m].  A scale of NaN makes its row's or column's products NaN.
+ * dtype: DT of Other, of C and Bias without out_f32.
+ * N % 16 == 0, K % 128 == 0, K < 2^17, any M >= 1.  B starts on 16 bytes; operands that are
+ * not all 16-byte aligned run a plain kernel (several times slower).
+ * ws / ws_bytes: optional device scratch of ternocl_int8_gemm_ws_bytes(M, N, K) bytes (0:
+ * none used), 16-byte aligned, laid out and used as ternocl_int2_fp16_upcvt_gemm's: a K
+ * split of few tiles over a long K (the same bits as without).  Its counters take any
+ * contents.  NULL or short: unsplit.  Calls that share ws must not overlap. */
+size_t ternocl_int8_gemm_ws_bytes(int M, int N, int K);
+ternocl_status ternocl_int8_gemm(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
+                                 const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32,
+                                 void *ws, size_t ws_bytes, void *stream);
+/* Host packers of that format (CPU; no GPU call): W int8 [K, N] row-major; K % 16 == 0. */
+ternocl_status ternocl_int8_pack(const int8_t *W, int8_t *B, int K, int N);
+ternocl_status ternocl_int8_unpack(const int8_t *B, int8_t *W, int K, int N);
+
 /* ---- MoE routing -----------------------------------------------------------------
  * The experts and weights of each token from its router logits, as the MoE entries
  * take them (ids int32 [T, topk], RW [T, topk]; no reference counterpart):

@@ -29,7 +29,8 @@ __all__ = [
     "hadamard_fwht",
     "moe_tile_rows", "int2_moe_route", "int2_moe_gather", "int2_moe_gemm", "int2_moe_combine",
     "int2_moe_prefill_ws_bytes", "int2_moe_prefill", "int2_moe_prefill_int8_ws_bytes", "int2_moe_prefill_int8",
-    "int4_gemm", "int4_gemm_ws_bytes", "int4_pack", "int4_unpack", "moe_topk", "logprobs", "logprobs_ws_bytes",
+    "int4_gemm", "int4_gemm_ws_bytes", "int4_pack", "int4_unpack", "rmsnorm", "quant_rows",
+    "int8_gemm", "int8_gemm_ws_bytes", "int8_pack", "int8_unpack", "moe_topk", "logprobs", "logprobs_ws_bytes",
 ]
 
 FP16, BF16, FP32 = 0, 1, 2  # (FP32: logits and routing weights)
@@ -480,6 +481,67 @@ def int4_unpack(B, K: int):
         raise TernoclError(1, f"int4_unpack: B must be [K/32, N, 4], got {list(B.shape)} with K = {K}")
     W = np.empty((K, B.shape[1]), np.int8)
     _check(lib().ternocl_int4_unpack(_cptr(B), _cptr(W), K, B.shape[1]))
+    return W
+
+
+# ---- norm, 8-bit rows and products of 8-bit integers (no reference counterpart) -------------
+
+_QUANTS = {"none": 0, "rows": 1, "groups": 2}
+
+
+def rmsnorm(X, R, W, H, Y, Q, SQ, M: int, K: int, eps: float = 1e-6, woff: float = 0.0, quant: str = "none", ldx=None,
+            ldr=None, stream=None) -> None:
+    """h = X + R (R None: X); H = h; n = h (woff + W) / sqrt(mean(h^2) + eps); Y = n; H and Y in X's dtype or
+    None, H may be X or R.  quant "rows": Q int8 [M, K] and SQ fp32 [M] with n = Q SQ, for ``int8_gemm``;
+    "groups": ``quant_a``'s SQ [K/128, ldsa(M)] and Q of Y, for ``int2_int8_gemm``; "none": neither.  W: [K]
+    fp16, bf16 or fp32, or None (a weight of 1); ldx, ldr: elements from row to row (K)."""
+    if quant not in _QUANTS:
+        raise TernoclError(1, f"quant must be 'none', 'rows' or 'groups', got {quant!r}")
+    _check(lib().ternocl_rmsnorm(_dtype_of(X), _ptr(X), K if ldx is None else ldx, _ptr(R), K if ldr is None else ldr,
+                                 0 if W is None else _float_type(W), _ptr(W), woff, eps, _ptr(H), _ptr(Y), _QUANTS[quant],
+                                 _ptr(Q), _ptr(SQ), M, K, _stream(stream)))
+
+
+def quant_rows(X, Q, SQ, M: int, K: int, ld=None, stream=None) -> None:
+    """Q int8 [M, K] and SQ fp32 [M] with X = Q SQ, the largest of a row at 127, for ``int8_gemm``; ld: elements
+    from row to row of X (K)."""
+    _check(lib().ternocl_quant_rows(_dtype_of(X), _ptr(X), K if ld is None else ld, _ptr(Q), _ptr(SQ), M, K, _stream(stream)))
+
+
+def int8_gemm_ws_bytes(M: int, N: int, K: int) -> int:
+    """Workspace bytes of ``int8_gemm`` (0 when none is used)."""
+    return lib().ternocl_int8_gemm_ws_bytes(M, N, K)
+
+
+def int8_gemm(A, SA, B, SB, C, Other, Bias, M: int, N: int, K: int, postop: int = 0, out_f32: bool = False, ws=None,
+              stream=None) -> None:
+    """C = ct(epi((A x B) SB SA)): A int8 [M, K] with token scales SA fp32 [M] (``rmsnorm``, ``quant_rows``), B int8
+    [K/16, N, 16] of ``int8_pack`` with channel scales SB fp32 [N], the epilogues of ``int2_fp16_upcvt_gemm``.
+    ``ws`` (int8_gemm_ws_bytes, 16-byte aligned): the K split of few tiles over a long K."""
+    d = Other if out_f32 else C  # (what is of 16 bits: C and Bias, or Other alone)
+    _check(lib().ternocl_int8_gemm(FP16 if d is None else _dtype_of(d), _ptr(A), _ptr(SA), _ptr(B), _ptr(SB), _ptr(C),
+                                   _ptr(Other), _ptr(Bias), M, N, K, postop, int(bool(out_f32)), _ptr(ws), _nbytes(ws),
+                                   _stream(stream)))
+
+
+def int8_pack(W):
+    """int8 [K, N] -> B int8 [K/16, N, 16] (ternocl_int8_pack, on the host)."""
+    import numpy as np
+    W = _host_i8(W)
+    K, N = W.shape
+    B = np.empty((K // 16, N, 16), np.int8)
+    _check(lib().ternocl_int8_pack(_cptr(W), _cptr(B), K, N))
+    return B
+
+
+def int8_unpack(B, K: int):
+    """B int8 [K/16, N, 16] -> int8 [K, N] (ternocl_int8_unpack, on the host)."""
+    import numpy as np
+    B = np.ascontiguousarray(B, dtype=np.int8)
+    if B.ndim != 3 or B.shape[0] != K // 16 or B.shape[2] != 16:
+        raise TernoclError(1, f"int8_unpack: B must be [K/16, N, 16], got {list(B.shape)} with K = {K}")
+    W = np.empty((K, B.shape[1]), np.int8)
+    _check(lib().ternocl_int8_unpack(_cptr(B), _cptr(W), K, B.shape[1]))
     return W
 
 

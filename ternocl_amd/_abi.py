@@ -76,6 +76,12 @@ SYMBOLS: dict[str, tuple] = {
     "ternocl_int4_gemm": (I, [I, P, P, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
     "ternocl_int4_pack": (I, [P, P, I, I]),
     "ternocl_int4_unpack": (I, [P, P, I, I]),
+    "ternocl_rmsnorm": (I, [I, P, C.c_int64, P, C.c_int64, I, P, C.c_float, C.c_float, P, P, I, P, P, I, I, P]),
+    "ternocl_quant_rows": (I, [I, P, C.c_int64, P, P, I, I, P]),
+    "ternocl_int8_gemm_ws_bytes": (Z, [I, I, I]),
+    "ternocl_int8_gemm": (I, [I, P, P, P, P, P, P, P, I, I, I, I, I, P, Z, P]),
+    "ternocl_int8_pack": (I, [P, P, I, I]),
+    "ternocl_int8_unpack": (I, [P, P, I, I]),
     "ternocl_moe_topk": (I, [I, P, C.c_int64, P, P, I, P, I, I, I, I, I, I, I, I, C.c_float, P]),
     "ternocl_logprobs_ws_bytes": (Z, [I, I, I]),
     "ternocl_logprobs": (I, [I, P, C.c_int64, P, P, P, P, P, I, I, I, C.c_float, P, Z, P]),

@@ -148,6 +148,14 @@ ternocl_status moe_decode_noalloc_run(int dtype, const void *X, const int *ids, 
                                       int topk, int H, int I, const uint32_t *Bg, const void *Sg,
                                       const uint32_t *Bu, const void *Su, const uint32_t *Bd, const void *Sd,
                                       void *O, hipStream_t st);
+// kernels (rmsnorm.hip)
+ternocl_status rmsnorm_run(int dtype, const void *X, long ldx, const void *R, long ldr, int wtype, const void *W, float woff,
+                           float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K, hipStream_t st);
+ternocl_status quant_rows_run(int dtype, const void *X, long ldx, int8_t *Q, float *SQ, int M, int K, hipStream_t st);
+// kernels (int8_plain.hip)
+ternocl_status int8_plain_run(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
+                              const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32,
+                              hipStream_t st);
 // kernels (int4_gemv.hip)
 bool int4_gemv_supports(int M, int K, int group, bool zero);
 ternocl_status int4_gemv_run(int dtype, const void *A, const uint32_t *B, const void *S, const void *Z, void *C,
@@ -208,6 +216,8 @@ static ternocl_status check_gemm_common(int dtype, const void *A, const void *B,
     if (postop_needs_bias(postop) && !Bias) FAIL(TERNOCL_ERR_INVALID_ARG, "this postop reads Bias: it must be non-null");
     return TERNOCL_OK;
 }
+
+constexpr int kInt8MaxK = (1 << 17) - 128;  // 2^14 K below 2^31
 
 extern "C" {
 
@@ -715,9 +725,68 @@ ternocl_status ternocl_int4_gemm(int dtype, const void *A, const uint32_t *B, co
     return int4_plain_run(dtype, A, B, S, Z, C, Other, Bias, M, N, K, group, postop, out_f32, (hipStream_t)stream);
 }
 
-// ---- routing, log probabilities ------------------------------------------------
+// ---- norm, 8-bit rows, products of 8-bit integers --------------------------------
 
 static bool float_type(int t) { return t == TERNOCL_FP16 || t == TERNOCL_BF16 || t == TERNOCL_FP32; }
+
+static ternocl_status check_rows(int dtype, const void *X, int64_t ldx, int M, int K) {
+    ternocl_status s = check_dtype(dtype);
+    if (s != TERNOCL_OK) return s;
+    if (!X) FAIL(TERNOCL_ERR_INVALID_ARG, "X must be non-null");
+    if (M < 1 || M > 1 << 23 || K < 1) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need 1 <= M <= 2^23 and K >= 1");
+    if (ldx < K) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ldx must be at least K");
+    if ((uintptr_t)X & 1) FAIL(TERNOCL_ERR_INVALID_ARG, "X must be aligned to its element");
+    return TERNOCL_OK;
+}
+
+ternocl_status ternocl_rmsnorm(int dtype, const void *X, int64_t ldx, const void *R, int64_t ldr, int wtype, const void *W,
+                               float woff, float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K,
+                               void *stream) {
+    ternocl_status s = check_rows(dtype, X, ldx, M, K);
+    if (s != TERNOCL_OK) return s;
+    if (R && ldr < K) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "ldr must be at least K");
+    if (W && !float_type(wtype)) FAIL(TERNOCL_ERR_INVALID_ARG, "wtype must be TERNOCL_FP16, TERNOCL_BF16 or TERNOCL_FP32");
+    if (!std::isfinite(woff)) FAIL(TERNOCL_ERR_INVALID_ARG, "woff must be finite");
+    if (!(eps > 0.0f) || !std::isfinite(eps)) FAIL(TERNOCL_ERR_INVALID_ARG, "eps must be positive and finite");
+    if (quant < 0 || quant > 2) FAIL(TERNOCL_ERR_INVALID_ARG, "quant must be 0 (none), 1 (rows) or 2 (groups)");
+    if (quant && (!Q || !SQ)) FAIL(TERNOCL_ERR_INVALID_ARG, "quant writes Q and SQ: both must be non-null");
+    if (!quant && !Y) FAIL(TERNOCL_ERR_INVALID_ARG, "nothing to compute: Y is null and quant 0");
+    if (quant == 2 && K % kGS) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "quant 2: K must be a multiple of 128");
+    if (H && !R) FAIL(TERNOCL_ERR_INVALID_ARG, "H is the sum with R: R must be non-null");
+    if (H && M > 1 && ((H == X && ldx != K) || (H == R && ldr != K)))
+        FAIL(TERNOCL_ERR_INVALID_ARG, "H has rows of K elements: in place of X or R these must have them too");
+    if (((uintptr_t)R | (uintptr_t)H | (uintptr_t)Y | (quant == 2 ? (uintptr_t)SQ : 0)) & 1 ||
+        (quant == 1 && ((uintptr_t)SQ & 3)) || ((uintptr_t)W & (wtype == TERNOCL_FP32 ? 3 : 1)))
+        FAIL(TERNOCL_ERR_INVALID_ARG, "R, W, H, Y and SQ must be aligned to their elements");
+    return rmsnorm_run(dtype, X, (long)ldx, R, (long)ldr, wtype, W, woff, eps, H, Y, quant, Q, SQ, M, K, (hipStream_t)stream);
+}
+
+ternocl_status ternocl_quant_rows(int dtype, const void *X, int64_t ldx, int8_t *Q, float *SQ, int M, int K, void *stream) {
+    ternocl_status s = check_rows(dtype, X, ldx, M, K);
+    if (s != TERNOCL_OK) return s;
+    if (!Q || !SQ) FAIL(TERNOCL_ERR_INVALID_ARG, "Q and SQ must be non-null");
+    if ((uintptr_t)SQ & 3) FAIL(TERNOCL_ERR_INVALID_ARG, "SQ must be aligned to its element");
+    return quant_rows_run(dtype, X, (long)ldx, Q, SQ, M, K, (hipStream_t)stream);
+}
+
+size_t ternocl_int8_gemm_ws_bytes(int M, int N, int K) {
+    if (M < 1 || N < 16 || N % 16 || K < kGS || K % kGS || K > kInt8MaxK) return 0;
+    return 0;
+}
+
+ternocl_status ternocl_int8_gemm(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
+                                 const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32,
+                                 void *ws, size_t ws_bytes, void *stream) {
+    ternocl_status s = check_gemm_common(dtype, A, B, SB, C, Other, Bias, M, N, K, postop, out_f32);
+    if (s != TERNOCL_OK) return s;
+    if (!SA) FAIL(TERNOCL_ERR_INVALID_ARG, "SA must be non-null");
+    if (K > kInt8MaxK) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "K must be below 2^17 (sums of 32 bits)");
+    if ((uintptr_t)B & 15) FAIL(TERNOCL_ERR_INVALID_ARG, "B must be 16-byte aligned");
+    if (((uintptr_t)SA | (uintptr_t)SB) & 3) FAIL(TERNOCL_ERR_INVALID_ARG, "SA and SB must be aligned to their elements");
+    return int8_plain_run(dtype, A, SA, B, SB, C, Other, Bias, M, N, K, postop, out_f32, (hipStream_t)stream);
+}
+
+// ---- routing, log probabilities ------------------------------------------------
 
 ternocl_status ternocl_moe_topk(int ltype, const void *logits, int64_t ld, const float *bias, int *ids, int wtype,
                                 void *RW, int T, int E, int topk, int score, int n_group, int topk_group,

@@ -10,7 +10,8 @@
 //     column after column, each padded to whole words with zeros) and 4 zero
 //     pad words; slice ranks [ls-1][N] = non-zeros of column n in the bitmap
 //     words below s * ceil(K / ls) / 32 (common/bitcos.hpp:81-94);
-//   * int4 (values -8..7): the layout of ternocl_int4_gemm.
+//   * int4 (values -8..7): the layout of ternocl_int4_gemm;
+//   * int8: the layout of ternocl_int8_gemm.
 // Nothing here touches the GPU.
 #include <cstdint>
 #include <cstring>
@@ -85,6 +86,24 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N) {
                 W[(size_t)(8 * kw + r) * N + n] = (int8_t)(q > 7 ? q - 16 : q);
             }
         }
+    return TERNOCL_OK;
+}
+
+ternocl_status ternocl_int8_pack(const int8_t *W, int8_t *B, int K, int N) {
+    if (!W || !B) FAIL(TERNOCL_ERR_INVALID_ARG, "W and B must be non-null");
+    if (N < 1 || K < 16 || K % 16) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need N >= 1 and K % 16 == 0");
+    for (int kb = 0; kb < K / 16; ++kb)
+        for (int n = 0; n < N; ++n)
+            for (int r = 0; r < 16; ++r) B[((size_t)kb * N + n) * 16 + r] = W[(size_t)(16 * kb + r) * N + n];
+    return TERNOCL_OK;
+}
+
+ternocl_status ternocl_int8_unpack(const int8_t *B, int8_t *W, int K, int N) {
+    if (!W || !B) FAIL(TERNOCL_ERR_INVALID_ARG, "W and B must be non-null");
+    if (N < 1 || K < 16 || K % 16) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "need N >= 1 and K % 16 == 0");
+    for (int kb = 0; kb < K / 16; ++kb)
+        for (int n = 0; n < N; ++n)
+            for (int r = 0; r < 16; ++r) W[(size_t)(16 * kb + r) * N + n] = B[((size_t)kb * N + n) * 16 + r];
     return TERNOCL_OK;
 }
 

@@ -23,6 +23,9 @@ Operators (the reference kernels they stand for, as in the C ABI):
   moe_prefill_int8  the int8 MoE prefill layer            (int2_moe/int2_moe_prefill_int8.cl)
 and, without a reference counterpart, what stands around those layers in a model:
   int4_gemm         products with 4-bit weights and group scales (a head)
+  rmsnorm           the residual's addition, the norm and its output in 8 bits
+  quant_rows        activations in 8 bits with a scale for each row
+  int8_gemm         products of 8-bit integers with a scale for each token and channel
   moe_topk          routing: router logits -> the MoE layers' ids and weights
   logprobs          log probabilities, entropy and top alternatives of logits
 """
@@ -35,7 +38,7 @@ import torch
 import ternocl_amd as T
 
 __all__ = ["int2_gemm", "quant_a", "int2_int8_gemm", "bitcos_gemm", "fwht", "moe_prefill", "moe_decode", "moe_prefill_int8",
-           "int4_gemm", "moe_topk", "logprobs"]
+           "int4_gemm", "rmsnorm", "quant_rows", "int8_gemm", "moe_topk", "logprobs"]
 
 
 def _out_dtype(A: torch.Tensor, out_f32: bool) -> torch.dtype:
@@ -371,6 +374,112 @@ def _chk_rows(x: torch.Tensor, name: str) -> None:
 
 def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _chk_norm(x, residual, weight, quant) -> None:
+    _chk_rows(x, "x")
+    torch._check(x.dtype in _DT, lambda: f"x: dtype {x.dtype}, expected float16 or bfloat16")
+    torch._check(x.shape[1] >= 1, lambda: "x must have columns")
+    if residual is not None:
+        _chk_rows(residual, "residual")
+        torch._check(residual.dtype == x.dtype and residual.shape == x.shape and residual.device == x.device,
+                     lambda: "residual must have x's dtype, shape and device")
+    _chk(weight, "weight", _LT, (x.shape[1],), x.device)
+    torch._check(quant in T._QUANTS, lambda: "quant must be 'none', 'rows' or 'groups'")
+    torch._check(quant != "groups" or x.shape[1] % 128 == 0, lambda: "groups: x must have a multiple of 128 columns")
+
+
+def _norm_out(x, residual, quant, norm):
+    """(h, y, q, scales), what is not asked for without elements."""
+    M, K = x.shape
+    h = x.new_empty((M, K) if residual is not None else (0,))
+    y = x.new_empty((M, K) if norm else (0,))
+    q = x.new_empty((M, K) if quant != "none" else (0,), dtype=torch.int8)
+    if quant == "groups":
+        s = x.new_empty((K // 128, (M + 31) // 32 * 32))
+    else:
+        s = x.new_empty((M,) if quant == "rows" else (0,), dtype=torch.float32)
+    return h, y, q, s
+
+
+@torch.library.custom_op("ternocl::rmsnorm", mutates_args=())
+def rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float, woff: float,
+            quant: str, norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(h, y, q, scales) of x [M, K]: h = x + residual, y = rmsnorm(h) * (woff + weight) where norm asks for it, its
+    codes q int8 [M, K] and scales: "rows" fp32 [M] for int8_gemm, "groups" quant_a's for int2_int8_gemm, "none"."""
+    _chk_norm(x, residual, weight, quant)
+    torch._check(norm or quant != "none", lambda: "nothing to compute: norm is false and quant 'none'")
+    M, K = x.shape
+    h, y, q, s = _norm_out(x, residual, quant, norm)
+    if M:
+        with torch.cuda.device(x.device):
+            T.rmsnorm(x, residual, weight, h if residual is not None else None, y if norm else None,
+                      q if quant != "none" else None, s if quant != "none" else None, M, K, eps, woff, quant,
+                      ldx=_pitch(x), ldr=None if residual is None else _pitch(residual))
+    return h, y, q, s
+
+
+@rmsnorm.register_fake
+def _(x, residual, weight, eps, woff, quant, norm):
+    _chk_norm(x, residual, weight, quant)
+    return _norm_out(x, residual, quant, norm)
+
+
+@torch.library.custom_op("ternocl::quant_rows", mutates_args=())
+def quant_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q int8 [M, K], scales fp32 [M]) of x [M, K], x = q * scales[:, None]."""
+    _chk_norm(x, None, None, "rows")
+    M, K = x.shape
+    _, _, q, s = _norm_out(x, None, "rows", False)
+    if M:
+        with torch.cuda.device(x.device):
+            T.quant_rows(x, q, s, M, K, ld=_pitch(x))
+    return q, s
+
+
+@quant_rows.register_fake
+def _(x):
+    _chk_norm(x, None, None, "rows")
+    return _norm_out(x, None, "rows", False)[2:]
+
+
+def _chk_int8_gemm(A, SA, B, SB, dtype, other, bias, out_f32) -> None:
+    torch._check(A.dim() == 2 and B.dim() == 3, lambda: "A must be int8 [M, K], B int8 [K/16, N, 16]")
+    M, K = A.shape
+    N = B.shape[1]
+    d = A.device
+    torch._check(dtype in _DT, lambda: "dtype must be float16 or bfloat16")
+    torch._check(128 <= K < 2**17 and K % 128 == 0, lambda: "K must be a multiple of 128 below 2^17")
+    torch._check(N >= 16 and N % 16 == 0, lambda: "N must be a multiple of 16")
+    _chk(A, "A", torch.int8, (M, K), d)
+    _chk(SA, "SA", torch.float32, (M,), d)
+    _chk(B, "B", torch.int8, (K // 16, N, 16), d)
+    _chk(SB, "SB", torch.float32, (N,), d)
+    _chk(other, "other", dtype, (M, N), d)
+    _chk(bias, "bias", torch.float32 if out_f32 else dtype, (N,), d)
+
+
+@torch.library.custom_op("ternocl::int8_gemm", mutates_args=())
+def int8_gemm(A: torch.Tensor, SA: torch.Tensor, B: torch.Tensor, SB: torch.Tensor, dtype: torch.dtype,
+              other: Optional[torch.Tensor], bias: Optional[torch.Tensor], postop: int, out_f32: bool) -> torch.Tensor:
+    """C [M, N] = epi((A x B) SB SA) in dtype (fp32 with out_f32): A int8 [M, K], SA fp32 [M] (rmsnorm, quant_rows), B
+    int8 [K/16, N, 16] (int8_pack), SB fp32 [N]; other and bias in C's dtype (other in dtype also with out_f32)."""
+    _chk_int8_gemm(A, SA, B, SB, dtype, other, bias, out_f32)
+    M, K = A.shape
+    N = B.shape[1]
+    C = torch.empty((M, N), dtype=torch.float32 if out_f32 else dtype, device=A.device)
+    if M == 0:
+        return C
+    with torch.cuda.device(A.device):
+        ws = _scratch(A.device, T.int8_gemm_ws_bytes(M, N, K))
+        T.int8_gemm(A, SA, B, SB, C, other, bias, M, N, K, postop, out_f32, ws=ws)
+    return C
+
+
+@int8_gemm.register_fake
+def _(A, SA, B, SB, dtype, other, bias, postop, out_f32):
+    _chk_int8_gemm(A, SA, B, SB, dtype, other, bias, out_f32)
+    return A.new_empty((A.shape[0], B.shape[1]), dtype=torch.float32 if out_f32 else dtype)
 
 
 def _chk_topk(logits, bias, topk, dtype) -> None:
