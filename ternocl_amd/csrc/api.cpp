@@ -152,6 +152,11 @@ ternocl_status moe_decode_noalloc_run(int dtype, const void *X, const int *ids, 
 ternocl_status rmsnorm_run(int dtype, const void *X, long ldx, const void *R, long ldr, int wtype, const void *W, float woff,
                            float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K, hipStream_t st);
 ternocl_status quant_rows_run(int dtype, const void *X, long ldx, int8_t *Q, float *SQ, int M, int K, hipStream_t st);
+// kernels (int8_gemm_kw.hip, int8_gemm_tile.hip)
+size_t int8_gemm_ws_need(int M, int N, int K);
+ternocl_status int8_gemm_run(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
+                             const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32, void *ws,
+                             size_t ws_bytes, hipStream_t st);
 // kernels (int8_plain.hip)
 ternocl_status int8_plain_run(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
                               const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32,
@@ -218,6 +223,7 @@ static ternocl_status check_gemm_common(int dtype, const void *A, const void *B,
 }
 
 constexpr int kInt8MaxK = (1 << 17) - 128;  // 2^14 K below 2^31
+constexpr int kInt8MaxN = 1 << 26;          // 4 blocks of 16 rows of K in 32-bit offsets
 
 extern "C" {
 
@@ -771,7 +777,7 @@ ternocl_status ternocl_quant_rows(int dtype, const void *X, int64_t ldx, int8_t 
 
 size_t ternocl_int8_gemm_ws_bytes(int M, int N, int K) {
     if (M < 1 || N < 16 || N % 16 || K < kGS || K % kGS || K > kInt8MaxK) return 0;
-    return 0;
+    return int8_gemm_ws_need(M, N, K);
 }
 
 ternocl_status ternocl_int8_gemm(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
@@ -783,6 +789,9 @@ ternocl_status ternocl_int8_gemm(int dtype, const int8_t *A, const float *SA, co
     if (K > kInt8MaxK) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "K must be below 2^17 (sums of 32 bits)");
     if ((uintptr_t)B & 15) FAIL(TERNOCL_ERR_INVALID_ARG, "B must be 16-byte aligned");
     if (((uintptr_t)SA | (uintptr_t)SB) & 3) FAIL(TERNOCL_ERR_INVALID_ARG, "SA and SB must be aligned to their elements");
+    const uintptr_t low = (uintptr_t)A | (uintptr_t)SB | (uintptr_t)C | (uintptr_t)Other | (uintptr_t)Bias;
+    if ((low & 15) == 0 && N <= kInt8MaxN)
+        return int8_gemm_run(dtype, A, SA, B, SB, C, Other, Bias, M, N, K, postop, out_f32, ws, ws_bytes, (hipStream_t)stream);
     return int8_plain_run(dtype, A, SA, B, SB, C, Other, Bias, M, N, K, postop, out_f32, (hipStream_t)stream);
 }
 
