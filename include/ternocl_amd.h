@@ -534,9 +534,9 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
  * X, R: DT [M, K] with ldx, ldr >= K elements from row to row.  W: [K] of wtype
  * (TERNOCL_FP16, _BF16 or _FP32; NULL: a weight of 1, woff not read); woff: 0, or 1 for
  * weights kept about zero; eps > 0.  Sums and norms are 64-bit; H and Y are rounded to
- * fp32, then to DT.  1 <= M <= 2^23, K >= 1.  Rows of 8-element multiples up to K = 32768
- * whose pointers and pitches are multiples of 16 bytes (Q: 8) take a kernel that reads
- * each element once, others a slower one.  No output overlaps another tensor but H as said. */
+ * fp32, then to DT.  1 <= M <= 2^23, K >= 1.  Rows of up to 32768 are read once (fastest
+ * where pointers, pitches and rows are multiples of 16 bytes; Q: 8), longer ones twice.
+ * No output overlaps another tensor but H as said. */
 ternocl_status ternocl_rmsnorm(int dtype, const void *X, int64_t ldx, const void *R, int64_t ldr, int wtype, const void *W,
                                float woff, float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K,
                                void *stream);
