@@ -3,6 +3,9 @@
 // straight into matrix-core fragments.
 #include "int8_epi.hpp"
 
+#include <algorithm>
+#include <cmath>
+
 namespace tcl {
 hipError_t int8_tile_run(int tile, int dtype, const I8Args &a, hipStream_t st);  // int8_gemm_tile.hip
 namespace {
@@ -207,26 +210,76 @@ template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream
 
 // ---- host side: the choice of tile and K slices ------------------------------------
 
+// A launch's time in us, by tile.  With w = tiles x slices / 256 workgroups a CU (part of them in
+// whole rounds), s = stages of 128 rows of K a slice and 10^6 weights and outputs:
+//   walk    = (s + edge) (one + two min(w - 1, 1) + more (w - 2)) for w above 1 and 2, `one`
+//             times 1 + far where the weights come from HBM and not the last-level cache, and
+//             times 1 + rows (M - 1) / 8 for activations loaded as fragments
+//   memory  = weights / in + 2 outputs / out
+//   time    = base + (walk^4 + memory^4)^(1/4), with slices + arrive + each slices + sums slices
+//             outputs
+// Fitted (logarithms, least squares, one fit a tile) to 300000 graph-timed calls on three sets of
+// operands, M = 1..4096, K = 256..14336, N = 64..151680: rms 5 to 10%; the tile chosen by it is 1.9%
+// behind the fastest of all on average (95 of 100 within 11%, one at worst 85%: a call of 4 us).
+// Narrow tiles fill the chip; wide ones read the activations, low ones the weights fewer times.
+enum I8Kind { kFew, kRows, kTile };  // activations as fragments (M <= 8), through a wave's LDS, int8_gemm_tile.hip
 struct I8Choice {
     int bm, bn;
-    bool tile;  // int8_gemm_tile.hip's, by its number
+    I8Kind kind;
     int num;
+    struct {
+        double base, one, two, more, in, whole, arrive, sums, each, edge, out, far, rows;
+    } t;
 };
-constexpr I8Choice kI8[] = {{16, 16, false, 0}, {16, 32, false, 1}, {16, 64, false, 2}, {32, 64, true, 5}, {64, 64, true, 4},
-                            {64, 128, true, 3}, {64, 256, true, 2}, {128, 256, true, 1}, {128, 512, true, 0}};
+constexpr I8Choice kI8[] = {
+    {16, 16, kFew, 0, {2.85, 0.0373, 0.0706, 0.072, 7.4, 1, 0.545, 4.12, 0.312, 3.68, 0.145, 0.351, 0.809}},
+    {16, 32, kFew, 1, {2.83, 0.067, 0.136, 0.151, 6.88, 1, 0.655, 4.47, 0.308, 0.624, 0.463, 0, 0.415}},
+    {16, 64, kFew, 2, {2.7, 0.149, 0.221, 0.337, 6.48, 1, 0.717, 6.01, 0.322, 0.701, 0.323, 0.0728, 0.119}},
+    {16, 16, kRows, 3, {2.83, 0.0645, 0.0694, 0.0886, 7.08, 0.856, 0.627, 3.75, 0.321, 1.08, 0.445, 0, 0}},
+    {16, 32, kRows, 4, {2.93, 0.082, 0.15, 0.161, 6.58, 0.843, 0.68, 3.72, 0.318, 0.324, 0.611, 0, 0}},
+    {32, 32, kRows, 5, {3.18, 0.0995, 0.182, 0.183, 6.83, 0.834, 0.684, 4.97, 0.316, 0.869, 0.678, 0, 0}},
+    {32, 64, kTile, 5, {3.14, 0.119, 0.143, 0.151, 5.55, 0.858, 0.659, 2.7, 0.337, 7.11, 0.793, 0.596, 0}},
+    {32, 128, kTile, 6, {3.35, 0.218, 0.212, 0.241, 6.41, 0.832, 0, 2.12, 1.13, 1.89, 2, 0.794, 0}},
+    {64, 64, kTile, 4, {2.63, 0.174, 0.247, 0.228, 5.32, 0.805, 0.426, 2.89, 0.621, 13.9, 0.635, 0.259, 0}},
+    {64, 128, kTile, 3, {4.48, 0.298, 0.311, 0.33, 6.51, 0.753, 0, 1.79, 2.01, 3.68, 2.78, 0.383, 0}},
+    {64, 128, kTile, 2, {3.12, 0.25, 0.409, 0.358, 6.38, 0.685, 0.541, 2.19, 1.04, 9.97, 0.971, 0.522, 0}},
+    {64, 256, kTile, 1, {4.53, 0.381, 0.63, 0.603, 6.21, 0.732, 0.922, 1.89, 2.01, 3.9, 2.13, 0.762, 0}},
+    {128, 512, kTile, 0, {7.77, 1.15, 2.37, 2, 5.46, 0.529, 0, 2.03, 7.49, 5.72, 1.79, 0.185, 0}}
+};
 
 struct I8Plan {
     int choice, ks;
 };
 
 I8Plan i8_plan(int M, int N, int K, size_t ws_bytes) {
-    auto tiles = [&](int i) { return (long)((M + kI8[i].bm - 1) / kI8[i].bm) * ((N + kI8[i].bn - 1) / kI8[i].bn); };
-    int c = M <= 16 ? 0 : 3;
-    const int last = M <= 16 ? 2 : 8;
-    while (c < last && tiles(c + 1) >= 200) ++c;
-    int ks = 1;
-    while (ks < 8 && tiles(c) * ks * 2 <= 512 && K / ks >= 4096 && kWsHeader + (size_t)ks * 2 * M * N * 4 <= ws_bytes) ks *= 2;
-    return {c, ks};
+    I8Plan best = {-1, 1};
+    double least = 1e30;
+    const double kn = 1e-6 * K * N, mn = 1e-6 * M * N, hbm = 1.0 / (1.0 + std::exp((85.0 - kn) / 10.0));
+    for (int i = 0; i < (int)(sizeof(kI8) / sizeof(kI8[0])); ++i) {
+        const I8Choice &c = kI8[i];
+        // (past those rows the fragments' loads, past 48 a tile's many row blocks are far behind; up to
+        // 16 rows a tile of 32 only where K is short)
+        if ((c.kind == kFew && M > 8) || (c.kind == kRows && M > (c.bm == 16 ? 48 : 96)) || (c.kind == kTile && M <= 16 && K > 1024) ||
+            (c.bm > 32 && c.bm >= 2 * M))
+            continue;
+        const long tiles = (long)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+        if (tiles > 8000000) continue;  // (a launch's threads: 32 bits)
+        for (int ks = 1; ks <= 8; ++ks) {
+            if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / 128 < 2 * ks || tiles * ks > 1024 || tiles > 300)) break;
+            const double w = tiles * ks / 256.0, r = c.t.whole * std::ceil(w) + (1.0 - c.t.whole) * w;
+            double one = c.t.one * (1.0 + c.t.far * hbm) * (1.0 + c.t.rows * (M - 1) / 8.0);
+            if (r > 1.0) one += c.t.two * std::min(r - 1.0, 1.0);
+            if (r > 2.0) one += c.t.more * (r - 2.0);
+            const double walk = ((K / 128 + ks - 1) / ks + c.t.edge) * one, mem = kn / c.t.in + 2.0 * mn / c.t.out;
+            double us = c.t.base + std::sqrt(std::sqrt(walk * walk * walk * walk + mem * mem * mem * mem));
+            if (ks > 1) us += c.t.arrive + c.t.each * ks + c.t.sums * ks * mn;
+            if (us < least) {
+                least = us;
+                best = {i, ks};
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -242,15 +295,21 @@ ternocl_status int8_gemm_run(int dtype, const int8_t *A, const float *SA, const 
                              const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32, void *ws,
                              size_t ws_bytes, hipStream_t st) {
     const I8Plan p = i8_plan(M, N, K, ws && ((uintptr_t)ws & 15) == 0 ? ws_bytes : 0);
+    if (p.choice < 0) {
+        set_error("M x N needs more tiles than a launch holds");
+        return TERNOCL_ERR_UNSUPPORTED_SHAPE;
+    }
     const I8Args a = {A, SA, B, SB, C, (const uint16_t *)Other, Bias, M, N, K, postop, out_f32, p.ks,
                       p.ks > 1 ? (int *)((uint8_t *)ws + kWsHeader) : nullptr, p.ks > 1 ? (uint64_t *)ws : nullptr};
     const I8Choice &c = kI8[p.choice];
-    if (c.tile) return launch_status(int8_tile_run(c.num, dtype, a, st));
-    const bool few = M <= 8;
+    if (c.kind == kTile) return launch_status(int8_tile_run(c.num, dtype, a, st));
     switch (c.num) {
-    case 0: return launch_status(few ? i8_kw_launch<I8Kw<16, 1, 1, 4, 4, 0>>(dtype, a, st) : i8_kw_launch<I8Kw<16, 1, 1, 4, 2, 2>>(dtype, a, st));
-    case 1: return launch_status(few ? i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 0>>(dtype, a, st) : i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 2>>(dtype, a, st));
-    default: return launch_status(few ? i8_kw_launch<I8Kw<16, 1, 4, 4, 1, 0>>(dtype, a, st) : i8_kw_launch<I8Kw<16, 1, 4, 4, 2, 2>>(dtype, a, st));
+    case 0: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 4, 0>>(dtype, a, st));
+    case 1: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 0>>(dtype, a, st));
+    case 2: return launch_status(i8_kw_launch<I8Kw<16, 1, 4, 4, 1, 0>>(dtype, a, st));
+    case 3: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 2, 2>>(dtype, a, st));
+    case 4: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 2>>(dtype, a, st));
+    default: return launch_status(i8_kw_launch<I8Kw<16, 2, 2, 4, 2, 2>>(dtype, a, st));
     }
 }
 

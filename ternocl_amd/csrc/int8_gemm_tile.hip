@@ -21,28 +21,26 @@ template <int MB_, int CB_, int WM_, int WN_, int WK_, int AD_, int PF_> struct 
     static_assert(LDS <= 160 * 1024, "a CU");
 };
 
-// Workgroup -> tile: XCD x (workgroups x, x + 8, ...) takes a contiguous range of the tiles
-// in panels of 8 row tiles, columns after columns, so that its 32 resident tiles are about 8
-// x 4 and share their rows and columns in its L2.
-__device__ __forceinline__ bool i8_tile_of(int id, int mt, int nt, int ksn, int &tm, int &tn, int &sl) {
-    const int total = mt * nt * ksn, per = (total + 7) / 8;
+// Workgroup -> tile: XCD x (workgroups x, x + 8, ...) takes a contiguous range of `total` parts
+// (`parts` a tile, from tile `first` on) in panels of up to `rows` row tiles (1024 rows),
+// columns after columns, so that its 32 resident tiles of 128 x 512 are about 8 x 4 and share
+// their rows and columns in its L2, and up to 1024 rows fetch the weights once.
+__device__ __forceinline__ bool i8_tile_of(int id, int first, int total, int mt, int nt, int rows, int parts, int &tm, int &tn, int &part) {
+    const int per = (total + 7) / 8;
     int t = (id & 7) * per + (id >> 3);
     if (t >= total || (id >> 3) >= per) return false;
-    sl = t % ksn;
-    t /= ksn;
-    const int panel = t / (8 * nt), r = t - panel * 8 * nt, pm = min(8, mt - 8 * panel);
+    part = t % parts;
+    t = first + t / parts;
+    const int panel = t / (rows * nt), r = t - panel * rows * nt, pm = min(rows, mt - rows * panel);
     tn = r / pm;
-    tm = 8 * panel + (r - tn * pm);
+    tm = rows * panel + (r - tn * pm);
     return true;
 }
 
-template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_tile(const I8Args a) {
+// The tile of rows m0 and columns n0 on, slice sl; cnt: its counter.
+template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Args &a, uint8_t *i8_lds, int m0, int n0, int sl, uint64_t *cnt) {
     constexpr int MB = T::MB, CB = T::CB, AP = T::AP, PF = T::PF, AD = T::AD;
-    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
-    const int mt = (a.M + T::BM - 1) / T::BM, nt = (a.N + T::BN - 1) / T::BN;
-    int tm, tn, sl;
-    if (!i8_tile_of(blockIdx.x, mt, nt, a.ksn, tm, tn, sl)) return;  // (whole workgroup)
-    const int m0 = tm * T::BM, n0 = tn * T::BN, mrows = min(T::BM, a.M - m0);
+    const int mrows = min(T::BM, a.M - m0);
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave / T::G, gw = wave % T::G, wm = gw / T::WN, wn = gw % T::WN;
     // this group's part of the slice's stages of 128 rows of K; all groups walk as many (`turns`)
@@ -183,7 +181,7 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
     __syncthreads();
     uint32_t *flag = (uint32_t *)i8_lds;
     if (wave == 0) {
-        const bool last = kw_arrive(a.cnt + 2 * ((size_t)tm * nt + tn), a.ksn, lane);
+        const bool last = kw_arrive(cnt, a.ksn, lane);
         if (lane == 0) *flag = last;
     }
     __syncthreads();
@@ -198,6 +196,29 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
     }
 }
 
+template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_tile(const I8Args a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
+    const int mt = (a.M + T::BM - 1) / T::BM, nt = (a.N + T::BN - 1) / T::BN;
+    int tm, tn, sl;
+    if (!i8_tile_of(blockIdx.x, 0, mt * nt * a.ksn, mt, nt, 1024 / T::BM, a.ksn, tm, tn, sl)) return;  // (whole workgroup)
+    i8_tile<T, BF16>(a, i8_lds, tm * T::BM, tn * T::BN, sl, a.ksn > 1 ? a.cnt + 2 * ((size_t)tm * nt + tn) : nullptr);
+}
+
+// The first `full` tiles as T's (a multiple of 256, a workgroup a CU), those of the last partial
+// round as two of H's each, half as wide: 4096 x 5120 x 34816 (8.5 rounds) (see below).
+template <class T, class H, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_tail(const I8Args a, int full) {
+    static_assert(H::BM == T::BM && 2 * H::BN == T::BN && H::THREADS == T::THREADS, "halves");
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
+    const int mt = (a.M + T::BM - 1) / T::BM, nt = (a.N + T::BN - 1) / T::BN;
+    int tm, tn, sl, id = blockIdx.x;
+    if (id < full) {
+        if (i8_tile_of(id, 0, full, mt, nt, 1024 / T::BM, 1, tm, tn, sl)) i8_tile<T, BF16>(a, i8_lds, tm * T::BM, tn * T::BN, 0, nullptr);
+    } else if (i8_tile_of(id - full, full, 2 * (mt * nt - full), mt, nt, 1024 / T::BM, 2, tm, tn, sl)) {
+        const int n0 = tn * T::BN + sl * H::BN;
+        if (n0 < a.N) i8_tile<H, BF16>(a, i8_lds, tm * T::BM, n0, 0, nullptr);
+    }
+}
+
 template <class T> hipError_t i8_tile_launch(int dtype, const I8Args &a, hipStream_t st) {
     const long tiles = (long)((a.M + T::BM - 1) / T::BM) * ((a.N + T::BN - 1) / T::BN) * a.ksn;
     const dim3 g((unsigned)(8 * ((tiles + 7) / 8)));
@@ -207,14 +228,30 @@ template <class T> hipError_t i8_tile_launch(int dtype, const I8Args &a, hipStre
     return hipGetLastError();
 }
 
+// 128 x 512 tiles, the last partial round of up to 128 as halves.
+hipError_t i8_wide_launch(int dtype, const I8Args &a, hipStream_t st) {
+    typedef I8Tile<4, 2, 1, 8, 1, 2, 4> T;
+    typedef I8Tile<4, 1, 1, 8, 1, 2, 4> H;
+    const long tiles = (long)((a.M + T::BM - 1) / T::BM) * ((a.N + T::BN - 1) / T::BN);
+    const int rem = (int)(tiles % 256);
+    if (a.ksn > 1 || tiles < 256 || rem == 0 || rem > 128) return i8_tile_launch<T>(dtype, a, st);
+    const int full = (int)(tiles - rem);
+    const dim3 g((unsigned)(full + 8 * ((2 * rem + 7) / 8)));
+    constexpr int lds = T::LDS > H::LDS ? T::LDS : H::LDS;
+    auto go = [&](auto k) { hipLaunchKernelGGL(k, g, dim3(T::THREADS), lds, st, a, full); };
+    if (dtype == TERNOCL_BF16) go(k_int8_gemm_tail<T, H, true>);
+    else go(k_int8_gemm_tail<T, H, false>);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t int8_tile_run(int tile, int dtype, const I8Args &a, hipStream_t st) {
     switch (tile) {
-    case 0: return i8_tile_launch<I8Tile<4, 2, 1, 8, 1, 2, 4>>(dtype, a, st);
-    case 1: return i8_tile_launch<I8Tile<4, 2, 1, 4, 1, 1, 4>>(dtype, a, st);
-    case 2: return i8_tile_launch<I8Tile<2, 1, 1, 8, 1, 4, 8>>(dtype, a, st);
-    case 3: return i8_tile_launch<I8Tile<2, 1, 1, 4, 2, 4, 8>>(dtype, a, st);
+    case 0: return i8_wide_launch(dtype, a, st);
+    case 1: return i8_tile_launch<I8Tile<2, 1, 1, 8, 1, 4, 8>>(dtype, a, st);
+    case 2: return i8_tile_launch<I8Tile<2, 1, 1, 4, 2, 4, 8>>(dtype, a, st);
+    case 3: return i8_tile_launch<I8Tile<2, 1, 1, 4, 1, 2, 8>>(dtype, a, st);
     case 4: return i8_tile_launch<I8Tile<2, 1, 1, 2, 4, 2, 8>>(dtype, a, st);
     case 5: return i8_tile_launch<I8Tile<1, 1, 1, 2, 4, 2, 8>>(dtype, a, st);
     default: return i8_tile_launch<I8Tile<1, 1, 1, 4, 1, 2, 8>>(dtype, a, st);
