@@ -167,37 +167,49 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
         m = R * mb + (l & (R - 1));
         n = n0 + R * cb + 8 * j + 4 * (l / R);
     };
-    for (int i = tid; i < T::ITEMS; i += T::THREADS) {
-        int m, n;
-        place(i, m, n);
-        if (m >= mrows || n >= a.N) continue;
+    auto sum = [&](int i) __attribute__((always_inline)) {
         i32x4_t s = red[i];
 #pragma unroll
         for (int w = 1; w < T::WK; ++w) s += red[w * T::ITEMS + i];
-        if (a.ksn > 1) i8_part_store(a.part + ((size_t)sl * a.M + m0 + m) * a.N + n, s);
-        else i8_store4<BF16>(a, m0 + m, n, s);
+        return s;
+    };
+    if (a.ksn > 1) {
+        for (int i = tid; i < T::ITEMS; i += T::THREADS) {
+            int m, n;
+            place(i, m, n);
+            if (m < mrows && n < a.N) i8_part_store(a.part + ((size_t)sl * a.M + m0 + m) * a.N + n, sum(i));
+        }
+        // the last of the tile's slices adds them
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        uint32_t *flag = (uint32_t *)i8_lds;
+        if (wave == 0) {
+            const bool last = kw_arrive(a.cnt + 2 * ((size_t)tm * nt + tn), a.ksn, lane);
+            if (lane == 0) *flag = last;
+        }
+        __syncthreads();
+        if (!*flag) return;
     }
-    if (a.ksn == 1) return;
-    // the last of the tile's slices adds them
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    uint32_t *flag = (uint32_t *)i8_lds;
-    if (wave == 0) {
-        const bool last = kw_arrive(a.cnt + 2 * ((size_t)tm * nt + tn), a.ksn, lane);
-        if (lane == 0) *flag = last;
-    }
-    __syncthreads();
-    if (!*flag) return;
-    for (int i = tid; i < T::ITEMS; i += T::THREADS) {
-        int m, n;
-        place(i, m, n);
-        if (m >= mrows || n >= a.N) continue;
-        const int *p = a.part + (size_t)(m0 + m) * a.N + n;
-        i32x4_t s = i8_part_load(p);
-        for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
-        i8_store4<BF16>(a, m0 + m, n, s);
-    }
+    epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
+        const I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> e(a);
+        for (int i = tid; i < T::ITEMS; i += T::THREADS) {
+            int m, n;
+            place(i, m, n);
+            if (m >= mrows || n >= a.N) continue;
+            const auto col = e.col(n);
+            const auto row = e.row(m0 + m, n);
+            i32x4_t s;
+            if (a.ksn > 1) {
+                const int *p = a.part + (size_t)(m0 + m) * a.N + n;
+                s = i8_part_load(p);
+                for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
+            } else {
+                s = sum(i);
+            }
+            e.store(m0 + m, n, s, col, row);
+        }
+    });
 }
 
 template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream_t st) {

@@ -140,41 +140,62 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
     __syncthreads();
     // 32 rows of a wave's sums at a time through LDS, so that a row's columns lie on adjacent
     // lanes; the groups' waves share the addition
-    constexpr int LPR = 8 * CB, RPI = 64 / LPR;  // lanes a row, rows a pass
+    constexpr int LPR = 8 * CB, RPI = 64 / LPR, NI = 32 / RPI / T::WK;  // lanes a row, rows a pass, passes a wave
+    static_assert(NI * RPI * T::WK == 32, "whole passes");
     int *red = (int *)i8_lds + gw * 32 * T::PITCH;
-    const int rr = lane / LPR, rc = 4 * (lane % LPR);
-    const bool split = a.ksn > 1;
+    const int rr = RPI * kg + lane / LPR, rc = 4 * (lane % LPR), n = nb + rc, nc = min(n, a.N - 4);
+    auto blocks = [&](auto emit) __attribute__((always_inline)) {  // emit(first row, its NI sums, RPI WK rows apart)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
+        for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+            for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *(i32x4_t *)(red + kg * T::G * 32 * T::PITCH + c * T::PITCH + 32 * cb + 8 * j + 4 * h) =
-                    i32x4_t{acc[mb][cb][4 * j], acc[mb][cb][4 * j + 1], acc[mb][cb][4 * j + 2], acc[mb][cb][4 * j + 3]};
-        if constexpr (T::WK > 1) {
-            __syncthreads();
-        } else {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-        for (int i = kg; i < 32 / RPI; i += T::WK) {
-            const int row = RPI * i + rr, m = (wm * MB + mb) * 32 + row, n = nb + rc;
-            i32x4_t s = *(const i32x4_t *)(red + row * T::PITCH + rc);
+                for (int j = 0; j < 4; ++j)
+                    *(i32x4_t *)(red + kg * T::G * 32 * T::PITCH + c * T::PITCH + 32 * cb + 8 * j + 4 * h) =
+                        i32x4_t{acc[mb][cb][4 * j], acc[mb][cb][4 * j + 1], acc[mb][cb][4 * j + 2], acc[mb][cb][4 * j + 3]};
+            if constexpr (T::WK > 1) {
+                __syncthreads();
+            } else {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+            i32x4_t s[NI];
 #pragma unroll
-            for (int k = 1; k < T::WK; ++k) s += *(const i32x4_t *)(red + (k * T::G * 32 + row) * T::PITCH + rc);
-            if (m < mrows && n < a.N) {
-                if (split) i8_part_store(a.part + ((size_t)sl * a.M + m0 + m) * a.N + n, s);
-                else i8_store4<BF16>(a, m0 + m, n, s);
+            for (int i = 0; i < NI; ++i) {
+                const int *p = red + (rr + RPI * T::WK * i) * T::PITCH + rc;
+                s[i] = *(const i32x4_t *)p;
+#pragma unroll
+                for (int k = 1; k < T::WK; ++k) s[i] += *(const i32x4_t *)(p + k * T::G * 32 * T::PITCH);
+            }
+            emit((wm * MB + mb) * 32 + rr, s);
+            if constexpr (T::WK > 1) {
+                if (mb < MB - 1) __syncthreads();
+            } else {
+                __builtin_amdgcn_wave_barrier();
             }
         }
-        if constexpr (T::WK > 1) {
-            if (mb < MB - 1) __syncthreads();
-        } else {
-            __builtin_amdgcn_wave_barrier();
-        }
+    };
+    if (a.ksn == 1) {
+        epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
+            typedef I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> E;
+            const E e(a);
+            const typename E::Col col = e.col(nc);
+            blocks([&](int m, const i32x4_t *s) __attribute__((always_inline)) {
+                typename E::Row row[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) row[i] = e.row(m0 + min(m + RPI * T::WK * i, mrows - 1), nc);
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    if (m + RPI * T::WK * i < mrows && n < a.N) e.store(m0 + m + RPI * T::WK * i, n, s[i], col, row[i]);
+            });
+        });
+        return;
     }
-    if (!split) return;
+    blocks([&](int m, const i32x4_t *s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (m + RPI * T::WK * i < mrows && n < a.N) i8_part_store(a.part + ((size_t)sl * a.M + m0 + m + RPI * T::WK * i) * a.N + n, s[i]);
+    });
     // the last of the tile's slices adds them
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_waitcnt(0);
@@ -186,14 +207,19 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
     }
     __syncthreads();
     if (!*flag) return;
-    for (int i = tid; i < mrows * (T::BN / 4); i += T::THREADS) {
-        const int m = m0 + i / (T::BN / 4), n = n0 + 4 * (i % (T::BN / 4));
-        if (n >= a.N) continue;
-        const int *p = a.part + (size_t)m * a.N + n;
-        i32x4_t s = i8_part_load(p);
-        for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
-        i8_store4<BF16>(a, m, n, s);
-    }
+    epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
+        const I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> e(a);
+        for (int i = tid; i < mrows * (T::BN / 4); i += T::THREADS) {
+            const int m = m0 + i / (T::BN / 4), nn = n0 + 4 * (i % (T::BN / 4));
+            if (nn >= a.N) continue;
+            const auto col = e.col(nn);
+            const auto row = e.row(m, nn);
+            const int *p = a.part + (size_t)m * a.N + nn;
+            i32x4_t s = i8_part_load(p);
+            for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
+            e.store(m, nn, s, col, row);
+        }
+    });
 }
 
 template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_tile(const I8Args a) {
