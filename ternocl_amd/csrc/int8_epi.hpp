@@ -27,46 +27,51 @@ typedef int i32x16_t __attribute__((ext_vector_type(16)));
 // activations (2^120 at bf16), and the channel's has brought the sum down before it.
 __device__ __forceinline__ float i8_scaled(int acc, float sb, float sa) { return ((float)acc * sb) * sa; }
 
+typedef uint32_t i8_u32x2_t __attribute__((ext_vector_type(2)));
+typedef float i8_f32x4_t __attribute__((ext_vector_type(4)));
+
 // The epilogue of outputs (m, n .. n + 3), n % 4 == 0, in two parts, so that a lane's loads are in
-// flight together: what it reads, then the output.
-template <bool BF16, int P, bool F32> struct I8Epi {
-    typedef uint32_t U2 __attribute__((ext_vector_type(2)));
-    typedef float F4 __attribute__((ext_vector_type(4)));
-    const I8Args &a;
-    __device__ __forceinline__ I8Epi(const I8Args &a_) : a(a_) {}
-    struct Col {
-        F4 sb, bias;
-    };
-    struct Row {
-        float sa;
-        U2 other;
-    };
-    static __device__ __forceinline__ F4 four(U2 t) {
-        return F4{dt2f<BF16>(t[0] & 0xffffu), dt2f<BF16>(t[0] >> 16), dt2f<BF16>(t[1] & 0xffffu), dt2f<BF16>(t[1] >> 16)};
-    }
-    __device__ __forceinline__ Col col(int n) const {
-        Col c;
-        c.sb = *(const F4 *)(a.SB + n);
-        if constexpr (postop_needs_bias(P)) c.bias = F32 ? *(const F4 *)((const float *)a.Bias + n) : four(*(const U2 *)((const uint16_t *)a.Bias + n));
-        return c;
-    }
-    __device__ __forceinline__ Row row(int m, int n) const {
-        Row r;
-        r.sa = a.SA[m];
-        if constexpr (postop_needs_other(P)) r.other = *(const U2 *)(a.Other + (size_t)m * a.N + n);
-        return r;
-    }
-    __device__ __forceinline__ void store(int m, int n, i32x4_t s, const Col &c, const Row &r) const {
-        F4 o = {}, b = {}, v;
-        if constexpr (postop_needs_other(P)) o = four(r.other);
-        if constexpr (postop_needs_bias(P)) b = c.bias;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = epi_apply_c<P>(i8_scaled(s[i], c.sb[i], r.sa), o[i], b[i]);
-        const size_t at = (size_t)m * a.N + n;
-        if constexpr (F32) *(F4 *)((float *)a.C + at) = v;
-        else *(U2 *)((uint16_t *)a.C + at) = U2{f2dt<BF16>(v[0]) | (f2dt<BF16>(v[1]) << 16), f2dt<BF16>(v[2]) | (f2dt<BF16>(v[3]) << 16)};
-    }
+// flight together, or while the products run: what it reads, as it is stored, then the output.
+struct I8Col {
+    i8_f32x4_t sb, bias;  // (bias: fp32, or DT pairs in the first two)
 };
+struct I8Row {
+    float sa;
+    i8_u32x2_t other;
+};
+__device__ __forceinline__ I8Col i8_col(const I8Args &a, int n) {
+    I8Col c;
+    c.sb = *(const i8_f32x4_t *)(a.SB + n);
+    if (postop_needs_bias(a.postop)) {
+        if (a.out_f32) {
+            c.bias = *(const i8_f32x4_t *)((const float *)a.Bias + n);
+        } else {
+            const i8_u32x2_t t = *(const i8_u32x2_t *)((const uint16_t *)a.Bias + n);
+            c.bias = i8_f32x4_t{__uint_as_float(t[0]), __uint_as_float(t[1]), 0.0f, 0.0f};
+        }
+    }
+    return c;
+}
+__device__ __forceinline__ I8Row i8_row(const I8Args &a, int m, int n) {
+    I8Row r;
+    r.sa = a.SA[m];
+    if (postop_needs_other(a.postop)) r.other = *(const i8_u32x2_t *)(a.Other + (size_t)m * a.N + n);
+    return r;
+}
+template <bool BF16, int P, bool F32>
+__device__ __forceinline__ void i8_out(const I8Args &a, int m, int n, i32x4_t s, const I8Col &c, const I8Row &r) {
+    auto four = [](uint32_t x, uint32_t y) __attribute__((always_inline)) {
+        return i8_f32x4_t{dt2f<BF16>(x & 0xffffu), dt2f<BF16>(x >> 16), dt2f<BF16>(y & 0xffffu), dt2f<BF16>(y >> 16)};
+    };
+    i8_f32x4_t o = {}, b = {}, v;
+    if constexpr (postop_needs_other(P)) o = four(r.other[0], r.other[1]);
+    if constexpr (postop_needs_bias(P)) b = F32 ? c.bias : four(__float_as_uint(c.bias[0]), __float_as_uint(c.bias[1]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = epi_apply_c<P>(i8_scaled(s[i], c.sb[i], r.sa), o[i], b[i]);
+    const size_t at = (size_t)m * a.N + n;
+    if constexpr (F32) *(i8_f32x4_t *)((float *)a.C + at) = v;
+    else *(i8_u32x2_t *)((uint16_t *)a.C + at) = i8_u32x2_t{f2dt<BF16>(v[0]) | (f2dt<BF16>(v[1]) << 16), f2dt<BF16>(v[2]) | (f2dt<BF16>(v[3]) << 16)};
+}
 
 // Four sums to and from the workspace, past the XCD's own L2.
 __device__ __forceinline__ void i8_part_store(int *p, i32x4_t s) {

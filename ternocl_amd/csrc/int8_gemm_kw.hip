@@ -22,6 +22,7 @@ template <int R_, int MB_, int CB_, int WK_, int PF_, int AD_> struct I8Kw {
     static constexpr int ITEMS = MB * CB * Q * 64, SUMS = WK * ITEMS * 16, ABUF = AD ? WK * 2 * BM * 128 : 0;
     static constexpr int LDS = SUMS > ABUF ? SUMS : ABUF;
     static_assert(AD == 0 || (PF % AD == 0 && PF % 2 == 0), "slots by the unrolled walk");
+    static_assert(ITEMS <= THREADS, "four outputs a thread at most");
 };
 
 // Workgroup -> tile: XCD x (workgroups x, x + 8, ...) takes a contiguous range of them, the
@@ -97,6 +98,16 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
 #pragma unroll
         for (int i = 0; i < AL; ++i) *(i32x4_t *)(aw + buf * T::BM * 128 + 1024 * i) = av[p][i];
     };
+    // this thread's outputs (m, n .. n + 3); what their epilogue reads is on its way while the
+    // products run
+    const int il = tid & 63, ib = tid >> 6, m = m0 + R * (ib / Q / CB) + (il & (R - 1)), n = n0 + R * (ib / Q % CB) + 8 * (ib % Q) + 4 * (il / R);
+    const bool mine = tid < T::ITEMS && m < m0 + mrows && n < a.N;
+    I8Col col;
+    I8Row row;
+    if (mine) {
+        col = i8_col(a, n);
+        row = i8_row(a, m, n);
+    }
     Acc acc[MB][CB];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
@@ -162,22 +173,12 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
                 red[wave * T::ITEMS + ((mb * CB + cb) * Q + j) * 64 + lane] =
                     i32x4_t{acc[mb][cb][4 * j], acc[mb][cb][4 * j + 1], acc[mb][cb][4 * j + 2], acc[mb][cb][4 * j + 3]};
     __syncthreads();
-    auto place = [&](int i, int &m, int &n) __attribute__((always_inline)) {
-        const int l = i & 63, b = i >> 6, j = b % Q, cb = b / Q % CB, mb = b / Q / CB;
-        m = R * mb + (l & (R - 1));
-        n = n0 + R * cb + 8 * j + 4 * (l / R);
-    };
-    auto sum = [&](int i) __attribute__((always_inline)) {
-        i32x4_t s = red[i];
-#pragma unroll
-        for (int w = 1; w < T::WK; ++w) s += red[w * T::ITEMS + i];
-        return s;
-    };
     if (a.ksn > 1) {
-        for (int i = tid; i < T::ITEMS; i += T::THREADS) {
-            int m, n;
-            place(i, m, n);
-            if (m < mrows && n < a.N) i8_part_store(a.part + ((size_t)sl * a.M + m0 + m) * a.N + n, sum(i));
+        if (mine) {
+            i32x4_t s = red[tid];
+#pragma unroll
+            for (int w = 1; w < T::WK; ++w) s += red[w * T::ITEMS + tid];
+            i8_part_store(a.part + ((size_t)sl * a.M + m) * a.N + n, s);
         }
         // the last of the tile's slices adds them
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -191,24 +192,19 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
         __syncthreads();
         if (!*flag) return;
     }
+    if (!mine) return;
+    i32x4_t s;
+    if (a.ksn > 1) {
+        const int *p = a.part + (size_t)m * a.N + n;
+        s = i8_part_load(p);
+        for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
+    } else {
+        s = red[tid];
+#pragma unroll
+        for (int w = 1; w < T::WK; ++w) s += red[w * T::ITEMS + tid];
+    }
     epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
-        const I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> e(a);
-        for (int i = tid; i < T::ITEMS; i += T::THREADS) {
-            int m, n;
-            place(i, m, n);
-            if (m >= mrows || n >= a.N) continue;
-            const auto col = e.col(n);
-            const auto row = e.row(m0 + m, n);
-            i32x4_t s;
-            if (a.ksn > 1) {
-                const int *p = a.part + (size_t)(m0 + m) * a.N + n;
-                s = i8_part_load(p);
-                for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
-            } else {
-                s = sum(i);
-            }
-            e.store(m0 + m, n, s, col, row);
-        }
+        i8_out<BF16, decltype(P_)::value, decltype(F_)::value>(a, m, n, s, col, row);
     });
 }
 

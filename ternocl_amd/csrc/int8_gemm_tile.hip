@@ -84,6 +84,21 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) bf[slot][cb] = *(const i32x4_t *)(p + vb[cb]);
     };
+    // the epilogue takes 32 rows of a wave's sums at a time through LDS, so that a row's columns lie
+    // on adjacent lanes; the groups' waves share the addition
+    constexpr int LPR = 8 * CB, RPI = 64 / LPR, NI = 32 / RPI / T::WK;  // lanes a row, rows a pass, passes a wave
+    static_assert(NI * RPI * T::WK == 32, "whole passes");
+    int *red = (int *)i8_lds + gw * 32 * T::PITCH;
+    const int rr = RPI * kg + lane / LPR, rc = 4 * (lane % LPR), n = nb + rc, nc = min(n, a.N - 4);
+    // (few outputs a lane: what the epilogue reads is on its way while the products run)
+    constexpr bool EARLY = MB == 1 && NI <= 2;
+    I8Col col;
+    I8Row row[NI];
+    if (EARLY && a.ksn == 1) {
+        col = i8_col(a, nc);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) row[i] = i8_row(a, m0 + min(32 * wm + rr + RPI * T::WK * i, mrows - 1), nc);
+    }
     i32x16_t acc[MB][CB];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
@@ -138,12 +153,6 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
         buf ^= 1;
     }
     __syncthreads();
-    // 32 rows of a wave's sums at a time through LDS, so that a row's columns lie on adjacent
-    // lanes; the groups' waves share the addition
-    constexpr int LPR = 8 * CB, RPI = 64 / LPR, NI = 32 / RPI / T::WK;  // lanes a row, rows a pass, passes a wave
-    static_assert(NI * RPI * T::WK == 32, "whole passes");
-    int *red = (int *)i8_lds + gw * 32 * T::PITCH;
-    const int rr = RPI * kg + lane / LPR, rc = 4 * (lane % LPR), n = nb + rc, nc = min(n, a.N - 4);
     auto blocks = [&](auto emit) __attribute__((always_inline)) {  // emit(first row, its NI sums, RPI WK rows apart)
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
@@ -176,17 +185,16 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
         }
     };
     if (a.ksn == 1) {
+        if constexpr (!EARLY) col = i8_col(a, nc);
         epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
-            typedef I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> E;
-            const E e(a);
-            const typename E::Col col = e.col(nc);
             blocks([&](int m, const i32x4_t *s) __attribute__((always_inline)) {
-                typename E::Row row[NI];
+                if constexpr (!EARLY)
 #pragma unroll
-                for (int i = 0; i < NI; ++i) row[i] = e.row(m0 + min(m + RPI * T::WK * i, mrows - 1), nc);
+                    for (int i = 0; i < NI; ++i) row[i] = i8_row(a, m0 + min(m + RPI * T::WK * i, mrows - 1), nc);
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    if (m + RPI * T::WK * i < mrows && n < a.N) e.store(m0 + m + RPI * T::WK * i, n, s[i], col, row[i]);
+                    if (m + RPI * T::WK * i < mrows && n < a.N)
+                        i8_out<BF16, decltype(P_)::value, decltype(F_)::value>(a, m0 + m + RPI * T::WK * i, n, s[i], col, row[i]);
             });
         });
         return;
@@ -208,16 +216,15 @@ template <class T, bool BF16> __device__ __forceinline__ void i8_tile(const I8Ar
     __syncthreads();
     if (!*flag) return;
     epi_dispatch(a.postop, a.out_f32, [&](auto P_, auto F_) __attribute__((always_inline)) {
-        const I8Epi<BF16, decltype(P_)::value, decltype(F_)::value> e(a);
         for (int i = tid; i < mrows * (T::BN / 4); i += T::THREADS) {
             const int m = m0 + i / (T::BN / 4), nn = n0 + 4 * (i % (T::BN / 4));
             if (nn >= a.N) continue;
-            const auto col = e.col(nn);
-            const auto row = e.row(m, nn);
+            const I8Col cl = i8_col(a, nn);
+            const I8Row rw = i8_row(a, m, nn);
             const int *p = a.part + (size_t)m * a.N + nn;
             i32x4_t s = i8_part_load(p);
             for (int k = 1; k < a.ksn; ++k) s += i8_part_load(p + (size_t)k * a.M * a.N);
-            e.store(m, nn, s, col, row);
+            i8_out<BF16, decltype(P_)::value, decltype(F_)::value>(a, m, nn, s, cl, rw);
         }
     });
 }
