@@ -11,17 +11,17 @@ hipError_t int8_tile_run(int tile, int dtype, const I8Args &a, hipStream_t st); 
 namespace {
 
 // R MB rows x R CB columns, R = 16 or 32 (the matrix instruction), WK waves over K, PF units
-// of 128 rows of K of weights in flight.  AD: 0 for activations loaded as fragments, else the
+// of U rows of K of weights in flight.  AD: 0 for activations loaded as fragments, else the
 // units of them in flight on their way through a wave's own LDS.
-template <int R_, int MB_, int CB_, int WK_, int PF_, int AD_> struct I8Kw {
-    static constexpr int R = R_, MB = MB_, CB = CB_, WK = WK_, PF = PF_, AD = AD_;
+template <int R_, int MB_, int CB_, int WK_, int PF_, int AD_, int U_ = 128> struct I8Kw {
+    static constexpr int R = R_, MB = MB_, CB = CB_, WK = WK_, PF = PF_, AD = AD_, U = U_;
     static constexpr int THREADS = 64 * WK, BM = R * MB, BN = R * CB;
-    static constexpr int S = R / 8;            // matrix instructions (16-byte loads) a unit and block
+    static constexpr int S = R * U / 1024;     // matrix instructions (16-byte loads) a unit and block
     static constexpr int Q = R == 16 ? 1 : 4;  // 4-column quads of a lane's outputs of a block
     static constexpr int AL = BM / 8;          // 16-byte loads of a unit's rows
     static constexpr int ITEMS = MB * CB * Q * 64, SUMS = WK * ITEMS * 16, ABUF = AD ? WK * 2 * BM * 128 : 0;
     static constexpr int LDS = SUMS > ABUF ? SUMS : ABUF;
-    static_assert(AD == 0 || (PF % AD == 0 && PF % 2 == 0), "slots by the unrolled walk");
+    static_assert(AD == 0 || (PF % AD == 0 && PF % 2 == 0 && U == 128), "slots by the unrolled walk");
     static_assert(ITEMS <= THREADS, "four outputs a thread at most");
 };
 
@@ -43,7 +43,8 @@ template <int R> struct I8Acc;
 template <> struct I8Acc<16> { typedef i32x4_t T; };
 template <> struct I8Acc<32> { typedef i32x16_t T; };
 
-template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_kw(const I8Args a) {
+// NT: weights loaded past the last-level cache.
+template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_kw(const I8Args a) {
     constexpr int R = T::R, MB = T::MB, CB = T::CB, PF = T::PF, S = T::S, Q = T::Q, AD = T::AD, AL = T::AL;
     typedef typename I8Acc<R>::T Acc;
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
@@ -53,10 +54,10 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
     const int m0 = tm * T::BM, n0 = tn * T::BN, mrows = min(T::BM, a.M - m0);
     const int tid = threadIdx.x, lane = tid & 63, c = lane & (R - 1), g = lane / R;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int units = a.K / 128, s0 = (int)((long)units * sl / a.ksn), s1 = (int)((long)units * (sl + 1) / a.ksn);
+    const int units = a.K / T::U, s0 = (int)((long)units * sl / a.ksn), s1 = (int)((long)units * (sl + 1) / a.ksn);
     const int u0 = s0 + (s1 - s0) * wave / T::WK, u1 = s0 + (s1 - s0) * (wave + 1) / T::WK;
-    // instruction s of a unit: lane (c, g) holds rows (128 / S) s + 16 g .. + 15 of K of its
-    // row and column
+    // instruction s of a unit: lane (c, g) holds rows (U / S) s + 16 g .. + 15 of K of its row
+    // and column
     const int8_t *Ab = a.A + (size_t)m0 * a.K;
     uint32_t va[AD ? AL : MB], vb[CB], ar[S];
     if constexpr (AD) {  // 8 rows of 128 bytes a load
@@ -70,7 +71,7 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
     }
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) vb[cb] = ((uint32_t)g * (uint32_t)a.N + (uint32_t)min(n0 + R * cb + c, a.N - 1)) * 16u;
-    const size_t bunit = (size_t)a.N * 128, bstep = bunit / S;
+    const size_t bunit = (size_t)a.N * T::U, bstep = bunit / S;
     i32x4_t bf[PF][S][CB], af[AD ? 1 : PF][S][MB], av[AD ? AD : 1][AL];
     uint8_t *ab = i8_lds + wave * 2 * T::BM * 128, *aw = ab + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
     // (past the end: read again, not multiplied)
@@ -80,13 +81,16 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) bf[p][s][cb] = __builtin_nontemporal_load((const i32x4_t *)(pb + s * bstep + vb[cb]));
+            for (int cb = 0; cb < CB; ++cb) {
+                const i32x4_t *w = (const i32x4_t *)(pb + s * bstep + vb[cb]);
+                bf[p][s][cb] = NT ? __builtin_nontemporal_load(w) : *w;
+            }
         if constexpr (!AD) {
-            const int8_t *pa = Ab + 128 * (size_t)uc;
+            const int8_t *pa = Ab + T::U * (size_t)uc;
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int mb = 0; mb < MB; ++mb) af[p][s][mb] = *(const i32x4_t *)(pa + s * (128 / S) + va[mb]);
+                for (int mb = 0; mb < MB; ++mb) af[p][s][mb] = *(const i32x4_t *)(pa + s * (T::U / S) + va[mb]);
         }
     };
     auto a_load = [&](int u, int p) __attribute__((always_inline)) {
@@ -208,11 +212,15 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
     });
 }
 
+// Weights of more than 100 MB, which the 256 MB cache cannot keep beside others, go past it: 1 x
+// 5120 x 34816 33.9 -> 31.8 us, 4 x 4096 x 151680 112 -> 104; smaller ones that are still there
+// from their last use are read faster: 24 x 14336 x 4096 15.7 -> 12.3 (from HBM 15.3 and 15.4).
 template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream_t st) {
     const long tiles = (long)((a.M + T::BM - 1) / T::BM) * ((a.N + T::BN - 1) / T::BN) * a.ksn;
+    const bool nt = (long)a.K * a.N > 100000000;
     auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3((unsigned)(8 * ((tiles + 7) / 8))), dim3(T::THREADS), T::LDS, st, a); };
-    if (dtype == TERNOCL_BF16) go(k_int8_gemm_kw<T, true>);
-    else go(k_int8_gemm_kw<T, false>);
+    if (dtype == TERNOCL_BF16) nt ? go(k_int8_gemm_kw<T, true, true>) : go(k_int8_gemm_kw<T, true, false>);
+    else nt ? go(k_int8_gemm_kw<T, false, true>) : go(k_int8_gemm_kw<T, false, false>);
     return hipGetLastError();
 }
 
@@ -226,9 +234,9 @@ template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream
 //   memory  = weights / in + 2 outputs / out
 //   time    = base + (walk^4 + memory^4)^(1/4), with slices + arrive + each slices + sums slices
 //             outputs
-// Fitted (logarithms, least squares, one fit a tile) to 300000 graph-timed calls on three sets of
-// operands, M = 1..4096, K = 256..14336, N = 64..151680: rms 5 to 10%; the tile chosen by it is 1.9%
-// behind the fastest of all on average (95 of 100 within 11%, one at worst 85%: a call of 4 us).
+// Fitted (logarithms, least squares, one fit a tile) to some 300000 graph-timed calls on three sets
+// of operands, 11630 shapes of M = 1..4096, K = 256..14336, N = 64..151680: rms 5 to 11%; the tile
+// chosen by it is 1.3% behind the fastest of 21 on average (95 of 100 within 8%, the worst 41%).
 // Narrow tiles fill the chip; wide ones read the activations, low ones the weights fewer times.
 enum I8Kind { kFew, kRows, kTile };  // activations as fragments (M <= 8), through a wave's LDS, int8_gemm_tile.hip
 struct I8Choice {
@@ -240,19 +248,20 @@ struct I8Choice {
     } t;
 };
 constexpr I8Choice kI8[] = {
-    {16, 16, kFew, 0, {2.85, 0.0373, 0.0706, 0.072, 7.4, 1, 0.545, 4.12, 0.312, 3.68, 0.145, 0.351, 0.809}},
-    {16, 32, kFew, 1, {2.83, 0.067, 0.136, 0.151, 6.88, 1, 0.655, 4.47, 0.308, 0.624, 0.463, 0, 0.415}},
-    {16, 64, kFew, 2, {2.7, 0.149, 0.221, 0.337, 6.48, 1, 0.717, 6.01, 0.322, 0.701, 0.323, 0.0728, 0.119}},
-    {16, 16, kRows, 3, {2.83, 0.0645, 0.0694, 0.0886, 7.08, 0.856, 0.627, 3.75, 0.321, 1.08, 0.445, 0, 0}},
-    {16, 32, kRows, 4, {2.93, 0.082, 0.15, 0.161, 6.58, 0.843, 0.68, 3.72, 0.318, 0.324, 0.611, 0, 0}},
-    {32, 32, kRows, 5, {3.18, 0.0995, 0.182, 0.183, 6.83, 0.834, 0.684, 4.97, 0.316, 0.869, 0.678, 0, 0}},
-    {32, 64, kTile, 5, {3.14, 0.119, 0.143, 0.151, 5.55, 0.858, 0.659, 2.7, 0.337, 7.11, 0.793, 0.596, 0}},
-    {32, 128, kTile, 6, {3.35, 0.218, 0.212, 0.241, 6.41, 0.832, 0, 2.12, 1.13, 1.89, 2, 0.794, 0}},
-    {64, 64, kTile, 4, {2.63, 0.174, 0.247, 0.228, 5.32, 0.805, 0.426, 2.89, 0.621, 13.9, 0.635, 0.259, 0}},
-    {64, 128, kTile, 3, {4.48, 0.298, 0.311, 0.33, 6.51, 0.753, 0, 1.79, 2.01, 3.68, 2.78, 0.383, 0}},
-    {64, 128, kTile, 2, {3.12, 0.25, 0.409, 0.358, 6.38, 0.685, 0.541, 2.19, 1.04, 9.97, 0.971, 0.522, 0}},
-    {64, 256, kTile, 1, {4.53, 0.381, 0.63, 0.603, 6.21, 0.732, 0.922, 1.89, 2.01, 3.9, 2.13, 0.762, 0}},
-    {128, 512, kTile, 0, {7.77, 1.15, 2.37, 2, 5.46, 0.529, 0, 2.03, 7.49, 5.72, 1.79, 0.185, 0}}
+    {16, 16, kFew, 0, {2.87, 0.0272, 0.0549, 0.0614, 6.74, 1, 0.483, 8.4, 0.303, 3.77, 0.222, 1.62, 0.99}},
+    {16, 32, kFew, 1, {2.99, 0.0443, 0.0996, 0.12, 6.99, 1, 0.545, 4.68, 0.303, 1.36, 1.17e+07, 1.07, 0.533}},
+    {16, 16, kRows, 2, {2.94, 0.0397, 0.0303, 0.0727, 6.56, 0.685, 0.478, 6.13, 0.32, 1.82, 0.916, 2.18, 0}},
+    {16, 32, kRows, 3, {3.07, 0.0511, 0.089, 0.143, 6.81, 0.674, 0.594, 4.26, 0.31, 0.795, 2.86, 1.81, 0}},
+    {16, 64, kRows, 4, {3.4, 0.0847, 0.191, 0.294, 6.81, 0.754, 0.793, 3.41, 0.313, 0.573, 2.56, 1.14, 0}},
+    {32, 32, kRows, 5, {3.4, 0.0692, 0.12, 0.173, 7.32, 0.77, 0.659, 4.84, 0.318, 0.489, 1.13, 0.916, 0}},
+    {32, 64, kTile, 0, {3.19, 0.113, 0.149, 0.151, 6.06, 0.91, 0.585, 2.58, 0.348, 6.78, 0.856, 0.867, 0}},
+    {32, 128, kTile, 1, {3.13, 0.228, 0.234, 0.245, 6.48, 0.748, 0.337, 1.79, 1.11, 1.74, 2.38, 0.729, 0}},
+    {32, 128, kTile, 2, {3.18, 0.187, 0.241, 0.244, 6.19, 0.858, 0.632, 2.07, 0.622, 3.95, 1.34, 0.971, 0}},
+    {64, 128, kTile, 3, {3.43, 0.328, 0.337, 0.334, 6.41, 0.739, 0, 1.53, 2.01, 3.12, 2.85, 0.283, 0}},
+    {64, 128, kTile, 4, {2.75, 0.261, 0.43, 0.365, 6.27, 0.733, 0.226, 2.2, 1.09, 8.37, 1.16, 0.437, 0}},
+    {64, 256, kTile, 5, {2.87, 0.377, 0.738, 0.616, 6.49, 0.735, 0.182, 2.61, 1.95, 5.53, 1.78, 0.718, 0}},
+    {128, 256, kTile, 6, {4.9, 0.782, 0.999, 0.969, 6.84, 0.719, 0, 1.47, 7.36, 3.76, 2.44, 0.144, 0}},
+    {128, 512, kTile, 7, {3.69, 1.14, 2.39, 1.72, 5.27, 0.462, 0, 2, 7.38, 4.53, 2.34, 0.178, 0}}
 };
 
 struct I8Plan {
@@ -273,7 +282,7 @@ I8Plan i8_plan(int M, int N, int K, size_t ws_bytes) {
         const long tiles = (long)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
         if (tiles > 8000000) continue;  // (a launch's threads: 32 bits)
         for (int ks = 1; ks <= 8; ++ks) {
-            if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / 128 < 2 * ks || tiles * ks > 1024 || tiles > 300)) break;
+            if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / 128 < 4 * ks || tiles * ks > 640 || tiles > 256)) break;
             const double w = tiles * ks / 256.0, r = c.t.whole * std::ceil(w) + (1.0 - c.t.whole) * w;
             double one = c.t.one * (1.0 + c.t.far * hbm) * (1.0 + c.t.rows * (M - 1) / 8.0);
             if (r > 1.0) one += c.t.two * std::min(r - 1.0, 1.0);
@@ -313,10 +322,10 @@ ternocl_status int8_gemm_run(int dtype, const int8_t *A, const float *SA, const 
     if (c.kind == kTile) return launch_status(int8_tile_run(c.num, dtype, a, st));
     switch (c.num) {
     case 0: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 4, 0>>(dtype, a, st));
-    case 1: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 0>>(dtype, a, st));
-    case 2: return launch_status(i8_kw_launch<I8Kw<16, 1, 4, 4, 1, 0>>(dtype, a, st));
-    case 3: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 2, 2>>(dtype, a, st));
-    case 4: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 2>>(dtype, a, st));
+    case 1: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 4, 0, 64>>(dtype, a, st));
+    case 2: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 2, 2>>(dtype, a, st));
+    case 3: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 2>>(dtype, a, st));
+    case 4: return launch_status(i8_kw_launch<I8Kw<16, 1, 4, 4, 2, 2>>(dtype, a, st));
     default: return launch_status(i8_kw_launch<I8Kw<16, 2, 2, 4, 2, 2>>(dtype, a, st));
     }
 }

@@ -281,13 +281,14 @@ hipError_t i8_wide_launch(int dtype, const I8Args &a, hipStream_t st) {
 
 hipError_t int8_tile_run(int tile, int dtype, const I8Args &a, hipStream_t st) {
     switch (tile) {
-    case 0: return i8_wide_launch(dtype, a, st);
-    case 1: return i8_tile_launch<I8Tile<2, 1, 1, 8, 1, 4, 8>>(dtype, a, st);
-    case 2: return i8_tile_launch<I8Tile<2, 1, 1, 4, 2, 4, 8>>(dtype, a, st);
+    case 0: return i8_tile_launch<I8Tile<1, 1, 1, 2, 4, 2, 8>>(dtype, a, st);
+    case 1: return i8_tile_launch<I8Tile<1, 1, 1, 4, 1, 2, 8>>(dtype, a, st);
+    case 2: return i8_tile_launch<I8Tile<1, 1, 1, 4, 2, 2, 8>>(dtype, a, st);
     case 3: return i8_tile_launch<I8Tile<2, 1, 1, 4, 1, 2, 8>>(dtype, a, st);
-    case 4: return i8_tile_launch<I8Tile<2, 1, 1, 2, 4, 2, 8>>(dtype, a, st);
-    case 5: return i8_tile_launch<I8Tile<1, 1, 1, 2, 4, 2, 8>>(dtype, a, st);
-    default: return i8_tile_launch<I8Tile<1, 1, 1, 4, 1, 2, 8>>(dtype, a, st);
+    case 4: return i8_tile_launch<I8Tile<2, 1, 1, 4, 2, 4, 8>>(dtype, a, st);
+    case 5: return i8_tile_launch<I8Tile<2, 1, 1, 8, 1, 4, 8>>(dtype, a, st);
+    case 6: return i8_tile_launch<I8Tile<4, 2, 1, 4, 1, 1, 4>>(dtype, a, st);
+    default: return i8_wide_launch(dtype, a, st);
     }
 }
 
