@@ -1,6 +1,23 @@
-// int8_gemm_kw.hip -- products of 8-bit integers for few rows (ternocl_int8_gemm): a
-// workgroup's waves split K, each streaming its part of the weights and the activations
-// straight into matrix-core fragments.
+// int8_gemm_kw.hip -- products of 8-bit integers with a scale for each token and channel
+// (ternocl_int8_gemm) for up to some tens of rows on gfx950, and the choice between the engines:
+//
+//   C[m,n] = ct(epi((sum_k A[m,k] B[k,n]) SB[n] SA[m])),  exact 32-bit sums
+//
+// Few rows are bound by the weights' stream (K N bytes; at 24 rows 48 operations a byte, a
+// hundredth of the matrix cores' rate).  So nothing stands between memory and the matrix cores:
+// 16 rows of a column lie together ([K/16][N][16]), so that a 16-byte load a lane is an operand
+// of v_mfma_i32_16x16x64_i8 (four runs of 256 bytes, wider strips longer ones), with no LDS, no
+// barrier and no instruction on the way.
+//   * A workgroup's waves split K and each streams its own part of a strip of columns, several
+//     units of 64 or 128 rows in flight; their sums meet once, in LDS.  Sums are whole numbers:
+//     the same bits whatever the split.
+//   * Columns are the instruction's rows: a lane ends with four adjacent outputs of a row, and
+//     loads what their epilogue reads before the walk.
+//   * Activations of up to 8 rows are loaded as fragments (lanes past the last row read its line
+//     again); of more, where a fragment load would touch a cache line a row, in whole lines
+//     through the wave's own LDS: 48 x 5120 x 5120 15.2 -> 11.4 us.
+// Back to back, bf16: 1 x 4096 x 4096 (16.8 MB) 4.4 us captured, 24 x 14336 x 4096 (58.7 MB) 11.2,
+// 4 x 4096 x 151680 (621 MB, fp32 out) 104 us, 6.0 TB/s.
 #include "int8_epi.hpp"
 
 #include <algorithm>

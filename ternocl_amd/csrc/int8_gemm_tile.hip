@@ -1,5 +1,26 @@
-// int8_gemm_tile.hip -- products of 8-bit integers for many rows (ternocl_int8_gemm) on
-// gfx950's int8 matrix cores.
+// int8_gemm_tile.hip -- products of 8-bit integers with a scale for each token and channel
+// (ternocl_int8_gemm) for tens to thousands of rows on gfx950's int8 matrix cores:
+//
+//   C[m,n] = ct(epi((sum_k A[m,k] B[k,n]) SB[n] SA[m])),  exact 32-bit sums
+//
+// A tile's waves share its rows of A through LDS, chunk j of a row at j ^ (row % 8) (8 lanes read 8
+// different rows without a conflict), and take the weights, each its own columns, straight into
+// fragments ([K/16][N][16]: 16 bytes a lane).  A stage is 128 rows of K: two LDS buffers, the next
+// stage stored in the middle of the current one, one barrier; one to four more stages of A are on
+// their way in registers (4096 x 5120 x 34816: one 720 us, two 698) and four to sixteen steps of
+// weights.
+//   * 128 x 512, eight waves side by side of 128 x 64: for each stage 2048 cycles of matrix
+//     instructions a SIMD, 1152 of LDS and 1280 of L1 a CU.  256 x 256 as four waves of 128 x 128
+//     840 us where this took 782, as eight waves 787.  What bounds it is the matrix cores at the
+//     clock that power leaves: 2.1 to 2.3 10^15 operations a second by box (4096 x 5120 x 34816
+//     642 to 697 us; the library's int8 product 730, its 8192^3 one 2.13 10^15).
+//   * Small tiles of tens to hundreds of rows are as long as their stages' latency (loads, LDS,
+//     barrier: some 0.4 us): groups of waves split K, each with its own buffers, and add their sums
+//     through LDS once (128 x 4096 x 4096 11.3 -> 8.4 us; what the epilogue reads loaded during the
+//     walk 8.1).
+//   * The epilogue: 32 rows of a wave's sums through LDS, so that 8 CB lanes have a row's adjacent
+//     columns; the switch of its kind once a wave and the rows' loads together (4096 x 5120 x 34816 670
+//     -> 642 us, 1024 x 4096 x 14336 with silu(acc) * other 92 -> 64).
 #include "int8_epi.hpp"
 
 namespace tcl {
@@ -238,7 +259,7 @@ template <class T, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_in
 }
 
 // The first `full` tiles as T's (a multiple of 256, a workgroup a CU), those of the last partial
-// round as two of H's each, half as wide: 4096 x 5120 x 34816 (8.5 rounds) (see below).
+// round as two of H's each, half as wide: 4096 x 5120 x 34816 (8.5 rounds) 702 -> 670 us.
 template <class T, class H, bool BF16> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_tail(const I8Args a, int full) {
     static_assert(H::BM == T::BM && 2 * H::BN == T::BN && H::THREADS == T::THREADS, "halves");
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];

@@ -305,3 +305,86 @@ def test_norm_before_ternary_product(dev):
     sa, aq = o.quant_a(y)
     assert torch.equal(q, aq) and torch.equal(s[:, :M], sa[:, :M])
     assert torch.equal(o.int2_int8_gemm(q, s, B, S, None, None, 0, False), o.int2_int8_gemm(aq, sa, B, S, None, None, 0, False))
+
+
+@pytest.mark.parametrize("M,K,N,postop", [(1152, 1024, 14480, 5), (2300, 1024, 7376, 0), (2560, 1024, 6784, 1), (1024, 1024, 16848, 0)])
+def test_last_round_in_halves(dev, M, K, N, postop):
+    """A little more than 256 tiles of 128 x 512: those past the last whole round run as two of half the width, of a
+    last column of tiles that ends inside the first half too."""
+    import ternocl_amd as T
+    check(T, M, M, K, N, True, postop, False)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 14336, 64), (5, 14336, 512), (9, 8192, 64), (24, 14336, 512), (60, 8192, 64), (64, 14336, 2048),
+                                   (100, 4096, 64), (100, 14336, 512), (130, 14336, 2048), (300, 14336, 2048), (1000, 8192, 96)])
+@pytest.mark.parametrize("postop", [0, 5])
+def test_k_slices(dev, M, K, N, postop):
+    """Shapes that split K over workgroups with a workspace, at every tile that does: whole, short and no workspace, any
+    contents, the same bits."""
+    import ternocl_amd as T
+    nb = T.int8_gemm_ws_bytes(M, N, K)
+    assert nb > T.WS_HEADER_BYTES
+    A, SA, W, SB = make(M + N, M, K, N)
+    g = torch.Generator().manual_seed(M)
+    o = torch.randn((M, N), generator=g).half() if postop else None
+    b = torch.randn(N, generator=g).half() if postop else None
+    want = run(T, A, SA, W, SB, torch.float16, o, b, postop, False, ws=None)
+    if postop == 0:
+        assert torch.equal(want.cpu(), ((exact_sums(A, W).float() * SB) * SA[:, None]).half())
+    B, C = packed(W.cuda()), torch.empty((M, N), dtype=torch.float16, device="cuda")
+    a = [t if t is None else t.cuda() for t in (A, SA, SB, o, b)]
+    for n in (nb, nb - 4, T.WS_HEADER_BYTES + 8 * M * N, T.WS_HEADER_BYTES):
+        ws = torch.full((n + 16,), 0x5a, dtype=torch.uint8, device="cuda")
+        for _ in range(2):  # (as left by another use, then as the first call leaves it)
+            C.zero_()
+            T.int8_gemm(a[0], a[1], B, a[2], C, a[3], a[4], M, N, K, postop, False, ws=ws[:n])
+            torch.cuda.synchronize()
+            assert torch.equal(C, want)
+            assert (ws[n:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 512, 256), (6, 14336, 512), (20, 1024, 256), (70, 512, 512), (300, 256, 1024), (1152, 1024, 14480)])
+def test_residual_in_place(dev, M, K, N):
+    """C over Other: each output is read and written by one lane."""
+    import ternocl_amd as T
+    A, SA, W, SB = make(M, M, K, N)
+    o = torch.randn((M, N), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    a = (A.cuda(), SA.cuda(), packed(W.cuda()), SB.cuda())
+    nb = T.int8_gemm_ws_bytes(M, N, K)
+    for ws in (None, torch.zeros(nb, dtype=torch.uint8, device="cuda")) if nb else (None,):
+        C = torch.empty_like(o)
+        T.int8_gemm(*a, C, o, None, M, N, K, 2, False, ws=ws)
+        D = o.clone()
+        T.int8_gemm(*a, D, D, None, M, N, K, 2, False, ws=ws)
+        assert torch.equal(C, D)
+
+
+def test_captured_layer(dev):
+    """A captured MLP with its norm, replayed on new inputs with eager work between, equals eager calls."""
+    import ternocl_amd.torch_ops  # noqa: F401
+    o = torch.ops.ternocl
+    M, H, I = 5, 1024, 2048
+    g = torch.Generator("cuda").manual_seed(4)
+    r = lambda *s: torch.randn(s, device="cuda", generator=g)
+    x, res, w = r(M, H).bfloat16(), r(M, H).bfloat16(), torch.rand(H, device="cuda", generator=g)
+    Ws = [packed((r(*s) * 40).round().clamp(-127, 127).to(torch.int8)) for s in ((H, I), (H, I), (I, H))]
+    Ss = [torch.rand(n, device="cuda", generator=g) * 1e-3 for n in (I, I, H)]
+
+    def layer():
+        h, y, q, s = o.rmsnorm(x, res, w, 1e-6, 0.0, "rows", True)
+        up = o.int8_gemm(q, s, Ws[0], Ss[0], torch.bfloat16, None, None, 0, False)
+        act = o.int8_gemm(q, s, Ws[1], Ss[1], torch.bfloat16, up, None, 1, False)
+        q2, s2 = o.quant_rows(act)
+        return h, y, q, s, act, o.int8_gemm(q2, s2, Ws[2], Ss[2], torch.bfloat16, h, None, 2, False)
+
+    layer()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    for i in range(4):
+        x.copy_(r(M, H))
+        res.copy_(r(M, H))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, layer()))
