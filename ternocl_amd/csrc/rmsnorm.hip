@@ -29,6 +29,7 @@ struct NormArgs {
     int8_t *Q;
     void *SQ;
     int M, K;
+    int m0;  // a launch's first row
 };
 
 constexpr double kTie = 0.5 - 0x1p-30;  // past this a product with 127 / top may be on the wrong side of a half
@@ -68,7 +69,7 @@ constexpr int kAnyWaves = 4;
 constexpr int kShort = 256;  // threads of a workgroup of short rows
 template <bool BF16, bool NORM> __global__ void __launch_bounds__(64 * kAnyWaves) k_rows_any(const NormArgs a) {
     __shared__ RowStat red[kAnyWaves];
-    const int m = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, K = a.K;
+    const int m = a.m0 + blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, K = a.K;
     const uint16_t *x = a.X + (size_t)m * a.ldx, *r = a.R ? a.R + (size_t)m * a.ldr : nullptr;
     auto h_of = [&](int k) __attribute__((always_inline)) {
         const double h = dt2f<BF16>(x[k]);
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(L < 64 ? kShort : 1024) k_rows_vec(const NormA
     __shared__ double red[16][2];
     __shared__ uint32_t redbad[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m = L < 64 ? blockIdx.x * (kShort / L) + threadIdx.x / L : blockIdx.x, tid = L < 64 ? threadIdx.x % L : threadIdx.x;
+    const int m = a.m0 + (L < 64 ? blockIdx.x * (kShort / L) + threadIdx.x / L : blockIdx.x), tid = L < 64 ? threadIdx.x % L : threadIdx.x;
     const int nt = blockDim.x, nw = nt >> 6, vecs = (a.K + 7) >> 3;
     auto len = [&](int v) __attribute__((always_inline)) { return AL ? 8 : min(8, a.K - 8 * v); };
     if (L < 64 && m >= a.M) return;  // (a row's lanes leave together, and moves stay among them)
@@ -352,11 +353,12 @@ __global__ void __launch_bounds__(L < 64 ? kShort : 1024) k_rows_vec(const NormA
     }
 }
 
-template <bool NORM> ternocl_status rows_run(int dtype, const NormArgs &a, hipStream_t st) {
+// Rows a.m0 .. a.m0 + rows - 1.
+template <bool NORM> ternocl_status rows_launch(int dtype, const NormArgs &a, int rows, hipStream_t st) {
     const bool bf = dtype == TERNOCL_BF16;
     if (a.K > 32768) {
-        if (bf) hipLaunchKernelGGL((k_rows_any<true, NORM>), dim3(a.M), dim3(64 * kAnyWaves), 0, st, a);
-        else hipLaunchKernelGGL((k_rows_any<false, NORM>), dim3(a.M), dim3(64 * kAnyWaves), 0, st, a);
+        if (bf) hipLaunchKernelGGL((k_rows_any<true, NORM>), dim3(rows), dim3(64 * kAnyWaves), 0, st, a);
+        else hipLaunchKernelGGL((k_rows_any<false, NORM>), dim3(rows), dim3(64 * kAnyWaves), 0, st, a);
         return check_launch();
     }
     const uintptr_t low = (uintptr_t)a.X | (uintptr_t)a.R | (uintptr_t)a.W | (uintptr_t)a.H | (uintptr_t)a.Y | (uintptr_t)(2 * a.K) |
@@ -370,7 +372,7 @@ template <bool NORM> ternocl_status rows_run(int dtype, const NormArgs &a, hipSt
     if (vecs <= 32) {
         auto go = [&](auto l) {
             constexpr int L = decltype(l)::value;
-            const dim3 g((a.M + kShort / L - 1) / (kShort / L));
+            const dim3 g((rows + kShort / L - 1) / (kShort / L));
             pick([&](auto b, auto w) {
                 hipLaunchKernelGGL((k_rows_vec<decltype(b)::value, NORM, decltype(w)::value, 1, L>), g, dim3(kShort), 0, st, a, 1.0 / a.K);
             });
@@ -389,7 +391,7 @@ template <bool NORM> ternocl_status rows_run(int dtype, const NormArgs &a, hipSt
     const int nt = ((vecs + c - 1) / c + 63) / 64 * 64;
     auto go = [&](auto n) {
         pick([&](auto b, auto w) {
-            hipLaunchKernelGGL((k_rows_vec<decltype(b)::value, NORM, decltype(w)::value, decltype(n)::value>), dim3(a.M), dim3(nt), 0, st,
+            hipLaunchKernelGGL((k_rows_vec<decltype(b)::value, NORM, decltype(w)::value, decltype(n)::value>), dim3(rows), dim3(nt), 0, st,
                                a, 1.0 / a.K);
         });
     };
@@ -399,16 +401,26 @@ template <bool NORM> ternocl_status rows_run(int dtype, const NormArgs &a, hipSt
     return check_launch();
 }
 
+// (a launch holds 2^32 threads: 2^21 rows of up to 1024 at a time)
+template <bool NORM> ternocl_status rows_run(int dtype, NormArgs a, hipStream_t st) {
+    constexpr int step = 1 << 21;
+    for (a.m0 = 0; a.m0 < a.M; a.m0 += step) {
+        const ternocl_status s = rows_launch<NORM>(dtype, a, a.M - a.m0 < step ? a.M - a.m0 : step, st);
+        if (s != TERNOCL_OK) return s;
+    }
+    return TERNOCL_OK;
+}
+
 }  // namespace
 
 ternocl_status rmsnorm_run(int dtype, const void *X, long ldx, const void *R, long ldr, int wtype, const void *W, float woff,
                            float eps, void *H, void *Y, int quant, int8_t *Q, void *SQ, int M, int K, hipStream_t st) {
     return rows_run<true>(dtype, {(const uint16_t *)X, (const uint16_t *)R, ldx, ldr, wtype, W, woff, eps, (uint16_t *)H,
-                                  (uint16_t *)Y, quant, Q, SQ, M, K}, st);
+                                  (uint16_t *)Y, quant, Q, SQ, M, K, 0}, st);
 }
 
 ternocl_status quant_rows_run(int dtype, const void *X, long ldx, int8_t *Q, float *SQ, int M, int K, hipStream_t st) {
-    return rows_run<false>(dtype, {(const uint16_t *)X, nullptr, ldx, 0, 0, nullptr, 0.0f, 0.0f, nullptr, nullptr, 1, Q, SQ, M, K}, st);
+    return rows_run<false>(dtype, {(const uint16_t *)X, nullptr, ldx, 0, 0, nullptr, 0.0f, 0.0f, nullptr, nullptr, 1, Q, SQ, M, K, 0}, st);
 }
 
 }  // namespace tcl

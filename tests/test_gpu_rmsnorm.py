@@ -304,3 +304,28 @@ def test_streams_and_graph(dev):
             want = run(T, X, R, W, dt, "rows", True)
         st.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("K", [64, 77, 264])
+def test_many_rows(dev, K):
+    """More rows than one launch holds."""
+    import ternocl_amd as T
+    M = (1 << 21) + 3
+    X = torch.randn((M, K), device="cuda", dtype=torch.bfloat16)
+    Q, SQ = torch.full((M + 1, K), 7, dtype=torch.int8, device="cuda"), torch.full((M + 1,), 7.0, device="cuda")
+    Y, H = torch.empty_like(X), torch.empty_like(X)
+    for norm in (False, True):
+        if norm:
+            T.rmsnorm(X, X, None, H, Y, Q, SQ, M, K, quant="rows")
+        else:
+            T.quant_rows(X, Q, SQ, M, K)
+        torch.cuda.synchronize()
+        assert (Q[M] == 7).all() and SQ[M] == 7
+        for i in (0, (1 << 21) - 2, M - 4):
+            x = X[i:i + 4].double().cpu()
+            assert torch.equal(Q[i:i + 4].cpu(), codes_of(x)[0])  # (x + x scales by a power of two: the same codes)
+            if norm:
+                h, t, s = gold(X[i:i + 4], X[i:i + 4], None, 0.0)
+                assert torch.equal(H[i:i + 4].cpu(), h.float().bfloat16()) and near(Y[i:i + 4].cpu(), t * s, torch.bfloat16)
+    want = codes_of(X[::1001].double().cpu())[0]
+    assert torch.equal(Q[:M][::1001].cpu(), want)
