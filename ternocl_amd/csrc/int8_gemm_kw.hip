@@ -16,8 +16,8 @@
 //   * Activations of up to 8 rows are loaded as fragments (lanes past the last row read its line
 //     again); of more, where a fragment load would touch a cache line a row, in whole lines
 //     through the wave's own LDS: 48 x 5120 x 5120 15.2 -> 11.4 us.
-// Back to back, bf16: 1 x 4096 x 4096 (16.8 MB) 4.4 us captured, 24 x 14336 x 4096 (58.7 MB) 11.2,
-// 4 x 4096 x 151680 (621 MB, fp32 out) 104 us, 6.0 TB/s.
+// Captured, bf16, by box: 1 x 4096 x 4096 (16.8 MB) 4.4 to 5.1 us, 24 x 14336 x 4096 (58.7 MB, residual)
+// 11.2 to 11.5, 4 x 4096 x 151680 (621 MB, fp32 out) 104 to 111: 5.6 to 5.9 TB/s.
 #include "int8_epi.hpp"
 
 #include <algorithm>
@@ -27,16 +27,15 @@ namespace tcl {
 hipError_t int8_tile_run(int tile, int dtype, const I8Args &a, hipStream_t st);  // int8_gemm_tile.hip
 namespace {
 
-// R MB rows x R CB columns, R = 16 or 32 (the matrix instruction), WK waves over K, PF units
-// of U rows of K of weights in flight.  AD: 0 for activations loaded as fragments, else the
-// units of them in flight on their way through a wave's own LDS.
-template <int R_, int MB_, int CB_, int WK_, int PF_, int AD_, int U_ = 128> struct I8Kw {
-    static constexpr int R = R_, MB = MB_, CB = CB_, WK = WK_, PF = PF_, AD = AD_, U = U_;
+// 16 MB rows x 16 CB columns, WK waves over K, PF units of U rows of K of weights in flight.
+// AD: 0 for activations loaded as fragments, else the units of them in flight on their way
+// through a wave's own LDS.
+template <int MB_, int CB_, int WK_, int PF_, int AD_, int U_ = 128> struct I8Kw {
+    static constexpr int R = 16, MB = MB_, CB = CB_, WK = WK_, PF = PF_, AD = AD_, U = U_;
     static constexpr int THREADS = 64 * WK, BM = R * MB, BN = R * CB;
-    static constexpr int S = R * U / 1024;     // matrix instructions (16-byte loads) a unit and block
-    static constexpr int Q = R == 16 ? 1 : 4;  // 4-column quads of a lane's outputs of a block
-    static constexpr int AL = BM / 8;          // 16-byte loads of a unit's rows
-    static constexpr int ITEMS = MB * CB * Q * 64, SUMS = WK * ITEMS * 16, ABUF = AD ? WK * 2 * BM * 128 : 0;
+    static constexpr int S = U / 64;   // matrix instructions (16-byte loads) a unit and block
+    static constexpr int AL = BM / 8;  // 16-byte loads of a unit's rows
+    static constexpr int ITEMS = MB * CB * 64, SUMS = WK * ITEMS * 16, ABUF = AD ? WK * 2 * BM * 128 : 0;
     static constexpr int LDS = SUMS > ABUF ? SUMS : ABUF;
     static_assert(AD == 0 || (PF % AD == 0 && PF % 2 == 0 && U == 128), "slots by the unrolled walk");
     static_assert(ITEMS <= THREADS, "four outputs a thread at most");
@@ -56,14 +55,9 @@ __device__ __forceinline__ bool i8_kw_tile_of(int id, int mt, int nt, int ksn, i
     return true;
 }
 
-template <int R> struct I8Acc;
-template <> struct I8Acc<16> { typedef i32x4_t T; };
-template <> struct I8Acc<32> { typedef i32x16_t T; };
-
 // NT: weights loaded past the last-level cache.
 template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THREADS) k_int8_gemm_kw(const I8Args a) {
-    constexpr int R = T::R, MB = T::MB, CB = T::CB, PF = T::PF, S = T::S, Q = T::Q, AD = T::AD, AL = T::AL;
-    typedef typename I8Acc<R>::T Acc;
+    constexpr int R = T::R, MB = T::MB, CB = T::CB, PF = T::PF, S = T::S, AD = T::AD, AL = T::AL;
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
     const int mt = (a.M + T::BM - 1) / T::BM, nt = (a.N + T::BN - 1) / T::BN;
     int tm, tn, sl;
@@ -121,7 +115,7 @@ template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THRE
     };
     // this thread's outputs (m, n .. n + 3); what their epilogue reads is on its way while the
     // products run
-    const int il = tid & 63, ib = tid >> 6, m = m0 + R * (ib / Q / CB) + (il & (R - 1)), n = n0 + R * (ib / Q % CB) + 8 * (ib % Q) + 4 * (il / R);
+    const int il = tid & 63, ib = tid >> 6, m = m0 + R * (ib / CB) + (il & (R - 1)), n = n0 + R * (ib % CB) + 4 * (il / R);
     const bool mine = tid < T::ITEMS && m < m0 + mrows && n < a.N;
     I8Col col;
     I8Row row;
@@ -129,11 +123,11 @@ template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THRE
         col = i8_col(a, n);
         row = i8_row(a, m, n);
     }
-    Acc acc[MB][CB];
+    i32x4_t acc[MB][CB];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) acc[mb][cb] = Acc{};
+        for (int cb = 0; cb < CB; ++cb) acc[mb][cb] = i32x4_t{};
     // unit u in slot p: its rows lie in LDS buffer p % 2
     auto unit = [&](int u, int p, bool more) __attribute__((always_inline)) {
         if constexpr (AD) {
@@ -149,12 +143,8 @@ template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THRE
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                for (int mb = 0; mb < MB; ++mb) {  // (columns as the matrix' rows: a lane gets four adjacent ones)
-                    if constexpr (R == 16)
-                        acc[mb][cb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[p][s][cb], f[mb], acc[mb][cb], 0, 0, 0);
-                    else
-                        acc[mb][cb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[p][s][cb], f[mb], acc[mb][cb], 0, 0, 0);
-                }
+                for (int mb = 0; mb < MB; ++mb)  // (columns as the matrix' rows: a lane gets four adjacent ones)
+                    acc[mb][cb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[p][s][cb], f[mb], acc[mb][cb], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (more) b_load(u + PF, p);
@@ -189,10 +179,7 @@ template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THRE
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-            for (int j = 0; j < Q; ++j)
-                red[wave * T::ITEMS + ((mb * CB + cb) * Q + j) * 64 + lane] =
-                    i32x4_t{acc[mb][cb][4 * j], acc[mb][cb][4 * j + 1], acc[mb][cb][4 * j + 2], acc[mb][cb][4 * j + 3]};
+            red[wave * T::ITEMS + (mb * CB + cb) * 64 + lane] = acc[mb][cb];
     __syncthreads();
     if (a.ksn > 1) {
         if (mine) {
@@ -338,12 +325,12 @@ ternocl_status int8_gemm_run(int dtype, const int8_t *A, const float *SA, const 
     const I8Choice &c = kI8[p.choice];
     if (c.kind == kTile) return launch_status(int8_tile_run(c.num, dtype, a, st));
     switch (c.num) {
-    case 0: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 4, 0>>(dtype, a, st));
-    case 1: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 4, 0, 64>>(dtype, a, st));
-    case 2: return launch_status(i8_kw_launch<I8Kw<16, 1, 1, 4, 2, 2>>(dtype, a, st));
-    case 3: return launch_status(i8_kw_launch<I8Kw<16, 1, 2, 4, 2, 2>>(dtype, a, st));
-    case 4: return launch_status(i8_kw_launch<I8Kw<16, 1, 4, 4, 2, 2>>(dtype, a, st));
-    default: return launch_status(i8_kw_launch<I8Kw<16, 2, 2, 4, 2, 2>>(dtype, a, st));
+    case 0: return launch_status(i8_kw_launch<I8Kw<1, 1, 4, 4, 0>>(dtype, a, st));
+    case 1: return launch_status(i8_kw_launch<I8Kw<1, 2, 4, 4, 0, 64>>(dtype, a, st));
+    case 2: return launch_status(i8_kw_launch<I8Kw<1, 1, 4, 2, 2>>(dtype, a, st));
+    case 3: return launch_status(i8_kw_launch<I8Kw<1, 2, 4, 2, 2>>(dtype, a, st));
+    case 4: return launch_status(i8_kw_launch<I8Kw<1, 4, 4, 2, 2>>(dtype, a, st));
+    default: return launch_status(i8_kw_launch<I8Kw<2, 2, 4, 2, 2>>(dtype, a, st));
     }
 }
 
