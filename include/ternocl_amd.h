@@ -147,12 +147,14 @@ ternocl_status ternocl_int2_fp16_upcvt_gemm_ex(int dtype, const void *A, const u
  * 0: another engine), and its tile.  entry: 0 ternocl_int2_fp16_upcvt_gemm with
  * ws_bytes of workspace (0: none), 1 ternocl_int2_int8_gemm_ws, 2
  * ternocl_bitcos_fp16_upcvt_gemm_mt, 3 one product of M assignments over E
- * experts in ternocl_int2_moe_gemm / _prefill. */
+ * experts in ternocl_int2_moe_gemm / _prefill, 4 ternocl_int8_gemm with ws_bytes of
+ * workspace (1 for every tile, those of one wave over K too). */
 typedef struct {
     int rows, cols; /* output tile of a workgroup */
     int k_waves;    /* waves over K */
     int k_slices;   /* workgroups over K (> 1: sums in the workspace) */
-    int repacked;   /* entry 2: with a workspace the weights are re-packed first */
+    int repacked;   /* entry 2: with a workspace the weights are re-packed first; entry 4:
+                     * the activations pass through LDS */
 } ternocl_kw_tile;
 int ternocl_kw_tile_of(int entry, int M, int N, int K, int E, size_t ws_bytes, ternocl_kw_tile *tile);
 

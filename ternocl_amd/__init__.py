@@ -135,7 +135,8 @@ def int2_gemm_ws_bytes(M: int, N: int, K: int) -> int:
 
 def kw_tile_of(entry: int, M: int, N: int, K: int, E: int = 0, ws_bytes: int = 0):
     """(rows, cols, K waves, K slices, repacked) of the K-over-waves tile that a call takes, None where
-    another engine runs it (test hook; entry 0 int2, 1 s8 x s2, 2 M-tiled BITCOS, 3 MoE)."""
+    another engine runs it (test hook; entry 0 int2, 1 s8 x s2, 2 M-tiled BITCOS, 3 MoE, 4 int8: any tile, and
+    in place of repacked whether activations pass through LDS)."""
     t = _abi.KwTile()
     if not lib().ternocl_kw_tile_of(entry, M, N, K, E, ws_bytes, ctypes.byref(t)):
         return None

@@ -154,6 +154,7 @@ ternocl_status rmsnorm_run(int dtype, const void *X, long ldx, const void *R, lo
 ternocl_status quant_rows_run(int dtype, const void *X, long ldx, int8_t *Q, float *SQ, int M, int K, hipStream_t st);
 // kernels (int8_gemm_kw.hip, int8_gemm_tile.hip)
 size_t int8_gemm_ws_need(int M, int N, int K);
+bool int8_gemm_tile(int M, int N, int K, size_t ws_bytes, ternocl_kw_tile &t);
 ternocl_status int8_gemm_run(int dtype, const int8_t *A, const float *SA, const int8_t *B, const float *SB, void *C,
                              const void *Other, const void *Bias, int M, int N, int K, int postop, int out_f32, void *ws,
                              size_t ws_bytes, hipStream_t st);
@@ -258,6 +259,7 @@ int ternocl_kw_tile_of(int entry, int M, int N, int K, int E, size_t ws_bytes, t
     else if (ok && entry == 1) kw = int2_int8_kw_tile(M, N, K, ws_bytes, t);
     else if (ok && entry == 2) kw = bitcos_kw_tile(M, N, K, t);
     else if (ok && entry == 3 && E >= 1) kw = moe_kw_tile_of(M, E, N, K, t);
+    else if (ok && entry == 4 && K <= kInt8MaxK && N <= kInt8MaxN) kw = int8_gemm_tile(M, N, K, ws_bytes, t);
     if (tile) *tile = t;
     return kw ? 1 : 0;
 }

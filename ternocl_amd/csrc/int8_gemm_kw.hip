@@ -244,7 +244,7 @@ template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream
 // Narrow tiles fill the chip; wide ones read the activations, low ones the weights fewer times.
 enum I8Kind { kFew, kRows, kTile };  // activations as fragments (M <= 8), through a wave's LDS, int8_gemm_tile.hip
 struct I8Choice {
-    int bm, bn;
+    int bm, bn, wk;  // rows, columns, waves (kTile: groups of them) over K
     I8Kind kind;
     int num;
     struct {
@@ -252,20 +252,20 @@ struct I8Choice {
     } t;
 };
 constexpr I8Choice kI8[] = {
-    {16, 16, kFew, 0, {2.87, 0.0272, 0.0549, 0.0614, 6.74, 1, 0.483, 8.4, 0.303, 3.77, 0.222, 1.62, 0.99}},
-    {16, 32, kFew, 1, {2.99, 0.0443, 0.0996, 0.12, 6.99, 1, 0.545, 4.68, 0.303, 1.36, 1.17e+07, 1.07, 0.533}},
-    {16, 16, kRows, 2, {2.94, 0.0397, 0.0303, 0.0727, 6.56, 0.685, 0.478, 6.13, 0.32, 1.82, 0.916, 2.18, 0}},
-    {16, 32, kRows, 3, {3.07, 0.0511, 0.089, 0.143, 6.81, 0.674, 0.594, 4.26, 0.31, 0.795, 2.86, 1.81, 0}},
-    {16, 64, kRows, 4, {3.4, 0.0847, 0.191, 0.294, 6.81, 0.754, 0.793, 3.41, 0.313, 0.573, 2.56, 1.14, 0}},
-    {32, 32, kRows, 5, {3.4, 0.0692, 0.12, 0.173, 7.32, 0.77, 0.659, 4.84, 0.318, 0.489, 1.13, 0.916, 0}},
-    {32, 64, kTile, 0, {3.19, 0.113, 0.149, 0.151, 6.06, 0.91, 0.585, 2.58, 0.348, 6.78, 0.856, 0.867, 0}},
-    {32, 128, kTile, 1, {3.13, 0.228, 0.234, 0.245, 6.48, 0.748, 0.337, 1.79, 1.11, 1.74, 2.38, 0.729, 0}},
-    {32, 128, kTile, 2, {3.18, 0.187, 0.241, 0.244, 6.19, 0.858, 0.632, 2.07, 0.622, 3.95, 1.34, 0.971, 0}},
-    {64, 128, kTile, 3, {3.43, 0.328, 0.337, 0.334, 6.41, 0.739, 0, 1.53, 2.01, 3.12, 2.85, 0.283, 0}},
-    {64, 128, kTile, 4, {2.75, 0.261, 0.43, 0.365, 6.27, 0.733, 0.226, 2.2, 1.09, 8.37, 1.16, 0.437, 0}},
-    {64, 256, kTile, 5, {2.87, 0.377, 0.738, 0.616, 6.49, 0.735, 0.182, 2.61, 1.95, 5.53, 1.78, 0.718, 0}},
-    {128, 256, kTile, 6, {4.9, 0.782, 0.999, 0.969, 6.84, 0.719, 0, 1.47, 7.36, 3.76, 2.44, 0.144, 0}},
-    {128, 512, kTile, 7, {3.69, 1.14, 2.39, 1.72, 5.27, 0.462, 0, 2, 7.38, 4.53, 2.34, 0.178, 0}}
+    {16, 16, 4, kFew, 0, {2.87, 0.0272, 0.0549, 0.0614, 6.74, 1, 0.483, 8.4, 0.303, 3.77, 0.222, 1.62, 0.99}},
+    {16, 32, 4, kFew, 1, {2.99, 0.0443, 0.0996, 0.12, 6.99, 1, 0.545, 4.68, 0.303, 1.36, 1.17e+07, 1.07, 0.533}},
+    {16, 16, 4, kRows, 2, {2.94, 0.0397, 0.0303, 0.0727, 6.56, 0.685, 0.478, 6.13, 0.32, 1.82, 0.916, 2.18, 0}},
+    {16, 32, 4, kRows, 3, {3.07, 0.0511, 0.089, 0.143, 6.81, 0.674, 0.594, 4.26, 0.31, 0.795, 2.86, 1.81, 0}},
+    {16, 64, 4, kRows, 4, {3.4, 0.0847, 0.191, 0.294, 6.81, 0.754, 0.793, 3.41, 0.313, 0.573, 2.56, 1.14, 0}},
+    {32, 32, 4, kRows, 5, {3.4, 0.0692, 0.12, 0.173, 7.32, 0.77, 0.659, 4.84, 0.318, 0.489, 1.13, 0.916, 0}},
+    {32, 64, 4, kTile, 0, {3.19, 0.113, 0.149, 0.151, 6.06, 0.91, 0.585, 2.58, 0.348, 6.78, 0.856, 0.867, 0}},
+    {32, 128, 1, kTile, 1, {3.13, 0.228, 0.234, 0.245, 6.48, 0.748, 0.337, 1.79, 1.11, 1.74, 2.38, 0.729, 0}},
+    {32, 128, 2, kTile, 2, {3.18, 0.187, 0.241, 0.244, 6.19, 0.858, 0.632, 2.07, 0.622, 3.95, 1.34, 0.971, 0}},
+    {64, 128, 1, kTile, 3, {3.43, 0.328, 0.337, 0.334, 6.41, 0.739, 0, 1.53, 2.01, 3.12, 2.85, 0.283, 0}},
+    {64, 128, 2, kTile, 4, {2.75, 0.261, 0.43, 0.365, 6.27, 0.733, 0.226, 2.2, 1.09, 8.37, 1.16, 0.437, 0}},
+    {64, 256, 1, kTile, 5, {2.87, 0.377, 0.738, 0.616, 6.49, 0.735, 0.182, 2.61, 1.95, 5.53, 1.78, 0.718, 0}},
+    {128, 256, 1, kTile, 6, {4.9, 0.782, 0.999, 0.969, 6.84, 0.719, 0, 1.47, 7.36, 3.76, 2.44, 0.144, 0}},
+    {128, 512, 1, kTile, 7, {3.69, 1.14, 2.39, 1.72, 5.27, 0.462, 0, 2, 7.38, 4.53, 2.34, 0.178, 0}}
 };
 
 struct I8Plan {
@@ -309,6 +309,15 @@ I8Plan i8_plan(int M, int N, int K, size_t ws_bytes) {
 size_t int8_gemm_ws_need(int M, int N, int K) {
     const int ks = i8_plan(M, N, K, ~(size_t)0).ks;
     return ks == 1 ? 0 : kWsHeader + (size_t)ks * M * N * 4;
+}
+
+// The tile of a call on aligned operands, for ternocl_kw_tile_of.
+bool int8_gemm_tile(int M, int N, int K, size_t ws_bytes, ternocl_kw_tile &t) {
+    const I8Plan p = i8_plan(M, N, K, ws_bytes);
+    if (p.choice < 0) return false;
+    const I8Choice &c = kI8[p.choice];
+    t = {c.bm, c.bn, c.wk, p.ks, c.kind != kFew};
+    return true;
 }
 
 // (operands 16-byte aligned)
