@@ -555,8 +555,9 @@ ternocl_status ternocl_quant_rows(int dtype, const void *X, int64_t ldx, int8_t 
  * Sums are exact (any int8 values, -128 too), rounded once to fp32, multiplied by SB[n],
  * then by SA[m].  A scale of NaN makes its row's or column's products NaN.
  * dtype: DT of Other, of C and Bias without out_f32.
- * N % 16 == 0, K % 128 == 0, K < 2^17, any M >= 1.  B starts on 16 bytes; operands that are
- * not all 16-byte aligned run a plain kernel (several times slower).
+ * N % 16 == 0, N <= 2^30 - 64, K % 128 == 0, K < 2^17, M >= 1 (up to 10^9: a launch holds 8 million
+ * tiles of up to 128 x 512, and more are refused).  B starts on 16 bytes; operands that are not all
+ * 16-byte aligned, and N > 2^26, run a plain kernel (several times slower).
  * ws / ws_bytes: optional device scratch of ternocl_int8_gemm_ws_bytes(M, N, K) bytes (0:
  * none used), 16-byte aligned, laid out and used as ternocl_int2_fp16_upcvt_gemm's: a K
  * split of few tiles over a long K (the same bits as without).  Its counters take any

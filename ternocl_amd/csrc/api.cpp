@@ -225,6 +225,7 @@ static ternocl_status check_gemm_common(int dtype, const void *A, const void *B,
 
 constexpr int kInt8MaxK = (1 << 17) - 128;  // 2^14 K below 2^31
 constexpr int kInt8MaxN = 1 << 26;          // 4 blocks of 16 rows of K in 32-bit offsets
+constexpr int kInt8PlainMaxN = (1 << 30) - 64;  // a launch's 2^32 threads, 4 a column
 
 extern "C" {
 
@@ -789,6 +790,7 @@ ternocl_status ternocl_int8_gemm(int dtype, const int8_t *A, const float *SA, co
     if (s != TERNOCL_OK) return s;
     if (!SA) FAIL(TERNOCL_ERR_INVALID_ARG, "SA must be non-null");
     if (K > kInt8MaxK) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "K must be below 2^17 (sums of 32 bits)");
+    if (N > kInt8PlainMaxN) FAIL(TERNOCL_ERR_UNSUPPORTED_SHAPE, "N must be at most 2^30 - 64");
     if ((uintptr_t)B & 15) FAIL(TERNOCL_ERR_INVALID_ARG, "B must be 16-byte aligned");
     if (((uintptr_t)SA | (uintptr_t)SB) & 3) FAIL(TERNOCL_ERR_INVALID_ARG, "SA and SB must be aligned to their elements");
     const uintptr_t low = (uintptr_t)A | (uintptr_t)SB | (uintptr_t)C | (uintptr_t)Other | (uintptr_t)Bias;

@@ -283,7 +283,7 @@ I8Plan i8_plan(int M, int N, int K, size_t ws_bytes) {
         if ((c.kind == kFew && M > 8) || (c.kind == kRows && M > (c.bm == 16 ? 48 : 96)) || (c.kind == kTile && M <= 16 && K > 1024) ||
             (c.bm > 32 && c.bm >= 2 * M))
             continue;
-        const long tiles = (long)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+        const long tiles = (((long)M + c.bm - 1) / c.bm) * (((long)N + c.bn - 1) / c.bn);
         if (tiles > 8000000) continue;  // (a launch's threads: 32 bits)
         for (int ks = 1; ks <= 8; ++ks) {
             if (ks > 1 && (kWsHeader + (size_t)ks * M * N * 4 > ws_bytes || K / 128 < 4 * ks || tiles * ks > 640 || tiles > 256)) break;

@@ -151,3 +151,13 @@ def test_fake_refusals(call):
     import ternocl_amd.torch_ops  # noqa: F401
     with pytest.raises(Exception):
         call(torch.ops.ternocl)
+
+
+@pytest.mark.parametrize("M,N", [((1 << 30) + 200, 16), ((1 << 31) - 1, 16), ((1 << 31) - 128, 16), (1 << 20, 1 << 20), (1, 1 << 30),
+                                 (1, (1 << 31) - 16), ((1 << 31) - 1, (1 << 31) - 16)])
+def test_int8_gemm_past_a_launch(M, N):
+    """Refused as a shape before any device call, and no tile or workspace named for it."""
+    L = T.lib()
+    assert L.ternocl_int8_gemm(0, 4096, 4096, 4096, 4096, 4096, None, None, M, N, 128, 0, 0, None, 0, None) == SHAPE
+    assert L.ternocl_last_error().decode()
+    assert T.kw_tile_of(4, M, N, 128) is None and T.int8_gemm_ws_bytes(M, N, 128) == 0
