@@ -376,7 +376,7 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _chk_norm(x, residual, weight, quant) -> None:
+def _chk_norm(x, residual, weight, quant, norm) -> None:
     _chk_rows(x, "x")
     torch._check(x.dtype in _DT, lambda: f"x: dtype {x.dtype}, expected float16 or bfloat16")
     torch._check(x.shape[1] >= 1, lambda: "x must have columns")
@@ -386,6 +386,7 @@ def _chk_norm(x, residual, weight, quant) -> None:
                      lambda: "residual must have x's dtype, shape and device")
     _chk(weight, "weight", _LT, (x.shape[1],), x.device)
     torch._check(quant in T._QUANTS, lambda: "quant must be 'none', 'rows' or 'groups'")
+    torch._check(norm or quant != "none", lambda: "nothing to compute: norm is false and quant 'none'")
     torch._check(quant != "groups" or x.shape[1] % 128 == 0, lambda: "groups: x must have a multiple of 128 columns")
 
 
@@ -407,8 +408,7 @@ def rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[
             quant: str, norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(h, y, q, scales) of x [M, K]: h = x + residual, y = rmsnorm(h) * (woff + weight) where norm asks for it, its
     codes q int8 [M, K] and scales: "rows" fp32 [M] for int8_gemm, "groups" quant_a's for int2_int8_gemm, "none"."""
-    _chk_norm(x, residual, weight, quant)
-    torch._check(norm or quant != "none", lambda: "nothing to compute: norm is false and quant 'none'")
+    _chk_norm(x, residual, weight, quant, norm)
     M, K = x.shape
     h, y, q, s = _norm_out(x, residual, quant, norm)
     if M:
@@ -421,14 +421,14 @@ def rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[
 
 @rmsnorm.register_fake
 def _(x, residual, weight, eps, woff, quant, norm):
-    _chk_norm(x, residual, weight, quant)
+    _chk_norm(x, residual, weight, quant, norm)
     return _norm_out(x, residual, quant, norm)
 
 
 @torch.library.custom_op("ternocl::quant_rows", mutates_args=())
 def quant_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q int8 [M, K], scales fp32 [M]) of x [M, K], x = q * scales[:, None]."""
-    _chk_norm(x, None, None, "rows")
+    _chk_norm(x, None, None, "rows", False)
     M, K = x.shape
     _, _, q, s = _norm_out(x, None, "rows", False)
     if M:
@@ -439,7 +439,7 @@ def quant_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 @quant_rows.register_fake
 def _(x):
-    _chk_norm(x, None, None, "rows")
+    _chk_norm(x, None, None, "rows", False)
     return _norm_out(x, None, "rows", False)[2:]
 
 

@@ -161,3 +161,10 @@ def test_int8_gemm_past_a_launch(M, N):
     assert L.ternocl_int8_gemm(0, 4096, 4096, 4096, 4096, 4096, None, None, M, N, 128, 0, 0, None, 0, None) == SHAPE
     assert L.ternocl_last_error().decode()
     assert T.kw_tile_of(4, M, N, 128) is None and T.int8_gemm_ws_bytes(M, N, 128) == 0
+
+
+def test_fake_refuses_nothing_to_compute():
+    """As the operator itself, so that a trace does not pass what a run refuses."""
+    import ternocl_amd.torch_ops  # noqa: F401
+    with pytest.raises(Exception, match="nothing to compute"):
+        torch.ops.ternocl.rmsnorm(meta(5, 256), None, None, 1e-6, 0.0, "none", False)
