@@ -523,7 +523,8 @@ ternocl_status ternocl_int4_unpack(const uint32_t *B, int8_t *W, int K, int N);
  * What comes before a layer's products (no reference counterpart): the residual's
  * addition, the root-mean-square norm and the activations in 8 bits, in one pass:
  *   h = x + r (R NULL: x),  n = h (woff + w) / sqrt(mean_k h^2 + eps)
- *   H = DT(h)   [M, K], may be X or R itself;  NULL: not written
+ *   H = DT(h)   [M, K], only with R; may be X or R itself where that has rows of K (M 1: any);
+ *               NULL: not written
  *   Y = DT(n)   [M, K];  NULL: not written
  *   quant 0: no codes (Q and SQ not written, Y non-null)
  *   quant 1: Q int8 [M, K], SQ fp32 [M]: a scale for each row, for ternocl_int8_gemm:

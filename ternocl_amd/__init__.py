@@ -493,9 +493,10 @@ _QUANTS = {"none": 0, "rows": 1, "groups": 2}
 def rmsnorm(X, R, W, H, Y, Q, SQ, M: int, K: int, eps: float = 1e-6, woff: float = 0.0, quant: str = "none", ldx=None,
             ldr=None, stream=None) -> None:
     """h = X + R (R None: X); H = h; n = h (woff + W) / sqrt(mean(h^2) + eps); Y = n; H and Y in X's dtype or
-    None, H may be X or R.  quant "rows": Q int8 [M, K] and SQ fp32 [M] with n = Q SQ, for ``int8_gemm``;
-    "groups": ``quant_a``'s SQ [K/128, ldsa(M)] and Q of Y, for ``int2_int8_gemm``; "none": neither.  W: [K]
-    fp16, bf16 or fp32, or None (a weight of 1); ldx, ldr: elements from row to row (K)."""
+    None, H only with R and may be X or R where that has rows of K.  quant "rows": Q int8 [M, K] and SQ fp32 [M]
+    with n = Q SQ, for ``int8_gemm``; "groups": ``quant_a``'s SQ [K/128, ldsa(M)] and Q of Y, for
+    ``int2_int8_gemm``; "none": neither.  W: [K] fp16, bf16 or fp32, or None (a weight of 1); ldx, ldr: elements
+    from row to row (K)."""
     if quant not in _QUANTS:
         raise TernoclError(1, f"quant must be 'none', 'rows' or 'groups', got {quant!r}")
     _check(lib().ternocl_rmsnorm(_dtype_of(X), _ptr(X), K if ldx is None else ldx, _ptr(R), K if ldr is None else ldr,

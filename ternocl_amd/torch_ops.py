@@ -407,7 +407,8 @@ def _norm_out(x, residual, quant, norm):
 def rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float, woff: float,
             quant: str, norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(h, y, q, scales) of x [M, K]: h = x + residual, y = rmsnorm(h) * (woff + weight) where norm asks for it, its
-    codes q int8 [M, K] and scales: "rows" fp32 [M] for int8_gemm, "groups" quant_a's for int2_int8_gemm, "none"."""
+    codes q int8 [M, K] and scales: "rows" fp32 [M] for int8_gemm, "groups" quant_a's for int2_int8_gemm, "none".
+    What is not asked for has no elements, h without a residual too."""
     _chk_norm(x, residual, weight, quant, norm)
     M, K = x.shape
     h, y, q, s = _norm_out(x, residual, quant, norm)

@@ -168,3 +168,14 @@ def test_fake_refuses_nothing_to_compute():
     import ternocl_amd.torch_ops  # noqa: F401
     with pytest.raises(Exception, match="nothing to compute"):
         torch.ops.ternocl.rmsnorm(meta(5, 256), None, None, 1e-6, 0.0, "none", False)
+
+
+@pytest.mark.parametrize("kw,word", [(dict(R=None), "R must be non-null"), (dict(H=4096, ldx=264), "rows of K"),
+                                     (dict(H=8192, ldr=264), "rows of K")])
+def test_rmsnorm_says_when_h_is_refused(kw, word):
+    """The sum with R only with R, and in place of X or R only where these have rows of K; the interface says both."""
+    from pathlib import Path
+    assert _norm(**kw) == INVALID
+    assert word in T.lib().ternocl_last_error().decode()
+    text = " ".join((Path(__file__).resolve().parents[1] / "include" / "ternocl_amd.h").read_text().replace("*", " ").split())
+    assert "H = DT(h) [M, K], only with R; may be X or R itself where that has rows of K" in text
