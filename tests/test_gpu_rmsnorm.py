@@ -329,3 +329,45 @@ def test_many_rows(dev, K):
                 assert torch.equal(H[i:i + 4].cpu(), h.float().bfloat16()) and near(Y[i:i + 4].cpu(), t * s, torch.bfloat16)
     want = codes_of(X[::1001].double().cpu())[0]
     assert torch.equal(Q[:M][::1001].cpu(), want)
+
+
+@pytest.mark.parametrize("K", [64, 77, 256, 4096, 36864])
+@pytest.mark.parametrize("off", [1, 2, 4, 7])
+@pytest.mark.parametrize("quant", ["rows", "groups"])
+def test_outputs_at_any_element(dev, K, off, quant):
+    """H, Y, codes, scales and weights that start `off` elements past a 16-byte boundary: the bits of aligned ones, and
+    nothing before or behind them written.  In the group case with an infinity and a NaN, whose scales are compared
+    bit for bit with quant_a's."""
+    import ternocl_amd as T
+    if K % 128:
+        quant = "rows"
+    M = 5
+    X, R, W, dt = make(K + off, M, K, True, True, torch.float32)
+    if quant == "groups":
+        X[1, 3], X[3, K - 1] = float("inf"), float("nan")
+    want = run(T, X, R, W, dt, quant, True)
+    bufs = []
+
+    def at(n, d):
+        bufs.append(torch.full((n + 32,), 7, dtype=d, device="cuda"))
+        return bufs[-1][off:off + n]
+
+    w = at(K, torch.float32)
+    w.copy_(W)
+    ns = M if quant == "rows" else K // 128 * T.ldsa(M)
+    got = [at(M * K, dt), at(M * K, dt), at(M * K, torch.int8), at(ns, torch.float32 if quant == "rows" else dt)]
+    T.rmsnorm(X, R, w, *got, M, K, quant=quant)
+    torch.cuda.synchronize()
+    bits = lambda t: t.contiguous().view(torch.uint8)
+    for g, x in zip(got[:3], want):
+        assert torch.equal(bits(g), bits(x).flatten())
+    if quant == "rows":
+        assert torch.equal(bits(got[3]), bits(want[3]))
+    else:
+        sa, q = torch.empty((K // 128, T.ldsa(M)), dtype=dt, device="cuda"), torch.empty((M, K), dtype=torch.int8, device="cuda")
+        T.quant_a(got[1].clone(), sa, q, M, K)
+        g = got[3].view(K // 128, T.ldsa(M))
+        assert torch.equal(bits(g[:, :M]), bits(sa[:, :M])) and torch.equal(got[2].view(M, K), q)
+        assert (g[:, M:] == 7).all()
+    for b, t in zip(bufs, [w] + got):
+        assert (b[:off] == 7).all() and (b[off + t.numel():] == 7).all()
