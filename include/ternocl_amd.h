@@ -558,7 +558,8 @@ ternocl_status ternocl_quant_rows(int dtype, const void *X, int64_t ldx, int8_t 
  * dtype: DT of Other, of C and Bias without out_f32.
  * N % 16 == 0, N <= 2^30 - 64, K % 128 == 0, K < 2^17, M >= 1 (up to 10^9: a launch holds 8 million
  * tiles of up to 128 x 512, and more are refused).  B starts on 16 bytes; operands that are not all
- * 16-byte aligned, and N > 2^26, run a plain kernel (several times slower).
+ * 16-byte aligned, and N > 2^26, run a plain kernel (5 times slower for few rows, 10 to 30 times for
+ * hundreds).
  * ws / ws_bytes: optional device scratch of ternocl_int8_gemm_ws_bytes(M, N, K) bytes (0:
  * none used), 16-byte aligned, laid out and used as ternocl_int2_fp16_upcvt_gemm's: a K
  * split of few tiles over a long K (the same bits as without).  Its counters take any

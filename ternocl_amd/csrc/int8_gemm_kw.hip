@@ -3,9 +3,9 @@
 //
 //   C[m,n] = ct(epi((sum_k A[m,k] B[k,n]) SB[n] SA[m])),  exact 32-bit sums
 //
-// Few rows are bound by the weights' stream (K N bytes; at 24 rows 48 operations a byte, a
-// hundredth of the matrix cores' rate).  So nothing stands between memory and the matrix cores:
-// 16 rows of a column lie together ([K/16][N][16]), so that a 16-byte load a lane is an operand
+// Few rows are bound by the weights' stream (K N bytes; at 24 rows 48 operations a byte, at 5 to 6
+// TB/s an eighth of the rate that a large product reaches).  So nothing stands between memory and
+// the matrix cores: 16 rows of a column lie together ([K/16][N][16]), so that a 16-byte load a lane is an operand
 // of v_mfma_i32_16x16x64_i8 (four runs of 256 bytes, wider strips longer ones), with no LDS, no
 // barrier and no instruction on the way.
 //   * A workgroup's waves split K and each streams its own part of a strip of columns, several
@@ -13,11 +13,13 @@
 //     the same bits whatever the split.
 //   * Columns are the instruction's rows: a lane ends with four adjacent outputs of a row, and
 //     loads what their epilogue reads before the walk.
-//   * Activations of up to 8 rows are loaded as fragments (lanes past the last row read its line
-//     again); of more, where a fragment load would touch a cache line a row, in whole lines
+//   * Activations of up to 8 rows may be loaded as fragments (lanes past the last row read its line
+//     again); of more, where a fragment load would touch a cache line a row, they go in whole lines
 //     through the wave's own LDS: 48 x 5120 x 5120 15.2 -> 11.4 us.
-// Captured, bf16, by box: 1 x 4096 x 4096 (16.8 MB) 4.4 to 5.1 us, 24 x 14336 x 4096 (58.7 MB, residual)
-// 11.2 to 11.5, 4 x 4096 x 151680 (621 MB, fp32 out) 104 to 111: 5.6 to 5.9 TB/s.
+// Captured, bf16, by card, weights used just before and in the last-level cache where they fit / weights
+// from HBM, as a model's next token finds them: 1 x 4096 x 4096 (16.8 MB) 4.4 to 5.2 us / 5.5, 24 x 14336 x
+// 4096 (58.7 MB, residual) 11.2 to 12.3 / 17.8, 4 x 4096 x 151680 (621 MB, fp32 out) 104 to 116: 5.3 to 5.9
+// TB/s.  Both the choice of tile and the cache policy below are fitted to the former.
 #include "int8_epi.hpp"
 
 #include <algorithm>
@@ -218,7 +220,8 @@ template <class T, bool BF16, bool NT> __global__ void __launch_bounds__(T::THRE
 
 // Weights of more than 100 MB, which the 256 MB cache cannot keep beside others, go past it: 1 x
 // 5120 x 34816 33.9 -> 31.8 us, 4 x 4096 x 151680 112 -> 104; smaller ones that are still there
-// from their last use are read faster: 24 x 14336 x 4096 15.7 -> 12.3 (from HBM 15.3 and 15.4).
+// from their last use are read faster: 24 x 14336 x 4096 without a residual 15.7 -> 12.3 (from HBM
+// 15.3 past it and 15.4).
 template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream_t st) {
     const long tiles = (long)((a.M + T::BM - 1) / T::BM) * ((a.N + T::BN - 1) / T::BN) * a.ksn;
     const bool nt = (long)a.K * a.N > 100000000;
@@ -238,9 +241,13 @@ template <class T> hipError_t i8_kw_launch(int dtype, const I8Args &a, hipStream
 //   memory  = weights / in + 2 outputs / out
 //   time    = base + (walk^4 + memory^4)^(1/4), with slices + arrive + each slices + sums slices
 //             outputs
-// Fitted (logarithms, least squares, one fit a tile) to some 300000 graph-timed calls on three sets
-// of operands, 11630 shapes of M = 1..4096, K = 256..14336, N = 64..151680: rms 5 to 11%; the tile
-// chosen by it is 1.3% behind the fastest of 21 on average (95 of 100 within 8%, the worst 41%).
+// Fitted (logarithms, least squares, one fit a tile) to 220000 graph-timed calls on three sets of
+// operands (weights up to some 85 MB: from the last-level cache), 11630 shapes of M = 1..4096, K =
+// 256..14336, N = 64..151680: rms 4 to 9%.  21 tiles were timed and these 14 kept: the choice is
+// 1.1% behind the fastest of them on average and 1.4% behind the fastest of all (95 of 100 within 8%,
+// the worst 41%).  With weights from HBM 9 to 64 rows take 20 to 45% longer than they were timed
+// at, and another tile may be ahead (32 x 4096 x 14336: 17.5 us, 32 x 64 tiles 14.8).  The second
+// tile's `out` is what the fit left: no call of up to 8 rows is bound by its outputs.
 // Narrow tiles fill the chip; wide ones read the activations, low ones the weights fewer times.
 enum I8Kind { kFew, kRows, kTile };  // activations as fragments (M <= 8), through a wave's LDS, int8_gemm_tile.hip
 struct I8Choice {

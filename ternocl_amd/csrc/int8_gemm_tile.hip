@@ -7,13 +7,15 @@
 // which spreads 16 rows over all banks, runs the same), and take the weights, each its own columns,
 // straight into fragments ([K/16][N][16]: 16 bytes a lane).  A stage is 128 rows of K: two LDS buffers, the next
 // stage stored in the middle of the current one, one barrier; one to four more stages of A are on
-// their way in registers (4096 x 5120 x 34816: one 720 us, two 698) and four to sixteen steps of
+// their way in registers (4096 x 5120 x 34816: one 720 us, two 698) and four or eight steps of
 // weights.
 //   * 128 x 512, eight waves side by side of 128 x 64: for each stage 2048 cycles of matrix
 //     instructions a SIMD, 1152 of LDS and 1280 of L1 a CU.  256 x 256 as four waves of 128 x 128
 //     840 us where this took 782, as eight waves 787.  4096 x 5120 x 34816 takes 642 to 697 us by
-//     box (2.1 to 2.3 10^15 operations a second; the library's int8 product 730, its 8192^3 one 2.13
-//     10^15): matrix cores busy 61% of the SIMDs' time at 1.75 GHz, the clock that power leaves.
+//     card (2.1 to 2.3 10^15 operations a second; the library's int8 product 730, its 8192^3 one 2.13
+//     10^15), bound by power: the same instructions on operands of zeros take 520 us at 2.21 GHz
+//     with the matrix cores busy 57% of the SIMDs' time, on normal ones 650 us at 1.5 to 1.75 GHz, busy
+//     61 to 62%, timed in turn.
 //   * Small tiles of tens to hundreds of rows are as long as their stages' latency (loads, LDS,
 //     barrier: some 0.4 us): groups of waves split K, each with its own buffers, and add their sums
 //     through LDS once (128 x 4096 x 4096 11.3 -> 8.4 us; what the epilogue reads loaded during the

@@ -1,7 +1,8 @@
 // int8_plain.hip -- products of 8-bit integers with a scale for each token and channel
 // (ternocl_int8_gemm) for operands that are not 16-byte aligned, which the matrix-core
 // engines load 16 bytes at a time: v_dot4 on a lane per column, kPlainRows rows of A per
-// pass over the weights.
+// pass over the weights.  bf16 with a bias off 16 bytes, plain / matrix cores: 8 x 4096 x 4096 27 / 6.1 us,
+// 200 x 5120 x 5120 163 / 16.6, 1024 x 4096 x 14336 1750 / 60.
 //
 //   C[m,n] = ct(epi(SA[m] SB[n] sum_k A[m,k] B[k,n]))
 #include "int8_epi.hpp"

@@ -8,9 +8,9 @@
 //   groups: quant_a of Y: SQ[g, m] = DT(127 / max(absmax, FLT_EPSILON)), q = sat(rne(Y SQ))
 //
 // Everything before a rounding to DT or to a code is 64-bit: x + r of two 16-bit values is
-// exact there, and a code is the one that the formula gives also where a quotient lies next
-// to a half (fp32 is off by up to 2^-15 of a step there).  gfx950 runs a 64-bit FMA at the
-// rate of an fp32 one.
+// exact there (bf16 ones some 45 binary orders apart: off by 2^-53), and a code is the one that
+// the formula gives also where a quotient lies next to a half (fp32 is off by up to 2^-15 of a step
+// there).  gfx950 runs a 64-bit FMA at the rate of an fp32 one.
 #include "common.hpp"
 
 #include <cfloat>
@@ -64,7 +64,8 @@ __device__ __forceinline__ RowStat wave_stat(RowStat s) {
 }
 
 // Rows of any length: a workgroup a row, which is read twice, a wave 128 elements at a time (a
-// scale group).
+// scale group), 2 bytes a lane.  Only for rows past 32768: 512 x 53248 bf16 codes 144 us where the
+// bytes take 17 at the rate of a large copy, with residual and norm 428 where they take 40.
 constexpr int kAnyWaves = 4;
 constexpr int kShort = 256;  // threads of a workgroup of short rows
 template <bool BF16, bool NORM> __global__ void __launch_bounds__(64 * kAnyWaves) k_rows_any(const NormArgs a) {
@@ -385,7 +386,10 @@ template <bool NORM> ternocl_status rows_launch(int dtype, const NormArgs &a, in
     // Vectors a thread: one where a call is as long as a row's latency (one row of 4096: 3.5 us,
     // with two 3.9), more where workgroups queue (8192 x 5120 rows of codes: one 86.6, two
     // 63.8, four 64.9; without a norm, where a thread holds half as much, 2047 x 14336: two
-    // 22.7, four 20.5).
+    // 22.7, four 20.5).  By rows, one / two, codes after a norm: of 4096 at 256 rows 4.9 / 5.1, 384
+    // 6.1 / 5.8, 512 6.9 / 6.6, 768 9.8 / 9.3; of 1024 at 512 4.3 / 4.5, 1024 4.6 / 4.8, 1536 6.0 / 5.7.  Without
+    // a norm 4096 at 256 3.6 / 3.8, 512 4.8 / 4.2; 14336, two / four: 512 9.8 / 10.1, 1024 14.2 / 14.1, 2048
+    // 22.2 / 20.0.
     int c = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
     if (a.M > 512) c = vecs > 2048 || (!NORM && vecs > 512) ? 4 : 2;
     const int nt = ((vecs + c - 1) / c + 63) / 64 * 64;
